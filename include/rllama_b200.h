@@ -44,6 +44,7 @@ typedef enum rlb_dtype {  /* TensorDType (src/tensor.rs:81-101) */
 
 typedef struct rlb_ctx rlb_ctx;        /* replaces `OpenCL`       (src/tensor_opencl_support.rs:30-37) */
 typedef struct rlb_tensor rlb_tensor;  /* replaces `OpenCLTensor` (src/tensor_opencl_support.rs:39-52) */
+typedef struct rlb_cache4 rlb_cache4;  /* a KV cache held in 4 bits (no counterpart in the reference)   */
 typedef struct rlb_event rlb_event;    /* replaces `OpenCLEvent`  (src/tensor_opencl_support.rs:54-57) */
 typedef struct rlb_model rlb_model;    /* `Transformer`           (src/transformer.rs:22-36)           */
 typedef struct rlb_caches rlb_caches;  /* `TransformerCaches`     (src/transformer.rs:111-113)         */
@@ -61,6 +62,12 @@ int rlb_device_count(int* count);
 /* OpenCL::new(verbose, nth_device) (src/tensor_opencl_support.rs:86-128). Selects the
  * nth CUDA device, checks that it is compute capability 10.x, creates the stream.     */
 int rlb_ctx_create(int verbose, int nth_device, rlb_ctx** out);
+/* A context whose work goes to the caller's stream (a cudaStream_t of that device; NULL is the
+ * legacy default stream), for hosts that mix the tier-1 ops with their own GPU work: the calls
+ * follow what the caller queued before and come before what is queued after. The stream must
+ * outlive the context and the caller's current device is left as it was. The ops say which of them
+ * may be captured into a CUDA graph. Models need a context of their own stream (RLB_ERR_STATE).  */
+int rlb_ctx_create_on_stream(int verbose, int nth_device, void* cuda_stream, rlb_ctx** out);
 int rlb_ctx_destroy(rlb_ctx* ctx);
 /* OpenCL::flush (src/tensor_opencl_support.rs:130-132): waits for all queued work.    */
 int rlb_ctx_flush(rlb_ctx* ctx);
@@ -76,6 +83,12 @@ int rlb_tensor_upload(rlb_ctx* ctx, const void* host, int64_t rows, int64_t cols
  * src/tensor.rs:1016-1021).                                                           */
 int rlb_tensor_zeros(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t capacity_cols,
                      rlb_dtype dtype, rlb_tensor** out);
+/* A tensor over memory that the caller owns and keeps alive (no copy; no counterpart in the
+ * reference): device memory of the context's device, 16-byte aligned, rows a multiple of 16 bytes
+ * apart. On a context with a stream of its own the caller orders its accesses itself, e.g. with
+ * rlb_tensor_wait, which waits for the context's stream here. rlb_tensor_free drops the view only. */
+int rlb_tensor_wrap(rlb_ctx* ctx, void* device, int64_t rows, int64_t cols, int64_t capacity_cols,
+                    rlb_dtype dtype, rlb_tensor** out);
 /* OpenCLTensor::wait_until_ready (src/tensor_opencl_support.rs:177-196).              */
 int rlb_tensor_wait(rlb_tensor* t);
 /* OpenCLTensor::data_u16_from_gpu (src/tensor_opencl_support.rs:198-212): asynchronous
@@ -133,6 +146,62 @@ int rlb_attention_prefill(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor
  * a device resolves the array's device address; make it before any stream capture.      */
 int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor* kcache, const rlb_tensor* vcache,
                                 int32_t heads, int32_t max_seq_len, int32_t pos, int32_t n_split);
+
+/* ------------------------------------------------------------------------------------
+ * Tier 1, long contexts: what lies between the q/k/v projection and wo, for caches in f16, f32
+ * or 4 bits, a sliding window with first tokens that stay visible, and K/V heads shared by
+ * heads / kv_heads query heads each (query head h reads K/V head h / (heads / kv_heads)).
+ * head_dim is 64 or 128. Rows may be padded (capacity_cols), caches may not. A call with no rows
+ * does nothing. On a context of the caller's stream these ops may be captured into a CUDA graph
+ * (rlb_cache4_create excepted): a graph then owns the scratch of its calls, so graphs may be
+ * replayed in any order and next to one another. The shapes, pointers and positions are fixed at
+ * the time of capture.
+ * ---------------------------------------------------------------------------------- */
+
+/* compute_freqs_cis (src/transformer.rs:858-885) as a tensor: max_seq_len x head_dim f32, row p
+ * holds (cos, sin) of p * 10000^(-2j/head_dim) for the pairs j = 0 .. head_dim/2-1.          */
+int rlb_rope_table(rlb_ctx* ctx, int32_t max_seq_len, int32_t head_dim, rlb_tensor** out);
+/* n rows of a projection's f32 output into attention: RMSNorm of every q and k head over
+ * head_dim (x / sqrt(mean(x^2) + eps) * gain; a null gain: none; src/transformer.rs:476-480),
+ * rotation of the pairs (2j, 2j+1) by the table's row of the position (src/transformer.rs:823-856),
+ * q to q_out (may be q itself), k and v rounded to the caches' dtype at positions start_pos ..
+ * start_pos+n-1 (:751-761).
+ *   q, q_out  n x (heads*head_dim) f32       k, v  n x (kv_heads*head_dim) f32
+ *   gains     1 x head_dim f32 or null       rope  at least start_pos+n rows
+ *   caches    (kv_heads*max_seq_len) x head_dim: row (h*max_seq_len + t), f16 or f32          */
+int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_tensor* vcache, const rlb_tensor* q, const rlb_tensor* k,
+                         const rlb_tensor* v, const rlb_tensor* q_gain, const rlb_tensor* k_gain, float eps, const rlb_tensor* rope,
+                         int32_t heads, int32_t kv_heads, int32_t max_seq_len, int32_t start_pos);
+/* Attention of n >= 1 query rows at positions start_pos .. start_pos+n-1 over f16 or f32 caches
+ * (the layout above): the row at position p sees t <= p with t > p - window or t < sinks. A
+ * window of max_seq_len or more is none. A row that sees nothing (window 0, no sinks) is zero;
+ * what unseen cache rows hold does not matter.
+ *   q    n x (heads*head_dim) f32, rotated
+ *   out  n x (heads*head_dim) in the cache dtype, not q                                     */
+int rlb_attention_window(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor* kcache, const rlb_tensor* vcache, int32_t heads,
+                         int32_t kv_heads, int32_t max_seq_len, int32_t start_pos, int32_t window, int32_t sinks);
+
+/* A KV cache in 4 bits (0.5625 bytes a value). Every 32 neighbouring values of a head's row
+ * share an f16 scale d; a value is d * u with a whole u, -7 <= u <= 7:
+ *   m = min(max |x|, 65504), d = f16(bf16(m * f32(1/7))), u = x / d to the nearest (ties to even).
+ * d has eight significant bits, so every value that the cache can hold is an f16 number. A NaN
+ * makes its group NaN. Storage, for K and for V: codes[kv_heads][max_seq_len][head_dim/2] bytes
+ * and scales[kv_heads][max_seq_len][head_dim/32] f16. A row's codes are 32-bit words; value e is in
+ * word (e % 32) / 8 * (head_dim/32) + e / 32, and nibble j < 4 of a word holds u + 8 of its value
+ * 2j, nibble j + 4 that of 2j + 1. Created caches hold zeros.                                 */
+int rlb_cache4_create(rlb_ctx* ctx, int32_t kv_heads, int32_t max_seq_len, int32_t head_dim, rlb_cache4** out);
+/* The same over the caller's device memory (16-byte aligned; kept alive by the caller).       */
+int rlb_cache4_wrap(rlb_ctx* ctx, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int32_t kv_heads, int32_t max_seq_len,
+                    int32_t head_dim, rlb_cache4** out);
+int rlb_cache4_free(rlb_cache4* c);
+/* Writes n rows of rotated k and v, n x (kv_heads*head_dim), both f32 or both f16, to positions
+ * start_pos .. start_pos+n-1.                                                                 */
+int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, int32_t start_pos);
+/* The values held at positions start_pos .. start_pos+n-1 as n x (kv_heads*head_dim) f16 or f32
+ * rows; either of k_out and v_out may be null. Exact in both dtypes.                          */
+int rlb_cache4_read(rlb_cache4* c, rlb_tensor* k_out, rlb_tensor* v_out, int32_t start_pos);
+/* rlb_attention_window over the values the cache holds; out is f16.                           */
+int rlb_cache4_attention(rlb_cache4* c, rlb_tensor* out, const rlb_tensor* q, int32_t heads, int32_t start_pos, int32_t window, int32_t sinks);
 
 /* ------------------------------------------------------------------------------------
  * Tier 2: the fused model-level path (what Transformer::forward becomes).

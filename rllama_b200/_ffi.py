@@ -16,10 +16,12 @@ F32, F16 = 0, 1
 # every symbol include/rllama_b200.h declares
 EXPORTS = [
     "rlb_last_error", "rlb_device_count",
-    "rlb_ctx_create", "rlb_ctx_destroy", "rlb_ctx_flush", "rlb_ctx_kernel_launches",
-    "rlb_tensor_upload", "rlb_tensor_zeros", "rlb_tensor_wait", "rlb_tensor_download", "rlb_event_wait", "rlb_tensor_free",
+    "rlb_ctx_create", "rlb_ctx_create_on_stream", "rlb_ctx_destroy", "rlb_ctx_flush", "rlb_ctx_kernel_launches",
+    "rlb_tensor_upload", "rlb_tensor_zeros", "rlb_tensor_wrap", "rlb_tensor_wait", "rlb_tensor_download", "rlb_event_wait", "rlb_tensor_free",
     "rlb_copy_inplace", "rlb_transpose_from", "rlb_hadamard_product_inplace", "rlb_silu_inplace",
     "rlb_matrix_mul_inplace_transposed", "rlb_attention_decode", "rlb_attention_decode_static", "rlb_attention_prefill",
+    "rlb_rope_table", "rlb_norm_rope_append", "rlb_attention_window",
+    "rlb_cache4_create", "rlb_cache4_wrap", "rlb_cache4_free", "rlb_cache4_append", "rlb_cache4_read", "rlb_cache4_attention",
     "rlb_model_create", "rlb_model_set_tensor", "rlb_model_finalize", "rlb_model_free",
     "rlb_tp_nccl_unique_id", "rlb_tp_nccl_init", "rlb_tp_peer_export", "rlb_tp_peer_import", "rlb_tp_peer_import_local", "rlb_tp_set_mode",
     "rlb_caches_create", "rlb_caches_true_clone", "rlb_caches_shift_left", "rlb_caches_free", "rlb_caches_read",
@@ -71,16 +73,22 @@ def lib():
     L.rlb_last_error.argtypes = []
     sig = {
         "rlb_device_count": [P(ci)],
-        "rlb_ctx_create": [ci, ci, P(vp)], "rlb_ctx_destroy": [vp], "rlb_ctx_flush": [vp],
+        "rlb_ctx_create": [ci, ci, P(vp)], "rlb_ctx_create_on_stream": [ci, ci, vp, P(vp)], "rlb_ctx_destroy": [vp], "rlb_ctx_flush": [vp],
         "rlb_ctx_kernel_launches": [vp, P(ctypes.c_uint64)],
         "rlb_tensor_upload": [vp, vp, i64, i64, i64, ci, P(vp)],
         "rlb_tensor_zeros": [vp, i64, i64, i64, ci, P(vp)],
+        "rlb_tensor_wrap": [vp, vp, i64, i64, i64, ci, P(vp)],
         "rlb_tensor_wait": [vp], "rlb_tensor_download": [vp, vp, P(vp)], "rlb_event_wait": [vp], "rlb_tensor_free": [vp],
         "rlb_copy_inplace": [vp, vp], "rlb_transpose_from": [vp, vp], "rlb_hadamard_product_inplace": [vp, vp],
         "rlb_silu_inplace": [vp], "rlb_matrix_mul_inplace_transposed": [vp, vp, vp],
         "rlb_attention_decode": [vp, vp, vp, vp, i32, i32, i32, i32],
         "rlb_attention_decode_static": [vp, vp, vp, vp, i32, i32, i32, i32],
         "rlb_attention_prefill": [vp, vp, vp, vp, i32, i32, i32, i32],
+        "rlb_rope_table": [vp, i32, i32, P(vp)],
+        "rlb_norm_rope_append": [vp] * 8 + [ctypes.c_float, vp, i32, i32, i32, i32],
+        "rlb_attention_window": [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32],
+        "rlb_cache4_create": [vp, i32, i32, i32, P(vp)], "rlb_cache4_wrap": [vp, vp, vp, vp, vp, i32, i32, i32, P(vp)], "rlb_cache4_free": [vp],
+        "rlb_cache4_append": [vp, vp, vp, i32], "rlb_cache4_read": [vp, vp, vp, i32], "rlb_cache4_attention": [vp, vp, vp, i32, i32, i32, i32],
         "rlb_model_create": [vp, P(ModelParams), P(vp)],
         "rlb_model_set_tensor": [vp, ci, i32, vp, i64, i64, i64, ci],
         "rlb_model_finalize": [vp], "rlb_model_free": [vp],

@@ -781,6 +781,8 @@ extern "C" int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q,
     rlb_ctx* ctx = out->ctx;
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
     RLB_CUDA(cudaSetDevice(ctx->device));
+    if (ctx_capturing(ctx))
+        return rlb_fail(RLB_ERR_STATE, "attention_decode_static cannot be captured into a graph on a borrowed stream: its scratch is shared by the process");
     float* base = nullptr;
     RLB_TRY(static_scratch_address(ctx->device, &base));
     // the arrival counters must start from zero on every call (an earlier call that was cut short may
@@ -793,6 +795,6 @@ extern "C" int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q,
     a.counters = reinterpret_cast<unsigned int*>(base + 64);
     a.scratch = base + kStaticHeaderFloats;
     RLB_TRY(launch_attn_decode(ctx, kcache->dtype, a, 0));
-    RLB_CUDA(cudaEventRecord(out->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(out));
     return RLB_OK;
 }

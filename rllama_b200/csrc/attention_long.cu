@@ -1,0 +1,222 @@
+// Attention for long contexts: a sliding window with first tokens that stay visible, K/V heads shared by several query
+// heads, and caches in f32, f16 or 4 bits (cache4.h). The per-head part of Attention::forward (src/transformer.rs:727-781)
+// with the visible set narrowed: query row i, at position p = start + i, sees
+//     t <= p  and  (t > p - window  or  t < sinks),
+// out_i = sum_t exp(s_t) v_t / sum_t exp(s_t), s_t = q . k_t / sqrt(head_dim), in f32 with the running maximum taken out.
+// A row that sees nothing (window 0 and no first tokens) is zero. Cache rows that a query row does not see never reach its
+// result, whatever they hold.
+//
+// The union of what the positions p0..p1 see is two runs, [0, S) and [L, p1 + 1) with L = max(0, p0 + 1 - window) and
+// S = min(sinks, L); kernels walk it as one virtual index v -> v < S ? v : v - S + L.
+#include "cache4.h"
+#include "internal.h"
+
+#include <algorithm>
+#include <cfloat>
+
+namespace {
+
+struct Run {
+    int s, l, len;  // first run [0, s), second [l, l + len - s)
+    __device__ __forceinline__ int at(int v) const { return v < s ? v : v - s + l; }
+};
+__device__ __forceinline__ int window_low(const AttnLongArgs& a, int p) { return max(0, p + 1 - a.window); }
+__device__ __forceinline__ Run visible_run(const AttnLongArgs& a, int p0, int p1) {
+    Run r;
+    r.l = window_low(a, p0);
+    r.s = min(a.sinks, r.l);
+    r.len = r.s + p1 + 1 - r.l;
+    return r;
+}
+__device__ __forceinline__ bool visible(const AttnLongArgs& a, int p, int t) { return t <= p && (t >= window_low(a, p) || t < a.sinks); }
+
+// HD / 32 neighbouring values of a cache row, as f32.
+template <int KIND, int HD> __device__ __forceinline__ void load_row(const void* base, const __half* scales, int64_t row, int lane, float (&x)[HD / 32]) {
+    constexpr int N = HD / 32;
+    if constexpr (KIND == CACHE_F32) {
+        const float* p = reinterpret_cast<const float*>(base) + row * HD + lane * N;
+        if constexpr (N == 4) { const float4 v = *reinterpret_cast<const float4*>(p); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+        else { const float2 v = *reinterpret_cast<const float2*>(p); x[0] = v.x; x[1] = v.y; }
+    } else {
+        __half2 h[N / 2];
+        if constexpr (KIND == CACHE_F16) {
+            const __half* p = reinterpret_cast<const __half*>(base) + row * HD + lane * N;
+            if constexpr (N == 4) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+            else *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            constexpr int G = HD / kQ4Group;
+            const int e = lane * N;
+            const uint32_t w = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(base) + row * (HD / 2))[q4_word(e, G)];
+            const __half2 d = __half2half2(scales[row * G + e / kQ4Group]);
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) h[j] = __hmul2(q4_pair(w, (e % 8) / 2 + j), d);
+        }
+#pragma unroll
+        for (int j = 0; j < N / 2; j++) {
+            const float2 f = __half22float2(h[j]);
+            x[2 * j] = f.x;
+            x[2 * j + 1] = f.y;
+        }
+    }
+}
+
+template <int KIND> struct Out { typedef __half T; };
+template <> struct Out<CACHE_F32> { typedef float T; };
+__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+
+// One query row: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
+template <int KIND, int HD>
+__global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a) {
+    constexpr int N = HD / 32;
+    __shared__ float w_o[8][HD], w_m[8], w_l[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = blockIdx.x;
+    const int i = (int)(r / a.heads), head = (int)(r % a.heads), p = a.start + i;
+    const Run run = visible_run(a, p, p);
+    const int chunk = (run.len + a.n_split - 1) / a.n_split;
+    const int v0 = min(run.len, (int)blockIdx.y * chunk), v1 = min(run.len, v0 + chunk);
+    const int64_t base = (int64_t)(head / a.group) * a.max_seq;
+    const float c2 = rsqrtf((float)HD) * 1.4426950408889634f;
+    float q[N], o[N] = {}, m = -FLT_MAX, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * c2;
+    for (int v = v0 + warp; v < v1; v += 8) {
+        const int64_t row = base + run.at(v);
+        float k[N], x[N];
+        load_row<KIND, HD>(a.k, a.k_scale, row, lane, k);
+        load_row<KIND, HD>(a.v, a.v_scale, row, lane, x);
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; e++) s = fmaf(q[e], k[e], s);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        const float m_new = fmaxf(m, s), w = exp2f(s - m_new), scale = exp2f(m - m_new);
+        l = l * scale + w;
+#pragma unroll
+        for (int e = 0; e < N; e++) o[e] = fmaf(o[e], scale, w * x[e]);
+        m = m_new;
+    }
+    if (lane == 0) { w_m[warp] = m; w_l[warp] = l; }
+#pragma unroll
+    for (int e = 0; e < N; e++) w_o[warp][lane * N + e] = o[e];
+    __syncthreads();
+    if (threadIdx.x >= HD) return;
+    float M = -FLT_MAX, L = 0.f, O = 0.f;
+    for (int w = 0; w < 8; w++) M = fmaxf(M, w_m[w]);
+    for (int w = 0; w < 8; w++) {
+        const float f = exp2f(w_m[w] - M);
+        L = fmaf(w_l[w], f, L);
+        O = fmaf(w_o[w][threadIdx.x], f, O);
+    }
+    if (a.n_split > 1) {
+        const int64_t rec = r * a.n_split + blockIdx.y;
+        a.rec_o[rec * HD + threadIdx.x] = O;
+        if (threadIdx.x == 0) a.rec_ml[rec] = make_float2(M, L);
+    } else {
+        store_out(reinterpret_cast<typename Out<KIND>::T*>(a.out) + i * a.out_ld + head * HD + threadIdx.x, run.len > 0 ? O / L : 0.f);
+    }
+}
+
+// Joins the splits of a row; a CTA of HD threads per row.
+template <typename OT>
+__global__ void __launch_bounds__(128) attn_long_merge_kernel(const AttnLongArgs a) {
+    const int64_t r = blockIdx.x;
+    const int i = (int)(r / a.heads), head = (int)(r % a.heads), p = a.start + i;
+    float M = -FLT_MAX, L = 0.f, O = 0.f;
+    for (int s = 0; s < a.n_split; s++) M = fmaxf(M, a.rec_ml[r * a.n_split + s].x);
+    for (int s = 0; s < a.n_split; s++) {
+        const float2 ml = a.rec_ml[r * a.n_split + s];
+        const float f = exp2f(ml.x - M);
+        L = fmaf(ml.y, f, L);
+        O = fmaf(a.rec_o[(r * a.n_split + s) * a.hd + threadIdx.x], f, O);
+    }
+    store_out(reinterpret_cast<OT*>(a.out) + i * a.out_ld + head * a.hd + threadIdx.x, visible_run(a, p, p).len > 0 ? O / L : 0.f);
+}
+
+template <int KIND, int HD>
+int launch_rows(rlb_ctx* ctx, AttnLongArgs a) {
+    const int64_t rows = (int64_t)a.n * a.heads;
+    // eight CTAs an SM, and at least 64 positions to a split
+    const int64_t most = std::min<int64_t>((int64_t)a.sinks + a.window, (int64_t)a.start + a.n);
+    int64_t splits = std::min<int64_t>((8 * ctx->sm_count + rows - 1) / rows, (most + 63) / 64);
+    a.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(splits, 256));
+    OpWorkspace ws;
+    if (a.n_split > 1) {
+        const size_t recs = (size_t)rows * a.n_split;
+        RLB_TRY(ws.get(ctx, recs * (HD * sizeof(float) + sizeof(float2))));
+        a.rec_ml = (float2*)ws.p;
+        a.rec_o = (float*)(a.rec_ml + recs);
+    }
+    attn_long_row_kernel<KIND, HD><<<dim3((unsigned)rows, a.n_split), 256, 0, ctx->stream>>>(a);
+    RLB_LAUNCH_CHECK();
+    count_launch(ctx);
+    if (a.n_split > 1) {
+        attn_long_merge_kernel<typename Out<KIND>::T><<<(unsigned)rows, HD, 0, ctx->stream>>>(a);
+        RLB_LAUNCH_CHECK();
+        count_launch(ctx);
+    }
+    return RLB_OK;
+}
+
+// What both entry points require of q, out and the visible set.
+int check(const char* who, const rlb_tensor* out, const rlb_tensor* q, rlb_dtype out_dtype, int32_t heads, int32_t kv_heads, int32_t max_seq,
+          int64_t hd, int32_t start, int32_t window, int32_t sinks) {
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return rlb_fail(RLB_ERR_INVALID, "%s: heads %d is not a multiple of kv_heads %d", who, heads, kv_heads);
+    if (hd != 64 && hd != 128) return rlb_fail(RLB_ERR_INVALID, "%s: head_dim %lld is not supported (64 or 128)", who, (long long)hd);
+    if (max_seq < 1 || start < 0 || start + q->rows > max_seq)
+        return rlb_fail(RLB_ERR_INVALID, "%s: bad max_seq_len %d, start_pos %d or %lld rows", who, max_seq, start, (long long)q->rows);
+    if (window < 0 || sinks < 0) return rlb_fail(RLB_ERR_INVALID, "%s: window %d and sinks %d must not be negative", who, window, sinks);
+    if (q->dtype != RLB_F32 || q->cols != heads * hd) return rlb_fail(RLB_ERR_INVALID, "%s: q must be n x heads*head_dim f32", who);
+    if (out->dtype != out_dtype || out->rows != q->rows || out->cols != q->cols)
+        return rlb_fail(RLB_ERR_INVALID, "%s: out must be n x heads*head_dim in %s", who, out_dtype == RLB_F16 ? "f16" : "f32");
+    if (out->d == q->d && q->rows > 0) return rlb_fail(RLB_ERR_INVALID, "%s: out and q are one tensor", who);
+    if (q->rows * heads > 0x7fffffffll) return rlb_fail(RLB_ERR_LIMIT, "%s: %lld rows of %d heads are more than one launch takes", who, (long long)q->rows, heads);
+    return RLB_OK;
+}
+
+int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, int32_t heads, int32_t kv_heads, int32_t max_seq, int64_t hd,
+        int32_t start, int32_t window, int32_t sinks) {
+    if (q->rows == 0) return RLB_OK;
+    rlb_ctx* ctx = out->ctx;
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
+    a.q = (const float*)q->d; a.q_ld = q->cap; a.out = out->d; a.out_ld = out->cap;
+    a.n = (int)q->rows; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.hd = (int)hd; a.max_seq = max_seq;
+    a.start = start; a.window = window; a.sinks = sinks;
+    RLB_TRY(launch_attn_long(ctx, kind, a));
+    return tensor_mark_ready(out);
+}
+
+}  // namespace
+
+int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+    if (a.hd == 128) return kind == CACHE_F32 ? launch_rows<CACHE_F32, 128>(ctx, a) : kind == CACHE_F16 ? launch_rows<CACHE_F16, 128>(ctx, a) : launch_rows<CACHE_Q4, 128>(ctx, a);
+    return kind == CACHE_F32 ? launch_rows<CACHE_F32, 64>(ctx, a) : kind == CACHE_F16 ? launch_rows<CACHE_F16, 64>(ctx, a) : launch_rows<CACHE_Q4, 64>(ctx, a);
+}
+
+extern "C" int rlb_attention_window(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor* kcache, const rlb_tensor* vcache, int32_t heads,
+                                    int32_t kv_heads, int32_t max_seq_len, int32_t start_pos, int32_t window, int32_t sinks) {
+    RLB_TRY(same_ctx(out, q));
+    RLB_TRY(same_ctx(out, kcache));
+    RLB_TRY(same_ctx(out, vcache));
+    const int64_t hd = kcache->cols;
+    RLB_TRY(check("attention_window", out, q, kcache->dtype, heads, kv_heads, max_seq_len, hd, start_pos, window, sinks));
+    if (kcache->cap != hd || vcache->cap != hd || vcache->cols != hd || kcache->rows != (int64_t)kv_heads * max_seq_len ||
+        vcache->rows != kcache->rows || kcache->dtype != vcache->dtype)
+        return rlb_fail(RLB_ERR_INVALID, "attention_window: caches must be (kv_heads*max_seq_len) x head_dim without row padding");
+    AttnLongArgs a;
+    a.k = kcache->d; a.v = vcache->d;
+    return run(kcache->dtype == RLB_F16 ? CACHE_F16 : CACHE_F32, a, out, q, heads, kv_heads, max_seq_len, hd, start_pos, window, sinks);
+}
+
+extern "C" int rlb_cache4_attention(rlb_cache4* c, rlb_tensor* out, const rlb_tensor* q, int32_t heads, int32_t start_pos, int32_t window, int32_t sinks) {
+    if (!c) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_attention: null cache");
+    RLB_TRY(same_ctx(out, q));
+    if (out->ctx != c->ctx) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_attention: the rows and the cache live on different contexts");
+    RLB_TRY(check("rlb_cache4_attention", out, q, RLB_F16, heads, c->kv_heads, c->max_seq, c->hd, start_pos, window, sinks));
+    AttnLongArgs a;
+    a.k = c->codes[0]; a.v = c->codes[1]; a.k_scale = c->scales[0]; a.v_scale = c->scales[1];
+    return run(CACHE_Q4, a, out, q, heads, c->kv_heads, c->max_seq, c->hd, start_pos, window, sinks);
+}

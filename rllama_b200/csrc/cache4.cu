@@ -1,0 +1,243 @@
+// The 4-bit cache (format: cache4.h): creation, appending rows and reading them back. What the reference keeps in f16 or
+// f32 per head (src/transformer.rs:129-160, the write loop :751-761) in 0.5625 bytes a value.
+#include "cache4.h"
+#include "internal.h"
+
+#include <new>
+
+namespace {
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(h[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+
+struct AppendArgs {
+    const void* src[2];  // K and V rows
+    int64_t ld[2];
+    uint8_t* codes[2];
+    __half* scales[2];
+    int kv_heads, max_seq, start;
+    int64_t count;       // n * kv_heads * hd / 8 threads for each of K and V
+};
+
+// A thread takes eight neighbouring values (one word of codes), four threads a group.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) append4_kernel(const AppendArgs a) {
+    constexpr int WORDS = HD / 8, GROUPS = HD / kQ4Group;
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int which = blockIdx.y;
+    const bool live = t < a.count;  // (count is a multiple of 8: a group's four threads are all live or none is)
+    const int64_t tt = live ? t : 0;
+    const int word = (int)(tt % WORDS);
+    const int64_t rh = tt / WORDS;
+    const int head = (int)(rh % a.kv_heads);
+    const int64_t i = rh / a.kv_heads;
+    float x[8];
+    load8<T>(reinterpret_cast<const T*>(a.src[which]) + i * a.ld[which] + (int64_t)head * HD + word * 8, x);
+    float m = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        m = fmaxf(m, fabsf(x[e]));
+        bad |= x[e] != x[e];
+    }
+    if (bad) m = __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, m, o);
+        m = (m != m || other != other) ? __int_as_float(0x7fc00000) : fmaxf(m, other);  // fmaxf alone would drop a NaN
+    }
+    const __half d = m != m ? __ushort_as_half(0x7fff) : q4_scale(m);
+    if (!live) return;
+    const int64_t row = (int64_t)head * a.max_seq + a.start + i;
+    const int group = word / 4, block = word % 4;
+    reinterpret_cast<uint32_t*>(a.codes[which] + row * (HD / 2))[block * GROUPS + group] = q4_pack(x, __half2float(d));
+    if (block == 0) a.scales[which][row * GROUPS + group] = d;
+}
+
+struct ReadArgs {
+    void* dst[2];
+    int64_t ld[2];
+    const uint8_t* codes[2];
+    const __half* scales[2];
+    int kv_heads, max_seq, start;
+    int64_t count;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) read4_kernel(const ReadArgs a) {
+    constexpr int WORDS = HD / 8, GROUPS = HD / kQ4Group;
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int which = blockIdx.y;
+    if (t >= a.count || a.dst[which] == nullptr) return;
+    const int word = (int)(t % WORDS);
+    const int64_t rh = t / WORDS;
+    const int head = (int)(rh % a.kv_heads);
+    const int64_t i = rh / a.kv_heads, row = (int64_t)head * a.max_seq + a.start + i;
+    const int group = word / 4, block = word % 4;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(a.codes[which] + row * (HD / 2))[block * GROUPS + group];
+    const __half2 d = __half2half2(a.scales[which][row * GROUPS + group]);
+    __half2 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = __hmul2(q4_pair(w, j), d);
+    T* dst = reinterpret_cast<T*>(a.dst[which]) + i * a.ld[which] + (int64_t)head * HD + word * 8;
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+    } else {
+        const float2 f0 = __half22float2(v[0]), f1 = __half22float2(v[1]), f2 = __half22float2(v[2]), f3 = __half22float2(v[3]);
+        *reinterpret_cast<float4*>(dst) = make_float4(f0.x, f0.y, f1.x, f1.y);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(f2.x, f2.y, f3.x, f3.y);
+    }
+}
+
+int check_dims(const char* who, int32_t kv_heads, int32_t max_seq_len, int32_t head_dim) {
+    if (kv_heads < 1 || max_seq_len < 1) return rlb_fail(RLB_ERR_INVALID, "%s: bad kv_heads %d or max_seq_len %d", who, kv_heads, max_seq_len);
+    if (head_dim != 64 && head_dim != 128) return rlb_fail(RLB_ERR_INVALID, "%s: head_dim %d is not supported (64 or 128)", who, head_dim);
+    return RLB_OK;
+}
+
+// Rows of K or V given to or taken from the cache at positions start .. start + rows - 1.
+int check_rows(const char* who, const rlb_cache4* c, const rlb_tensor* t, int64_t n, int32_t start) {
+    if (t->ctx != c->ctx) return rlb_fail(RLB_ERR_INVALID, "%s: the rows and the cache live on different contexts", who);
+    if (t->rows != n || t->cols != (int64_t)c->kv_heads * c->hd) return rlb_fail(RLB_ERR_INVALID, "%s: rows must be n x kv_heads*head_dim", who);
+    if (start < 0 || start + n > c->max_seq) return rlb_fail(RLB_ERR_INVALID, "%s: positions %d..%lld are outside the cache's %d", who, start, (long long)(start + n), c->max_seq);
+    return RLB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rlb_cache4_create(rlb_ctx* ctx, int32_t kv_heads, int32_t max_seq_len, int32_t head_dim, rlb_cache4** out) {
+    if (!ctx || !out) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_create: null pointer");
+    *out = nullptr;
+    RLB_TRY(check_dims("rlb_cache4_create", kv_heads, max_seq_len, head_dim));
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
+    if (ctx_capturing(ctx)) return rlb_fail(RLB_ERR_STATE, "rlb_cache4_create allocates: it cannot be captured into a graph");
+    const size_t rows = (size_t)kv_heads * max_seq_len;
+    const size_t codes = (rows * (head_dim / 2) + 255) & ~(size_t)255, scales = (rows * (head_dim / kQ4Group) * 2 + 255) & ~(size_t)255;
+    rlb_cache4* c = new (std::nothrow) rlb_cache4();
+    if (!c) return rlb_fail(RLB_ERR_OOM, "rlb_cache4_create: out of host memory");
+    cudaError_t e = cudaMalloc(&c->owned, 2 * (codes + scales));
+    if (e != cudaSuccess) {
+        delete c;
+        cudaGetLastError();
+        return rlb_fail(RLB_ERR_OOM, "rlb_cache4_create: cudaMalloc(%zu): %s", 2 * (codes + scales), cudaGetErrorString(e));
+    }
+    e = cudaMemsetAsync(c->owned, 0, 2 * (codes + scales), ctx->stream);  // scale 0: every value is zero
+    if (e != cudaSuccess) {
+        cudaFree(c->owned);
+        delete c;
+        return rlb_fail(RLB_ERR_CUDA, "rlb_cache4_create: %s", cudaGetErrorString(e));
+    }
+    uint8_t* p = (uint8_t*)c->owned;
+    c->codes[0] = p; c->codes[1] = p + codes;
+    c->scales[0] = (__half*)(p + 2 * codes); c->scales[1] = (__half*)(p + 2 * codes + scales);
+    c->ctx = ctx; c->device = ctx->device; c->kv_heads = kv_heads; c->max_seq = max_seq_len; c->hd = head_dim;
+    *out = c;
+    return RLB_OK;
+}
+
+int rlb_cache4_wrap(rlb_ctx* ctx, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int32_t kv_heads, int32_t max_seq_len,
+                    int32_t head_dim, rlb_cache4** out) {
+    if (!ctx || !out) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_wrap: null pointer");
+    *out = nullptr;
+    RLB_TRY(check_dims("rlb_cache4_wrap", kv_heads, max_seq_len, head_dim));
+    for (const void* p : {k_codes, k_scales, v_codes, v_scales}) {
+        if (!p || ((uintptr_t)p & 15)) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_wrap: the four arrays must be 16-byte aligned");
+        RLB_TRY(check_device_memory(ctx, p, "rlb_cache4_wrap"));
+    }
+    rlb_cache4* c = new (std::nothrow) rlb_cache4();
+    if (!c) return rlb_fail(RLB_ERR_OOM, "rlb_cache4_wrap: out of host memory");
+    c->codes[0] = (uint8_t*)k_codes; c->codes[1] = (uint8_t*)v_codes;
+    c->scales[0] = (__half*)k_scales; c->scales[1] = (__half*)v_scales;
+    c->ctx = ctx; c->device = ctx->device; c->kv_heads = kv_heads; c->max_seq = max_seq_len; c->hd = head_dim;
+    *out = c;
+    return RLB_OK;
+}
+
+int rlb_cache4_free(rlb_cache4* c) {
+    if (!c) return RLB_OK;
+    if (c->owned) {
+        DeviceScope dev(c->device);
+        cudaFree(c->owned);  // waits for the device
+    }
+    delete c;
+    return RLB_OK;
+}
+
+int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, int32_t start_pos) {
+    if (!c || !k || !v) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_append: null pointer");
+    RLB_TRY(check_rows("rlb_cache4_append", c, k, k->rows, start_pos));
+    RLB_TRY(check_rows("rlb_cache4_append", c, v, k->rows, start_pos));
+    if (k->dtype != v->dtype) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_append: K and V rows must have one dtype");
+    if (k->rows == 0) return RLB_OK;
+    rlb_ctx* ctx = c->ctx;
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
+    AppendArgs a;
+    a.src[0] = k->d; a.src[1] = v->d; a.ld[0] = k->cap; a.ld[1] = v->cap;
+    for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
+    a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos;
+    a.count = k->rows * c->kv_heads * (c->hd / 8);
+    const dim3 grid((unsigned)((a.count + 255) / 256), 2);
+    if (k->dtype == RLB_F16) {
+        if (c->hd == 128) append4_kernel<__half, 128><<<grid, 256, 0, ctx->stream>>>(a);
+        else append4_kernel<__half, 64><<<grid, 256, 0, ctx->stream>>>(a);
+    } else {
+        if (c->hd == 128) append4_kernel<float, 128><<<grid, 256, 0, ctx->stream>>>(a);
+        else append4_kernel<float, 64><<<grid, 256, 0, ctx->stream>>>(a);
+    }
+    RLB_LAUNCH_CHECK();
+    count_launch(ctx);
+    return RLB_OK;
+}
+
+int rlb_cache4_read(rlb_cache4* c, rlb_tensor* k_out, rlb_tensor* v_out, int32_t start_pos) {
+    if (!c || (!k_out && !v_out)) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_read: null pointer");
+    const rlb_tensor* any = k_out ? k_out : v_out;
+    if (k_out) RLB_TRY(check_rows("rlb_cache4_read", c, k_out, any->rows, start_pos));
+    if (v_out) RLB_TRY(check_rows("rlb_cache4_read", c, v_out, any->rows, start_pos));
+    if (k_out && v_out && k_out->dtype != v_out->dtype) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_read: K and V rows must have one dtype");
+    if (any->rows == 0) return RLB_OK;
+    rlb_ctx* ctx = c->ctx;
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
+    ReadArgs a;
+    a.dst[0] = k_out ? k_out->d : nullptr; a.dst[1] = v_out ? v_out->d : nullptr;
+    a.ld[0] = k_out ? k_out->cap : 0; a.ld[1] = v_out ? v_out->cap : 0;
+    for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
+    a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos;
+    a.count = any->rows * c->kv_heads * (c->hd / 8);
+    const dim3 grid((unsigned)((a.count + 255) / 256), 2);
+    if (any->dtype == RLB_F16) {
+        if (c->hd == 128) read4_kernel<__half, 128><<<grid, 256, 0, ctx->stream>>>(a);
+        else read4_kernel<__half, 64><<<grid, 256, 0, ctx->stream>>>(a);
+    } else {
+        if (c->hd == 128) read4_kernel<float, 128><<<grid, 256, 0, ctx->stream>>>(a);
+        else read4_kernel<float, 64><<<grid, 256, 0, ctx->stream>>>(a);
+    }
+    RLB_LAUNCH_CHECK();
+    count_launch(ctx);
+    if (k_out) RLB_TRY(tensor_mark_ready(k_out));
+    if (v_out) RLB_TRY(tensor_mark_ready(v_out));
+    return RLB_OK;
+}
+
+}  // extern "C"

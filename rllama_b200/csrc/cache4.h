@@ -1,0 +1,50 @@
+// The 4-bit cache format.
+//
+// Per K or V row (one K/V head, one position, hd = 64 or 128 values) and per group of 32 neighbouring values there is one
+// f16 scale d and 32 codes u of 4 bits, -7 <= u <= 7; the value is d * u. With m the group's largest magnitude (at most
+// 65504), d = f16(bf16(m * f32(1/7))) and u = x / d rounded to the nearest integer (ties to even), clamped to 7. The
+// detour over bf16 leaves d eight significant bits; u has three, so d * u has at most eleven: every value that the cache
+// holds IS an f16 number, and the f16 tensor-core operands made from it carry no rounding of their own. The price is at
+// most 2^-9 of the step. A group of zeros (or of magnitudes below the smallest scale) has d = 0; a group holding a NaN
+// has d = NaN, so all of it reads back as NaN; infinities count as +-65504.
+//
+// Codes are stored as nibbles u + 8 in 32-bit words of eight neighbouring values. Inside a word, nibble j < 4 holds value
+// 2j and nibble j + 4 value 2j + 1, so one shift and one mask give a pair of neighbours in the two halves of a register.
+// The words of a row are ordered [block of eight inside the group][group]: word (e % 32) / 8 * (hd / 32) + e / 32 holds
+// value e. Four threads that read a quarter of the row each then hold the same share of every group, which is how a
+// tensor-core fragment wants its contraction index (four threads share one) with the group's scale factored out.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+constexpr int kQ4Group = 32;
+
+#ifdef __CUDACC__
+// The pair of values 2j, 2j + 1 of a word, without their scale: exact small integers.
+__device__ __forceinline__ __half2 q4_pair(uint32_t word, int j) {
+    const uint32_t t = ((word >> (4 * j)) & 0x000F000Fu) | 0x64006400u;  // 1024 + nibble: the nibble is the mantissa's low end
+    const uint32_t bias = 0x64086408u;                                   // 1032
+    return __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&bias));
+}
+__host__ __device__ __forceinline__ int q4_word(int e, int groups) { return (e % kQ4Group) / 8 * groups + e / kQ4Group; }
+
+// Scale of a group whose largest magnitude is m.
+__device__ __forceinline__ __half q4_scale(float m) {
+    return __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fmul_rn(fminf(m, 65504.f), 1.0f / 7.0f))));
+}
+// Nibble of x under the scale d.
+__device__ __forceinline__ uint32_t q4_code(float x, float d) {
+    if (!(d > 0.f)) return 8u;
+    return (uint32_t)((int)rintf(fminf(fmaxf(__fdiv_rn(x, d), -7.f), 7.f)) + 8);
+}
+// Eight values into a word.
+__device__ __forceinline__ uint32_t q4_pack(const float (&x)[8], float d) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w |= q4_code(x[e], d) << (4 * ((e >> 1) + (e & 1) * 4));
+    return w;
+}
+#endif

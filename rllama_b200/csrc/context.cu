@@ -6,6 +6,7 @@
 
 #include <cstdarg>
 #include <cstring>
+#include <new>
 
 namespace {
 thread_local char g_err[1024] = "";
@@ -25,6 +26,61 @@ int ctx_check_error_word(rlb_ctx* ctx) {
     return RLB_OK;
 }
 
+int same_ctx(const rlb_tensor* a, const rlb_tensor* b) {
+    if (!a || !b) return rlb_fail(RLB_ERR_INVALID, "null tensor");
+    if (a->ctx != b->ctx) return rlb_fail(RLB_ERR_INVALID, "tensors live on different contexts");
+    return RLB_OK;
+}
+
+bool ctx_capturing(const rlb_ctx* ctx) {
+    if (!ctx->borrowed_stream) return false;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(ctx->stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
+int tensor_mark_ready(rlb_tensor* t) {
+    if (!t->ready || ctx_capturing(t->ctx)) return RLB_OK;
+    RLB_CUDA(cudaEventRecord(t->ready, t->ctx->stream));
+    return RLB_OK;
+}
+
+int check_device_memory(const rlb_ctx* ctx, const void* p, const char* who) {
+    cudaPointerAttributes at;
+    cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return rlb_fail(RLB_ERR_INVALID, "%s: %s", who, cudaGetErrorString(e));
+    }
+    if (at.type != cudaMemoryTypeDevice || at.device != ctx->device)
+        return rlb_fail(RLB_ERR_INVALID, "%s: the pointer is not memory of device %d", who, ctx->device);
+    return RLB_OK;
+}
+
+int OpWorkspace::get(rlb_ctx* c, size_t bytes) {
+    ctx = c;
+    if (ctx_capturing(c)) {
+        cudaError_t e = cudaMallocAsync(&p, bytes, c->stream);
+        if (e != cudaSuccess) { p = nullptr; return rlb_fail(RLB_ERR_OOM, "scratch inside a graph (%zu bytes): %s", bytes, cudaGetErrorString(e)); }
+        in_graph = true;
+        return RLB_OK;
+    }
+    if (bytes > c->op_scratch_bytes) {
+        RLB_CUDA(cudaStreamSynchronize(c->stream));
+        if (c->op_scratch) cudaFree(c->op_scratch);
+        c->op_scratch = nullptr;
+        c->op_scratch_bytes = 0;
+        cudaError_t e = cudaMalloc(&c->op_scratch, bytes);
+        if (e != cudaSuccess) { c->op_scratch = nullptr; return rlb_fail(RLB_ERR_OOM, "scratch (%zu bytes): %s", bytes, cudaGetErrorString(e)); }
+        c->op_scratch_bytes = bytes;
+    }
+    p = c->op_scratch;
+    return RLB_OK;
+}
+
+OpWorkspace::~OpWorkspace() {
+    if (in_graph && p) cudaFreeAsync(p, ctx->stream);
+}
+
 extern "C" {
 
 const char* rlb_last_error(void) { return g_err; }
@@ -41,7 +97,7 @@ int rlb_device_count(int* count) {
     return RLB_OK;
 }
 
-int rlb_ctx_create(int verbose, int nth_device, rlb_ctx** out) {
+static int ctx_new(int verbose, int nth_device, bool borrow, cudaStream_t stream, rlb_ctx** out) {
     if (!out) return rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create: null out pointer");
     *out = nullptr;
     int n = 0;
@@ -67,20 +123,47 @@ int rlb_ctx_create(int verbose, int nth_device, rlb_ctx** out) {
     ctx->device = nth_device;
     ctx->sm_count = prop.multiProcessorCount;
     ctx->verbose = verbose != 0;
-    cudaError_t se = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
+    ctx->borrowed_stream = borrow;
+    ctx->stream = stream;
+    cudaError_t se = borrow ? cudaSuccess : cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
     if (se == cudaSuccess) se = cudaHostAlloc((void**)&ctx->h_err, 64, cudaHostAllocMapped);
     if (se == cudaSuccess) {
         *ctx->h_err = 0;
         se = cudaHostGetDevicePointer((void**)&ctx->d_err, ctx->h_err, 0);
     }
     if (se != cudaSuccess) {
-        if (ctx->stream) cudaStreamDestroy(ctx->stream);
+        if (ctx->stream && !borrow) cudaStreamDestroy(ctx->stream);
         if (ctx->h_err) cudaFreeHost(ctx->h_err);
         delete ctx;
         return rlb_fail(RLB_ERR_CUDA, "context set-up: %s", cudaGetErrorString(se));
     }
     *out = ctx;
     return RLB_OK;
+}
+
+int rlb_ctx_create(int verbose, int nth_device, rlb_ctx** out) { return ctx_new(verbose, nth_device, false, nullptr, out); }
+
+int rlb_ctx_create_on_stream(int verbose, int nth_device, void* cuda_stream, rlb_ctx** out) {
+    if (!out) return rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create_on_stream: null out pointer");
+    *out = nullptr;
+    cudaStream_t s = (cudaStream_t)cuda_stream;
+    int before = -1;
+    cudaGetDevice(&before);  // the caller's device stays current: it is the caller's stream that is used
+    int status = ctx_new(verbose, nth_device, true, s, out);
+    // (the legacy and the per-thread default stream belong to whatever device is current: nothing to compare)
+    if (status == RLB_OK && s != nullptr && s != cudaStreamLegacy && s != cudaStreamPerThread) {
+        int dev = -1;
+        cudaError_t e = cudaStreamGetDevice(s, &dev);
+        if (e != cudaSuccess) status = rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create_on_stream: not a stream: %s", cudaGetErrorString(e));
+        else if (dev != nth_device) status = rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create_on_stream: the stream belongs to device %d, not %d", dev, nth_device);
+        if (status != RLB_OK) {
+            cudaFreeHost((*out)->h_err);
+            delete *out;
+            *out = nullptr;
+        }
+    }
+    if (before >= 0) cudaSetDevice(before);
+    return status;
 }
 
 int rlb_ctx_destroy(rlb_ctx* ctx) {
@@ -90,7 +173,7 @@ int rlb_ctx_destroy(rlb_ctx* ctx) {
     if (ctx->op_scratch) cudaFree(ctx->op_scratch);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
     if (ctx->h_err) cudaFreeHost(ctx->h_err);
-    cudaStreamDestroy(ctx->stream);
+    if (!ctx->borrowed_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return RLB_OK;
 }
@@ -167,9 +250,26 @@ int rlb_tensor_zeros(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t capacity_
     return RLB_OK;
 }
 
+int rlb_tensor_wrap(rlb_ctx* ctx, void* device, int64_t rows, int64_t cols, int64_t capacity_cols, rlb_dtype dtype, rlb_tensor** out) {
+    if (!ctx || !out) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wrap: null pointer");
+    *out = nullptr;
+    if (rows < 0 || cols < 0 || capacity_cols < cols || (dtype != RLB_F16 && dtype != RLB_F32))
+        return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wrap: bad shape %lldx%lld (capacity %lld) or dtype %d", (long long)rows, (long long)cols,
+                        (long long)capacity_cols, (int)dtype);
+    if (((uintptr_t)device & 15) || (capacity_cols * (int64_t)dtype_size(dtype)) % 16 != 0)
+        return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wrap: the memory and its rows (capacity_cols %lld) must be 16-byte aligned", (long long)capacity_cols);
+    if (rows > 0 && cols > 0) RLB_TRY(check_device_memory(ctx, device, "rlb_tensor_wrap"));
+    rlb_tensor* t = new (std::nothrow) rlb_tensor();
+    if (!t) return rlb_fail(RLB_ERR_OOM, "rlb_tensor_wrap: out of host memory");
+    t->ctx = ctx; t->d = device; t->rows = rows; t->cols = cols; t->cap = capacity_cols; t->dtype = dtype; t->wrapped = true;
+    *out = t;
+    return RLB_OK;
+}
+
 int rlb_tensor_wait(rlb_tensor* t) {
     if (!t) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wait: null tensor");
-    RLB_CUDA(cudaEventSynchronize(t->ready));
+    if (t->ready) RLB_CUDA(cudaEventSynchronize(t->ready));
+    else RLB_CUDA(cudaStreamSynchronize(t->ctx->stream));
     return ctx_check_error_word(t->ctx);
 }
 
@@ -181,7 +281,13 @@ int rlb_tensor_download(rlb_tensor* t, void* host, rlb_event** out_event) {
     rlb_event* ev = new rlb_event();
     ev->ctx = ctx;
     cudaError_t e = cudaEventCreateWithFlags(&ev->ev, cudaEventDisableTiming);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(host, t->d, t->bytes(), cudaMemcpyDeviceToHost, ctx->stream);
+    if (e == cudaSuccess && t->wrapped) {  // what lies between the columns and capacity_cols is not the tensor's
+        const size_t es = dtype_size(t->dtype), pitch = (size_t)t->cap * es;
+        if (t->rows > 0 && t->cols > 0)
+            e = cudaMemcpy2DAsync(host, pitch, t->d, pitch, (size_t)t->cols * es, (size_t)t->rows, cudaMemcpyDeviceToHost, ctx->stream);
+    } else if (e == cudaSuccess) {
+        e = cudaMemcpyAsync(host, t->d, t->bytes(), cudaMemcpyDeviceToHost, ctx->stream);
+    }
     if (e == cudaSuccess) e = cudaEventRecord(ev->ev, ctx->stream);
     if (e != cudaSuccess) {
         if (ev->ev) cudaEventDestroy(ev->ev);
@@ -204,6 +310,10 @@ int rlb_event_wait(rlb_event* ev) {
 
 int rlb_tensor_free(rlb_tensor* t) {
     if (!t) return RLB_OK;
+    if (t->wrapped) {  // the caller's memory: nothing to wait for
+        delete t;
+        return RLB_OK;
+    }
     cudaSetDevice(t->ctx->device);
     if (t->ready) {
         cudaEventSynchronize(t->ready);  // the reference also waits for the initial write before dropping
@@ -214,9 +324,10 @@ int rlb_tensor_free(rlb_tensor* t) {
     return RLB_OK;
 }
 
-static int same_ctx(const rlb_tensor* a, const rlb_tensor* b) {
-    if (!a || !b) return rlb_fail(RLB_ERR_INVALID, "null tensor");
-    if (a->ctx != b->ctx) return rlb_fail(RLB_ERR_INVALID, "tensors live on different contexts");
+// Ops whose scratch belongs to the context: a captured copy of them would go on using scratch that the context may have
+// replaced since, or that another graph uses at the same time.
+static int refuse_capture(const rlb_ctx* ctx, const char* op) {
+    if (ctx_capturing(ctx)) return rlb_fail(RLB_ERR_STATE, "%s cannot be captured into a graph: its scratch belongs to the context", op);
     return RLB_OK;
 }
 
@@ -232,7 +343,7 @@ int rlb_copy_inplace(rlb_tensor* dst, const rlb_tensor* src) {
     OP_PROLOGUE(ctx, dst);
     RLB_CUDA(cudaMemcpy2DAsync(dst->d, dst->cap * dtype_size(dst->dtype), src->d, src->cap * dtype_size(src->dtype),
                                (size_t)src->cols * dtype_size(src->dtype), (size_t)src->rows, cudaMemcpyDeviceToDevice, ctx->stream));
-    RLB_CUDA(cudaEventRecord(dst->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(dst));
     return RLB_OK;
 }
 
@@ -243,7 +354,7 @@ int rlb_transpose_from(rlb_tensor* dst, const rlb_tensor* src) {
                         (long long)dst->cols, (long long)src->rows, (long long)src->cols);
     OP_PROLOGUE(ctx, dst);
     RLB_TRY(launch_transpose(ctx, dst->d, src->d, dst->dtype, dst->rows, dst->cols, dst->cap, src->cap));
-    RLB_CUDA(cudaEventRecord(dst->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(dst));
     return RLB_OK;
 }
 
@@ -253,7 +364,7 @@ int rlb_hadamard_product_inplace(rlb_tensor* dst, const rlb_tensor* other) {
         return rlb_fail(RLB_ERR_INVALID, "hadamard_product_inplace: shape or dtype mismatch");
     OP_PROLOGUE(ctx, dst);
     RLB_TRY(launch_hadamard(ctx, dst->d, other->d, dst->dtype, dst->rows, dst->cols, dst->cap, other->cap));
-    RLB_CUDA(cudaEventRecord(dst->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(dst));
     return RLB_OK;
 }
 
@@ -261,7 +372,7 @@ int rlb_silu_inplace(rlb_tensor* t) {
     if (!t) return rlb_fail(RLB_ERR_INVALID, "silu_inplace: null tensor");
     OP_PROLOGUE(ctx, t);
     RLB_TRY(launch_silu(ctx, t->d, t->dtype, t->rows, t->cols, t->cap));
-    RLB_CUDA(cudaEventRecord(t->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(t));
     return RLB_OK;
 }
 
@@ -276,11 +387,13 @@ int rlb_matrix_mul_inplace_transposed(rlb_tensor* dst, const rlb_tensor* src, co
     if (dst->rows != src->rows) return rlb_fail(RLB_ERR_INVALID, "Invalid matrix multiplication, different number of rows");
     if (dst->cols != other->rows) return rlb_fail(RLB_ERR_INVALID, "Invalid matrix multiplication, different number of cols");
     OP_PROLOGUE(ctx, dst);
+    RLB_TRY(refuse_capture(ctx, "matrix_mul_inplace_transposed"));
     const int vec = dst->dtype == RLB_F16 ? 8 : 4;
     // Rows are zero padded up to capacity_cols (src/tensor.rs:433-450), so the contraction may
     // run over the padded length.
     const int64_t kp = (src->cols + vec - 1) / vec * vec;
-    const bool padded_ok = kp <= src->cap && kp <= other->cap;
+    // (a wrapped tensor's row may be followed by anything: its contraction stops at its columns)
+    const bool padded_ok = kp <= src->cap && kp <= other->cap && (kp == src->cols || !(src->wrapped || other->wrapped));
     if (src->rows == 1 && padded_ok && other->rows > 0) {
         GemvArgs a;
         a.W = other->d; a.rows = (int)other->rows; a.K = (int)kp; a.ldw = other->cap;
@@ -295,7 +408,7 @@ int rlb_matrix_mul_inplace_transposed(rlb_tensor* dst, const rlb_tensor* src, co
         RLB_TRY(launch_gemm_nt_typed(ctx, dst->dtype, src->d, src->cap, other->d, other->cap, dst->d, dst->cap, (int)src->rows,
                                      (int)other->rows, (int)src->cols));
     }
-    RLB_CUDA(cudaEventRecord(dst->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(dst));
     return RLB_OK;
 }
 
@@ -325,6 +438,7 @@ extern "C" int rlb_attention_decode(rlb_tensor* out, const rlb_tensor* q, const 
     int hd = 0;
     RLB_TRY(attention_check(out, q, kcache, vcache, heads, max_seq_len, pos, n_split, &hd));
     OP_PROLOGUE(ctx, out);
+    RLB_TRY(refuse_capture(ctx, "attention_decode"));
     // scratch: [pos : 256 B][counters : heads, padded to 256 B][records]
     const size_t cnt_bytes = ((size_t)heads * sizeof(unsigned int) + 255) & ~(size_t)255;
     const size_t need = 256 + cnt_bytes + attn_decode_scratch_floats(heads, hd, n_split) * sizeof(float);
@@ -346,7 +460,7 @@ extern "C" int rlb_attention_decode(rlb_tensor* out, const rlb_tensor* q, const 
     a.counters = (unsigned int*)(base + 256);
     a.scratch = (float*)(base + 256 + cnt_bytes);
     RLB_TRY(launch_attn_decode(ctx, kcache->dtype, a, 0));
-    RLB_CUDA(cudaEventRecord(out->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(out));
     return RLB_OK;
 }
 
@@ -373,6 +487,6 @@ extern "C" int rlb_attention_prefill(rlb_tensor* out, const rlb_tensor* q, const
     a.n = (int)n; a.start_pos = start_pos; a.heads = heads; a.hd = (int)hd; a.max_seq = max_seq_len;
     a.allow_tc = tensor_cores != 0;
     RLB_TRY(launch_attn_prefill(ctx, kcache->dtype, a));
-    RLB_CUDA(cudaEventRecord(out->ready, ctx->stream));
+    RLB_TRY(tensor_mark_ready(out));
     return RLB_OK;
 }

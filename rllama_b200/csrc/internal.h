@@ -42,6 +42,7 @@ struct rlb_ctx {
     int sm_count = 0;
     bool verbose = false;
     cudaStream_t stream = nullptr;
+    bool borrowed_stream = false;  // the stream is the caller's (rlb_ctx_create_on_stream): never destroyed here, may be under capture
     std::recursive_mutex mu;
     uint64_t launches = 0;  // kernels launched by this library on this context
     void* op_scratch = nullptr;  // scratch of the standalone attention op, grown on demand
@@ -64,8 +65,42 @@ struct rlb_tensor {
     void* d = nullptr;
     int64_t rows = 0, cols = 0, cap = 0;
     rlb_dtype dtype = RLB_F32;
-    cudaEvent_t ready = nullptr;  // last operation queued on this tensor
+    cudaEvent_t ready = nullptr;  // last operation queued on this tensor (a wrapped tensor has none: see tensor_mark_ready)
+    bool wrapped = false;         // the memory is the caller's (rlb_tensor_wrap)
     size_t bytes() const { return (size_t)rows * cap * (dtype == RLB_F16 ? 2 : 4); }
+};
+
+// Records the tensor's event on the context's stream. Wrapped tensors have none (waiting on one waits for the stream), and
+// none is recorded into a graph that the caller is capturing: the event would stay bound to the graph.
+int tensor_mark_ready(rlb_tensor* t);
+// Whether the caller is capturing the context's (borrowed) stream.
+bool ctx_capturing(const rlb_ctx* ctx);
+// `p` is memory of the context's device (anything else would fault inside a kernel).
+int check_device_memory(const rlb_ctx* ctx, const void* p, const char* who);
+// Both tensors on one context (RLB_ERR_INVALID otherwise, also for a null tensor).
+int same_ctx(const rlb_tensor* a, const rlb_tensor* b);
+
+// Makes the context's device current for one call and the caller's device current again after it.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t err;
+    explicit DeviceScope(int device) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+};
+
+// Device scratch of one call. Eagerly it is the context's op_scratch (one stream, so calls follow one another); while the
+// stream is captured it is allocated and freed by nodes of the graph itself, so that graphs share no scratch with one
+// another or with eager calls and stay valid whatever the context does later.
+struct OpWorkspace {
+    rlb_ctx* ctx = nullptr;
+    void* p = nullptr;
+    bool in_graph = false;
+    int get(rlb_ctx* c, size_t bytes);
+    ~OpWorkspace();
 };
 
 struct rlb_event {
@@ -177,6 +212,37 @@ int launch_attn_prefill(rlb_ctx* ctx, rlb_dtype cache_dtype, const AttnPrefillAr
 // Tensor-core form (attention_tc.cu): f16 caches, head_dim 64 / 128, at least 32 query rows.
 bool attn_prefill_tc_supported(rlb_dtype cache_dtype, const AttnPrefillArgs& a);
 int launch_attn_prefill_tc(rlb_ctx* ctx, const AttnPrefillArgs& a, int* err);
+
+// ---------------------------------------------------------------------------------------
+// long-context attention (attention_long.cu): a window, first tokens kept, shared K/V heads, 4-bit caches
+// ---------------------------------------------------------------------------------------
+enum CacheKind { CACHE_F32 = 0, CACHE_F16 = 1, CACHE_Q4 = 2 };
+
+struct rlb_cache4 {
+    rlb_ctx* ctx = nullptr;
+    uint8_t* codes[2] = {nullptr, nullptr};   // K, V: [kv_heads][max_seq][hd / 2]  (cache4.h)
+    __half* scales[2] = {nullptr, nullptr};   // K, V: [kv_heads][max_seq][hd / 32]
+    int kv_heads = 0, max_seq = 0, hd = 0;
+    int device = 0;                           // (freeing does not look at the context, which may be gone by then)
+    void* owned = nullptr;                    // the allocation behind the four arrays, when the library made it
+};
+
+struct AttnLongArgs {
+    const float* q = nullptr;                 // n rows of heads * hd f32, row stride q_ld
+    int64_t q_ld = 0;
+    const void* k = nullptr;                  // [kv_heads][max_seq][hd] in the cache dtype, or the 4-bit codes
+    const void* v = nullptr;
+    const __half* k_scale = nullptr;          // 4-bit caches only
+    const __half* v_scale = nullptr;
+    void* out = nullptr;                      // n rows of heads * hd, row stride out_ld; f32 for f32 caches, else f16
+    int64_t out_ld = 0;
+    int n = 0, heads = 0, kv_heads = 0, group = 0, hd = 0, max_seq = 0;  // group = heads / kv_heads
+    int start = 0, window = 0, sinks = 0;
+    int n_split = 1;
+    float* rec_o = nullptr;                   // n_split > 1: [row][split][hd] unnormalised outputs ...
+    float2* rec_ml = nullptr;                 // ... and [row][split] (maximum, sum)
+};
+int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 
 // ---------------------------------------------------------------------------------------
 // row-wise / element-wise kernels used by prefill and the tier-1 ops (elementwise.cu)

@@ -515,6 +515,8 @@ int rlb_model_create(rlb_ctx* ctx, const rlb_model_params* p, rlb_model** out) {
     if (p->vocab_size % tp != 0) return rlb_fail(RLB_ERR_INVALID, "vocab_size %d is not divisible by tp_size %d", p->vocab_size, tp);
     if (p->n_heads < tp) return rlb_fail(RLB_ERR_INVALID, "fewer heads (%d) than tensor-parallel ranks (%d)", p->n_heads, tp);
 
+    if (ctx->borrowed_stream)
+        return rlb_fail(RLB_ERR_STATE, "a model captures its decode step on the context's stream: it needs a context with a stream of its own");
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
     RLB_CUDA(cudaSetDevice(ctx->device));
     rlb_model* m = new rlb_model();

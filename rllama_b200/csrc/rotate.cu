@@ -1,0 +1,176 @@
+// The way of q, k and v rows from their projection into attention, as one op: optional RMSNorm of every q and k head
+// (RMSNorm::forward, src/transformer.rs:476-480, over head_dim), the rotation of neighbouring pairs (apply_rotary_emb,
+// src/transformer.rs:823-856) and the cache write loop (:751-761).
+//
+//   y = x * (1 / sqrt(mean(x^2) + eps)) * gain            (only with gains)
+//   (a, b) -> (a cos - b sin, a sin + b cos)              pairs (2j, 2j+1), angle = position * 10000^(-2j / head_dim)
+//
+// All of it is f32; a cache row is rounded once, to the cache's dtype.
+#include "internal.h"
+
+#include <cmath>
+#include <new>
+#include <vector>
+
+namespace {
+
+struct RotateArgs {
+    const float* q; const float* k; const float* v;
+    float* q_out;
+    int64_t q_ld, k_ld, v_ld, qo_ld;
+    const float* q_gain; const float* k_gain;  // null: no norm
+    const float* table; int64_t table_ld;      // row of a position: (cos, sin) of pair 0, 1, ...
+    void* kcache; void* vcache;
+    int n, heads, kv_heads, max_seq, start;
+    float eps;
+};
+
+template <int N> struct Vec;
+template <> struct Vec<4> { typedef float4 T; };
+template <> struct Vec<2> { typedef float2 T; };
+
+template <typename CT, int N> __device__ __forceinline__ void store_cache(CT* p, const float (&x)[N]) {
+    if constexpr (sizeof(CT) == 2) {
+        __half2 h[N / 2];
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        if constexpr (N == 4) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+        else *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(h);
+    } else {
+        *reinterpret_cast<typename Vec<N>::T*>(p) = *reinterpret_cast<const typename Vec<N>::T*>(x);
+    }
+}
+
+// A warp per (token, slot); slots are the q heads, the k heads and the v heads. A lane holds HD / 32 neighbouring values,
+// i.e. whole pairs, and the norm's sum is one reduction over the warp.
+template <typename CT, int HD>
+__global__ void __launch_bounds__(256) norm_rope_append_kernel(const RotateArgs a) {
+    constexpr int N = HD / 32;
+    typedef typename Vec<N>::T V;
+    const int slots = a.heads + 2 * a.kv_heads;
+    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (w >= (int64_t)a.n * slots) return;
+    const int i = (int)(w / slots), slot = (int)(w % slots), c = (threadIdx.x & 31) * N;
+    const int kind = slot < a.heads ? 0 : slot < a.heads + a.kv_heads ? 1 : 2;
+    const int head = kind == 0 ? slot : kind == 1 ? slot - a.heads : slot - a.heads - a.kv_heads;
+    const float* src = kind == 0 ? a.q + i * a.q_ld : kind == 1 ? a.k + i * a.k_ld : a.v + i * a.v_ld;
+    float x[N];
+    *reinterpret_cast<V*>(x) = *reinterpret_cast<const V*>(src + head * HD + c);
+    const int pos = a.start + i;
+    const int64_t row = ((int64_t)head * a.max_seq + pos) * HD + c;
+    if (kind == 2) {
+        store_cache<CT, N>(reinterpret_cast<CT*>(a.vcache) + row, x);
+        return;
+    }
+    float f[N];
+    *reinterpret_cast<V*>(f) = *reinterpret_cast<const V*>(a.table + pos * a.table_ld + c);
+    const float* gain = kind == 0 ? a.q_gain : a.k_gain;
+    if (gain) {
+        float g[N];
+        *reinterpret_cast<V*>(g) = *reinterpret_cast<const V*>(gain + c);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; e++) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float s = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = x[e] * s * g[e];
+    }
+    float y[N];
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+        y[e] = __fsub_rn(__fmul_rn(x[e], f[e]), __fmul_rn(x[e + 1], f[e + 1]));
+        y[e + 1] = __fadd_rn(__fmul_rn(x[e], f[e + 1]), __fmul_rn(x[e + 1], f[e]));
+    }
+    if (kind == 0) *reinterpret_cast<V*>(a.q_out + i * a.qo_ld + head * HD + c) = *reinterpret_cast<const V*>(y);
+    else store_cache<CT, N>(reinterpret_cast<CT*>(a.kcache) + row, y);
+}
+
+template <typename CT>
+void launch(const RotateArgs& a, int hd, unsigned grid, cudaStream_t s) {
+    if (hd == 128) norm_rope_append_kernel<CT, 128><<<grid, 256, 0, s>>>(a);
+    else norm_rope_append_kernel<CT, 64><<<grid, 256, 0, s>>>(a);
+}
+
+int check_gain(const rlb_tensor* g, const rlb_tensor* like, int64_t hd) {
+    if (!g) return RLB_OK;
+    RLB_TRY(same_ctx(g, like));
+    if (g->dtype != RLB_F32 || g->rows != 1 || g->cols != hd) return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: a gain must be 1 x head_dim f32");
+    return RLB_OK;
+}
+
+}  // namespace
+
+extern "C" int rlb_rope_table(rlb_ctx* ctx, int32_t max_seq_len, int32_t head_dim, rlb_tensor** out) {
+    if (!ctx || !out) return rlb_fail(RLB_ERR_INVALID, "rlb_rope_table: null pointer");
+    *out = nullptr;
+    if (max_seq_len < 1 || head_dim < 4 || head_dim % 4 != 0)
+        return rlb_fail(RLB_ERR_INVALID, "rlb_rope_table: bad max_seq_len %d or head_dim %d (a multiple of 4)", max_seq_len, head_dim);
+    // compute_freqs_cis (src/transformer.rs:858-885): f64 angles, narrowed to f32 where they are applied
+    float* tab = new (std::nothrow) float[(size_t)max_seq_len * head_dim];
+    if (!tab) return rlb_fail(RLB_ERR_OOM, "rlb_rope_table: out of host memory");
+    for (int i = 0; i < head_dim / 2; i++) {
+        const double freq = 1.0 / pow(10000.0, (double)i * 2.0 / (double)head_dim);
+        for (int pos = 0; pos < max_seq_len; pos++) {
+            const double ang = freq * (double)pos;
+            tab[(size_t)pos * head_dim + 2 * i] = (float)cos(ang);
+            tab[(size_t)pos * head_dim + 2 * i + 1] = (float)sin(ang);
+        }
+    }
+    DeviceScope dev(ctx->device);
+    int s = dev.err == cudaSuccess ? RLB_OK : rlb_fail(RLB_ERR_CUDA, "rlb_rope_table: %s", cudaGetErrorString(dev.err));
+    if (s == RLB_OK) s = rlb_tensor_upload(ctx, tab, max_seq_len, head_dim, head_dim, RLB_F32, out);
+    if (s == RLB_OK) s = rlb_tensor_wait(*out);
+    if (s != RLB_OK && *out) {
+        rlb_tensor_free(*out);
+        *out = nullptr;
+    }
+    delete[] tab;
+    return s;
+}
+
+extern "C" int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_tensor* vcache, const rlb_tensor* q, const rlb_tensor* k,
+                                    const rlb_tensor* v, const rlb_tensor* q_gain, const rlb_tensor* k_gain, float eps, const rlb_tensor* rope,
+                                    int32_t heads, int32_t kv_heads, int32_t max_seq_len, int32_t start_pos) {
+    for (const rlb_tensor* t : {(const rlb_tensor*)kcache, (const rlb_tensor*)vcache, q, k, v, rope}) RLB_TRY(same_ctx(q_out, t));
+    const int64_t n = q->rows, hd = kcache->cols;
+    RLB_TRY(check_gain(q_gain, q_out, hd));
+    RLB_TRY(check_gain(k_gain, q_out, hd));
+    if (heads < 1 || kv_heads < 1 || max_seq_len < 1 || start_pos < 0 || start_pos + n > max_seq_len)
+        return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: bad heads %d, kv_heads %d, max_seq_len %d, start_pos %d or %lld rows", heads, kv_heads,
+                        max_seq_len, start_pos, (long long)n);
+    if (hd != 64 && hd != 128) return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: head_dim %lld is not supported (64 or 128)", (long long)hd);
+    if (kcache->cap != hd || vcache->cap != hd || vcache->cols != hd || kcache->rows != (int64_t)kv_heads * max_seq_len ||
+        vcache->rows != kcache->rows || kcache->dtype != vcache->dtype)
+        return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: caches must be (kv_heads*max_seq_len) x head_dim without row padding");
+    if (q->dtype != RLB_F32 || q->cols != heads * hd || q_out->dtype != RLB_F32 || q_out->rows != n || q_out->cols != q->cols)
+        return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: q and q_out must be n x heads*head_dim f32");
+    if (k->dtype != RLB_F32 || k->rows != n || k->cols != kv_heads * hd || v->dtype != RLB_F32 || v->rows != n || v->cols != k->cols)
+        return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: k and v must be n x kv_heads*head_dim f32");
+    if (rope->dtype != RLB_F32 || rope->cols != hd || rope->rows < start_pos + n)
+        return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: the rope table must be f32, head_dim wide and cover position %lld", (long long)(start_pos + n - 1));
+    if (!(eps >= 0.f)) return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: eps must not be negative");
+    const int64_t warps = n * ((int64_t)heads + 2 * (int64_t)kv_heads);
+    if ((warps + 7) / 8 > 0x7fffffffll) return rlb_fail(RLB_ERR_LIMIT, "norm_rope_append: %lld rows of %d heads are more than one launch takes", (long long)n, heads);
+    if (n == 0) return RLB_OK;
+    rlb_ctx* ctx = q_out->ctx;
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
+    RotateArgs a;
+    a.q = (const float*)q->d; a.k = (const float*)k->d; a.v = (const float*)v->d; a.q_out = (float*)q_out->d;
+    a.q_ld = q->cap; a.k_ld = k->cap; a.v_ld = v->cap; a.qo_ld = q_out->cap;
+    a.q_gain = q_gain ? (const float*)q_gain->d : nullptr; a.k_gain = k_gain ? (const float*)k_gain->d : nullptr;
+    a.table = (const float*)rope->d; a.table_ld = rope->cap;
+    a.kcache = kcache->d; a.vcache = vcache->d;
+    a.n = (int)n; a.heads = heads; a.kv_heads = kv_heads; a.max_seq = max_seq_len; a.start = start_pos; a.eps = eps;
+    const unsigned grid = (unsigned)((warps + 7) / 8);
+    if (kcache->dtype == RLB_F16) launch<__half>(a, (int)hd, grid, ctx->stream);
+    else launch<float>(a, (int)hd, grid, ctx->stream);
+    RLB_LAUNCH_CHECK();
+    count_launch(ctx);
+    RLB_TRY(tensor_mark_ready(q_out));
+    RLB_TRY(tensor_mark_ready(kcache));
+    return tensor_mark_ready(vcache);
+}
