@@ -8,62 +8,13 @@
 //
 // The union of what the positions p0..p1 see is two runs, [0, S) and [L, p1 + 1) with L = max(0, p0 + 1 - window) and
 // S = min(sinks, L); kernels walk it as one virtual index v -> v < S ? v : v - S + L.
-#include "cache4.h"
-#include "internal.h"
+#include "attention_long.h"
 
 #include <algorithm>
-#include <cfloat>
+
+using namespace attn_long;
 
 namespace {
-
-struct Run {
-    int s, l, len;  // first run [0, s), second [l, l + len - s)
-    __device__ __forceinline__ int at(int v) const { return v < s ? v : v - s + l; }
-};
-__device__ __forceinline__ int window_low(const AttnLongArgs& a, int p) { return max(0, p + 1 - a.window); }
-__device__ __forceinline__ Run visible_run(const AttnLongArgs& a, int p0, int p1) {
-    Run r;
-    r.l = window_low(a, p0);
-    r.s = min(a.sinks, r.l);
-    r.len = r.s + p1 + 1 - r.l;
-    return r;
-}
-__device__ __forceinline__ bool visible(const AttnLongArgs& a, int p, int t) { return t <= p && (t >= window_low(a, p) || t < a.sinks); }
-
-// HD / 32 neighbouring values of a cache row, as f32.
-template <int KIND, int HD> __device__ __forceinline__ void load_row(const void* base, const __half* scales, int64_t row, int lane, float (&x)[HD / 32]) {
-    constexpr int N = HD / 32;
-    if constexpr (KIND == CACHE_F32) {
-        const float* p = reinterpret_cast<const float*>(base) + row * HD + lane * N;
-        if constexpr (N == 4) { const float4 v = *reinterpret_cast<const float4*>(p); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-        else { const float2 v = *reinterpret_cast<const float2*>(p); x[0] = v.x; x[1] = v.y; }
-    } else {
-        __half2 h[N / 2];
-        if constexpr (KIND == CACHE_F16) {
-            const __half* p = reinterpret_cast<const __half*>(base) + row * HD + lane * N;
-            if constexpr (N == 4) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
-            else *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(p);
-        } else {
-            constexpr int G = HD / kQ4Group;
-            const int e = lane * N;
-            const uint32_t w = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(base) + row * (HD / 2))[q4_word(e, G)];
-            const __half2 d = __half2half2(scales[row * G + e / kQ4Group]);
-#pragma unroll
-            for (int j = 0; j < N / 2; j++) h[j] = __hmul2(q4_pair(w, (e % 8) / 2 + j), d);
-        }
-#pragma unroll
-        for (int j = 0; j < N / 2; j++) {
-            const float2 f = __half22float2(h[j]);
-            x[2 * j] = f.x;
-            x[2 * j + 1] = f.y;
-        }
-    }
-}
-
-template <int KIND> struct Out { typedef __half T; };
-template <> struct Out<CACHE_F32> { typedef float T; };
-__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
 
 // One query row: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
 template <int KIND, int HD>
@@ -135,28 +86,17 @@ __global__ void __launch_bounds__(128) attn_long_merge_kernel(const AttnLongArgs
 }
 
 template <int KIND, int HD>
-int launch_rows(rlb_ctx* ctx, AttnLongArgs a) {
-    const int64_t rows = (int64_t)a.n * a.heads;
-    // eight CTAs an SM, and at least 64 positions to a split
-    const int64_t most = std::min<int64_t>((int64_t)a.sinks + a.window, (int64_t)a.start + a.n);
-    int64_t splits = std::min<int64_t>((8 * ctx->sm_count + rows - 1) / rows, (most + 63) / 64);
-    a.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(splits, 256));
-    OpWorkspace ws;
-    if (a.n_split > 1) {
-        const size_t recs = (size_t)rows * a.n_split;
-        RLB_TRY(ws.get(ctx, recs * (HD * sizeof(float) + sizeof(float2))));
-        a.rec_ml = (float2*)ws.p;
-        a.rec_o = (float*)(a.rec_ml + recs);
-    }
-    attn_long_row_kernel<KIND, HD><<<dim3((unsigned)rows, a.n_split), 256, 0, ctx->stream>>>(a);
+int launch_rows(rlb_ctx* ctx, const AttnLongArgs& a) {
+    attn_long_row_kernel<KIND, HD><<<dim3((unsigned)(a.n * a.heads), a.n_split), 256, 0, ctx->stream>>>(a);
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
-    if (a.n_split > 1) {
-        attn_long_merge_kernel<typename Out<KIND>::T><<<(unsigned)rows, HD, 0, ctx->stream>>>(a);
-        RLB_LAUNCH_CHECK();
-        count_launch(ctx);
-    }
     return RLB_OK;
+}
+int rows_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
+    // eight CTAs an SM, and at least 64 positions to a split
+    const int64_t rows = (int64_t)a.n * a.heads, most = std::min<int64_t>((int64_t)a.sinks + a.window, (int64_t)a.start + a.n);
+    const int64_t splits = std::min<int64_t>((8 * ctx->sm_count + rows - 1) / rows, (most + 63) / 64);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(splits, 256));
 }
 
 // What both entry points require of q, out and the visible set.
@@ -191,9 +131,28 @@ int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, i
 
 }  // namespace
 
-int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
-    if (a.hd == 128) return kind == CACHE_F32 ? launch_rows<CACHE_F32, 128>(ctx, a) : kind == CACHE_F16 ? launch_rows<CACHE_F16, 128>(ctx, a) : launch_rows<CACHE_Q4, 128>(ctx, a);
-    return kind == CACHE_F32 ? launch_rows<CACHE_F32, 64>(ctx, a) : kind == CACHE_F16 ? launch_rows<CACHE_F16, 64>(ctx, a) : launch_rows<CACHE_Q4, 64>(ctx, a);
+int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
+    AttnLongArgs a = given;
+    const bool tiles = kind != CACHE_F32 && (int64_t)a.n * a.group >= 64;
+    a.n_split = tiles ? attn_long_tc_splits(ctx, a) : rows_splits(ctx, a);
+    const int64_t rows = (int64_t)a.n * a.heads;
+    OpWorkspace ws;
+    if (a.n_split > 1) {
+        const size_t recs = (size_t)rows * a.n_split;
+        RLB_TRY(ws.get(ctx, recs * (a.hd * sizeof(float) + sizeof(float2))));
+        a.rec_o = (float*)ws.p;
+        a.rec_ml = (float2*)(a.rec_o + recs * a.hd);
+    }
+    if (tiles) RLB_TRY(launch_attn_long_tc(ctx, kind, a));
+    else if (a.hd == 128) RLB_TRY(kind == CACHE_F32 ? (launch_rows<CACHE_F32, 128>(ctx, a)) : kind == CACHE_F16 ? (launch_rows<CACHE_F16, 128>(ctx, a)) : (launch_rows<CACHE_Q4, 128>(ctx, a)));
+    else RLB_TRY(kind == CACHE_F32 ? (launch_rows<CACHE_F32, 64>(ctx, a)) : kind == CACHE_F16 ? (launch_rows<CACHE_F16, 64>(ctx, a)) : (launch_rows<CACHE_Q4, 64>(ctx, a)));
+    if (a.n_split > 1) {
+        if (kind == CACHE_F32) attn_long_merge_kernel<float><<<(unsigned)rows, a.hd, 0, ctx->stream>>>(a);
+        else attn_long_merge_kernel<__half><<<(unsigned)rows, a.hd, 0, ctx->stream>>>(a);
+        RLB_LAUNCH_CHECK();
+        count_launch(ctx);
+    }
+    return RLB_OK;
 }
 
 extern "C" int rlb_attention_window(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor* kcache, const rlb_tensor* vcache, int32_t heads,

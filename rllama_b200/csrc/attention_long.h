@@ -1,0 +1,64 @@
+// Device helpers shared by the long-context attention kernels: the visible set, cache rows as f32, the plain form of a row.
+#pragma once
+
+#include <cfloat>
+
+#include "cache4.h"
+#include "internal.h"
+
+namespace attn_long {
+
+struct Run {
+    int s, l, len;  // first run [0, s), second [l, l + len - s)
+    __device__ __forceinline__ int at(int v) const { return v < s ? v : v - s + l; }
+};
+__device__ __forceinline__ int window_low(const AttnLongArgs& a, int p) { return max(0, p + 1 - a.window); }
+__device__ __forceinline__ Run visible_run(const AttnLongArgs& a, int p0, int p1) {
+    Run r;
+    r.l = window_low(a, p0);
+    r.s = min(a.sinks, r.l);
+    r.len = r.s + p1 + 1 - r.l;
+    return r;
+}
+__device__ __forceinline__ bool visible(const AttnLongArgs& a, int p, int t) { return t <= p && (t >= window_low(a, p) || t < a.sinks); }
+
+// HD / 32 neighbouring values of a cache row, as f32.
+template <int KIND, int HD> __device__ __forceinline__ void load_row(const void* base, const __half* scales, int64_t row, int lane, float (&x)[HD / 32]) {
+    constexpr int N = HD / 32;
+    if constexpr (KIND == CACHE_F32) {
+        const float* p = reinterpret_cast<const float*>(base) + row * HD + lane * N;
+        if constexpr (N == 4) { const float4 v = *reinterpret_cast<const float4*>(p); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+        else { const float2 v = *reinterpret_cast<const float2*>(p); x[0] = v.x; x[1] = v.y; }
+    } else {
+        __half2 h[N / 2];
+        if constexpr (KIND == CACHE_F16) {
+            const __half* p = reinterpret_cast<const __half*>(base) + row * HD + lane * N;
+            if constexpr (N == 4) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+            else *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            constexpr int G = HD / kQ4Group;
+            const int e = lane * N;
+            const uint32_t w = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(base) + row * (HD / 2))[q4_word(e, G)];
+            const __half2 d = __half2half2(scales[row * G + e / kQ4Group]);
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) h[j] = __hmul2(q4_pair(w, (e % 8) / 2 + j), d);
+        }
+#pragma unroll
+        for (int j = 0; j < N / 2; j++) {
+            const float2 f = __half22float2(h[j]);
+            x[2 * j] = f.x;
+            x[2 * j + 1] = f.y;
+        }
+    }
+}
+
+template <int KIND> struct Out { typedef __half T; };
+template <> struct Out<CACHE_F32> { typedef float T; };
+__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+
+}  // namespace attn_long
+
+// attention_long_tc.cu
+int attn_long_tc_splits(rlb_ctx* ctx, const AttnLongArgs& a);
+int launch_attn_long_tc(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
