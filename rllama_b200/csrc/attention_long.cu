@@ -134,7 +134,7 @@ int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, i
 int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     AttnLongArgs a = given;
     const bool tiles = kind != CACHE_F32 && (int64_t)a.n * a.group >= 64;
-    a.n_split = tiles ? attn_long_tc_splits(ctx, a) : rows_splits(ctx, a);
+    a.n_split = tiles ? attn_long_tc_splits(ctx, kind, a) : rows_splits(ctx, a);
     const int64_t rows = (int64_t)a.n * a.heads;
     OpWorkspace ws;
     if (a.n_split > 1) {

@@ -60,5 +60,5 @@ __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2hal
 }  // namespace attn_long
 
 // attention_long_tc.cu
-int attn_long_tc_splits(rlb_ctx* ctx, const AttnLongArgs& a);
+int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 int launch_attn_long_tc(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);

@@ -3,13 +3,17 @@
 // few tokens attend with many heads.
 //
 // A CTA owns 256 rows (two tiles of 128) of a K/V head and walks the positions that some of them see in steps of 128:
-//  * K and V steps pass through a ring of shared-memory stages. An f16 cache's are fetched by TMA (128-byte swizzle, the
-//    tensor's extent ends at the last visible position: rows behind it read as zeros). A 4-bit cache's are unpacked by
-//    four warps; its values are f16 numbers, so the unpacked operand carries no rounding.
-//  * one thread issues the MMAs: S = Q K^T (both operands in shared memory), then O += P V with P in tensor memory as the
-//    A operand. S, and over it P, and O of both tiles fill the 512 columns. While one tile's scores go through the
-//    softmax, the other tile's products run.
-//  * eight warps do the softmax, a thread a row: maximum of the step's 128 scores, weights 2^(s - m + 7) rounded to f16
+//  * K and V steps pass through a ring of shared-memory stages, in the order in which they are used: K0 K1 V0 K2 V1 K3 ...
+//    An f16 cache's are fetched by TMA (128-byte swizzle, the tensor's extent ends at the last visible position: rows
+//    behind it read as zeros). A 4-bit cache's are unpacked by four warps; its values are f16 numbers, so the unpacked
+//    operand carries no rounding.
+//  * one thread a tile issues its MMAs: S = Q K^T (both operands in shared memory), then O += P V with P in tensor memory as
+//    the A operand. Tensor memory holds, per tile, O, one buffer of 64 scores and two of 64 weights: the scores are free
+//    again as soon as the softmax has them in registers, so the next ones are computed during the exponentials, and a
+//    weight buffer is only needed again two steps later. Neither side waits for a chain of the other's. (Weights written
+//    over their scores made a step's chain softmax, output product, next scores: with one buffer of 128 scores 5200
+//    cycles for 256 x 128 scores, with two of 64 still 4000.)
+//  * eight warps do the softmax, a thread a row: maximum of the step's 64 scores, weights 2^(s - m + 7) rounded to f16
 //    (their sum is taken before the rounding), back to tensor memory. The running maximum m is only moved when a row's
 //    scores exceed it by 2^8 (then the row's O is scaled in place); weights therefore stay below 2^15, and the factor
 //    2^7 keeps weights down to 2^-21 of the largest normal f16 numbers. It cancels in O / l.
@@ -27,6 +31,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_long.h"
 
@@ -35,12 +40,7 @@ using namespace attn_long;
 namespace {
 
 constexpr int QT = 128;                 // rows of a tile (MMA M)
-constexpr int QB = 2 * QT;              // rows of a CTA
-constexpr int TK = 128;                 // positions of a step
-constexpr int kSoftmaxWarps = 8;
-constexpr int kMmaWarp = kSoftmaxWarps;
-constexpr int kLoadWarp = kMmaWarp + 1;
-constexpr int kUnpackWarps = 4;
+constexpr int TK = 64;                  // positions of a step
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr float kShift = 7.f;           // weights carry 2^7
 constexpr float kLag = 8.f;             // the running maximum may lag by 2^8
@@ -71,6 +71,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     *reinterpret_cast<volatile int*>(err) = 4;
     return false;
 }
+// The same for a whole warp, with one answer for all of its lanes (they go on together or not at all).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, dead, err));
+}
 // Waits, with the same limit, for work of the CTA's own that is in flight, whether or not the CTA gave up.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
     for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(bar, parity); i++) {}
@@ -99,21 +103,44 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
                  "r"(idesc), "r"(accumulate)
                  : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&x)[32]) {
-    uint32_t r[32];
+// 32 columns of the thread's lane. The values are there only after tmem_ld_wait, and `tmem_arrived` on them after it keeps
+// the compiler from using them before.
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t addr, float* x) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
         "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]), "=f"(x[10]),
+          "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]), "=f"(x[16]), "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]),
+          "=f"(x[21]), "=f"(x[22]), "=f"(x[23]), "=f"(x[24]), "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_arrived(float* x) {
 #pragma unroll
-    for (int e = 0; e < 32; e++) x[e] = __uint_as_float(r[e]);
+    for (int e = 0; e < 32; e++) asm volatile("" : "+f"(x[e]));
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&x)[32]) {
+    tmem_ld32_issue(addr, x);
+    tmem_ld_wait();
+    tmem_arrived(x);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&x)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]), "=f"(x[10]),
+          "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
+        : "r"(addr));
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; e++) asm volatile("" : "+f"(x[e]));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -213,30 +240,41 @@ __device__ __noinline__ void slow_row(const AttnLongArgs& a, int kvh, int row, i
 }
 
 template <int KIND, int HD> struct Layout {
+    // An f16 CTA has one tile, and two CTAs share an SM: one's first loads, masks and last stores fall into the other's main
+    // loop (8192 rows of 32 heads, window 2048: two tiles in one CTA 326 us, two CTAs 278). Unpacking 4-bit rows costs too much to be done for one tile: two share it.
+    static constexpr int TILES = KIND == CACHE_Q4 ? 2 : 1;
+    static constexpr int ROWS = TILES * QT;                  // rows of a CTA
     static constexpr int NB = HD / 64;                       // 64-column blocks of a row
     static constexpr uint32_t Q_BYTES = QT * HD * 2;
     static constexpr uint32_t STAGE = TK * HD * 2;
-    static constexpr int STAGES = HD == 64 ? 8 : 4;         // 128 KB
-    static constexpr int THREADS = (kLoadWarp + (KIND == CACHE_Q4 ? kUnpackWarps : 1)) * 32;
-    static constexpr size_t SMEM = 2 * Q_BYTES + STAGES * STAGE + 1024;
+    static constexpr int STAGES = (TILES == 2 ? 8 : 4) * 128 / HD;
+    static constexpr uint32_t TMEM_COLS = TILES * 256;
+    // warps: four a tile for the softmax, one a tile for its MMAs, then one that loads, or eight that unpack
+    static constexpr int SOFTMAX_WARPS = 4 * TILES, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = KIND == CACHE_Q4 ? 12 : MMA_WARP + TILES;
+    static constexpr int THREADS = (LOAD_WARP + (KIND == CACHE_Q4 ? 8 : 1)) * 32;
+    static constexpr size_t SMEM = TILES * Q_BYTES + STAGES * STAGE + 1024;
 };
+// 4-bit: 640 threads are launched with 96 registers each. The MMA and unpacking warps give 32 of theirs to the softmax warps:
+// 8 * 32 * 144 + 12 * 32 * 64 = 61440 = 640 * 96.
+constexpr int kSoftmaxRegs = 144, kOtherRegs = 64;
 
 template <int KIND, int HD>
-__global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
+__global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD>::TILES)
     attn_long_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_k_first, const __grid_constant__ CUtensorMap tm_v_first, const __grid_constant__ AttnLongArgs a, int* err) {
     typedef Layout<KIND, HD> Y;
-    constexpr int NB = Y::NB, STAGES = Y::STAGES;
-    constexpr uint32_t TMEM_COLS = 512, O_COL = 2 * TK;
+    constexpr int NB = Y::NB, STAGES = Y::STAGES, TILES = Y::TILES, QB = Y::ROWS;
+    constexpr uint32_t O_COL = TILES * 2 * TK;   // [tile]: S [TK], P [buffer][TK / 2]; then [tile]: O [HD]
     extern __shared__ unsigned char smem_raw[];
     unsigned char* q_s = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // [tile][HD/64][128][64]
-    unsigned char* ring = q_s + 2 * Y::Q_BYTES;                                                              // [stage][HD/64][128][64]
-    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], p_ready[2], pv_done[2], drained;
+    unsigned char* ring = q_s + TILES * Y::Q_BYTES;                                                              // [stage][HD/64][128][64]
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], q_ready[2], drained[2];
+    __shared__ __align__(8) uint64_t p_ready[4], pv_done[4];   // [tile][buffer]: a phase is seen before the next one begins
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_flag;
     volatile int* dead = &dead_flag;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (known to be uniform)
     const int kvh = blockIdx.x % a.kv_heads;
     const int n_rows = a.n * a.group;
     const int row0 = ((n_rows + QB - 1) / QB - 1 - (int)blockIdx.x / a.kv_heads) * QB;  // the longest rows first
@@ -244,73 +282,56 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
     const Steps st = make_steps(a, a.start + row0 / a.group, a.start + row_last / a.group);
     const int per = (st.n + a.n_split - 1) / a.n_split;
     const int j0 = min(st.n, (int)blockIdx.y * per), j1 = min(st.n, j0 + per);
-    int pa[2], pb[2];  // first and last position of each tile's rows
+    int pa[TILES], pb[TILES];  // first and last position of each tile's rows
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
+    for (int t = 0; t < TILES; t++) {
         pa[t] = a.start + min(row0 + t * QT, row_last) / a.group;
         pb[t] = a.start + min(row0 + t * QT + QT - 1, row_last) / a.group;
     }
-    const bool two = row0 + QT <= row_last;  // the second tile has rows
+    const bool two = TILES == 2 && row0 + QT <= row_last;  // the second tile has rows
     auto cols = [&](int t, int j) { return t == 0 || two ? step_cols(a, st, j, pa[t], pb[t]) : Cols{0, 0}; };
 
     if (threadIdx.x == 0) {
         dead_flag = 0;
         for (int s = 0; s < STAGES; s++) {
-            mbar_init(&full[s], KIND == CACHE_Q4 ? kUnpackWarps : 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&full[s], KIND == CACHE_Q4 ? 4 : 1);
+            mbar_init(&empty[s], TILES);
+        }
+        for (int b = 0; b < 4; b++) {
+            mbar_init(&p_ready[b], 4);
+            mbar_init(&pv_done[b], 1);
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_ready[t], 4);
-            mbar_init(&pv_done[t], 1);
+            mbar_init(&s_read[t], 4);
+            mbar_init(&q_ready[t], 4);
+            mbar_init(&drained[t], 1);
         }
-        mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) {
+    if (warp == Y::MMA_WARP) {
         __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(Y::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    // The queries as f16 in the A operand's layout: row r, 16-byte chunk c of a 64-column block at r * 128 + ((c ^ (r & 7)) * 16).
-    const int tile = warp >> 2, r = threadIdx.x & (QT - 1);   // (softmax threads: their tile and row)
-    const int row = min(row0 + tile * QT + r, row_last);
-    float c2 = 0.f;                                           // scores are s * c2 in units of log2 e
-    if (warp < kSoftmaxWarps) {
-        const bool live = row0 + tile * QT + r <= row_last;
-        const float4* src = reinterpret_cast<const float4*>(a.q + (int64_t)(row / a.group) * a.q_ld + (int64_t)(kvh * a.group + row % a.group) * HD);
-        float top = 0.f;
-        for (int c = 0; c < HD / 4; c++) {
-            const float4 v = src[c];
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-        // 2^e <= top < 2^(e+1); an infinite top keeps its factor (the row is not finite and is computed again)
-        int e = (int)((__float_as_uint(top) >> 23) & 0xff) - 127;
-        e = e > 127 ? 0 : max(e, -100);
-        const float up = live ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f, down = __uint_as_float((uint32_t)(e - 8 + 127) << 23);
-        c2 = rsqrtf((float)HD) * 1.4426950408889634f * down;
-        for (int c = 0; c < HD / 8; c++) {
-            const float4 v0 = src[2 * c], v1 = src[2 * c + 1];
-            __half2 h[4] = {__floats2half2_rn(v0.x * up, v0.y * up), __floats2half2_rn(v0.z * up, v0.w * up), __floats2half2_rn(v1.x * up, v1.y * up),
-                            __floats2half2_rn(v1.z * up, v1.w * up)};
-            *reinterpret_cast<uint4*>(q_s + tile * Y::Q_BYTES + (c >> 3) * (QT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads these through the async proxy
     }
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_slot;
 
-    if (warp >= kLoadWarp) {
-        // ------------------------------- K and V steps into the ring: K(j0), V(j0), K(j0 + 1), ... -------------------
+    if (warp >= Y::LOAD_WARP) {
+        // ------------------------------- K and V steps into the ring -------------------------------------------------
+        if constexpr (KIND == CACHE_Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         const int items = 2 * (j1 - j0);
+        auto item_is_v = [&](int x) { return x > 0 && (x % 2 == 0 || x == items - 1); };
+        auto item_step = [&](int x) { return j0 + (x == items - 1 ? x / 2 : item_is_v(x) ? x / 2 - 1 : (x + 1) / 2); };
         if constexpr (KIND == CACHE_F16) {
             if (lane == 0) {
                 int x = 0;
                 for (; x < items; x++) {
-                    const int s = x % STAGES, j = j0 + x / 2, t0 = st.at(j);
-                    const CUtensorMap* map = j < st.n_first ? ((x & 1) ? &tm_v_first : &tm_k_first) : ((x & 1) ? &tm_v : &tm_k);
+                    const int s = x % STAGES, j = item_step(x), t0 = st.at(j);
+                    const bool v = item_is_v(x);
+                    const CUtensorMap* map = j < st.n_first ? (v ? &tm_v_first : &tm_k_first) : (v ? &tm_v : &tm_k);
                     if (x >= STAGES && !mbar_wait(&empty[s], (x / STAGES - 1) & 1, dead, err)) break;
                     mbar_expect_tx(&full[s], Y::STAGE);
 #pragma unroll
@@ -319,26 +340,27 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
                 for (int y = max(0, x - STAGES); y < x; y++) mbar_drain(&full[y % STAGES], (y / STAGES) & 1);  // no copy outlives the CTA
             }
         } else {
-            // A thread unpacks a quarter of a row: the same block of eight values of every group (cache4.h). 32 rows a pass.
-            constexpr int G = HD / kQ4Group;
-            const int x0 = threadIdx.x - kLoadWarp * 32, quarter = x0 & 3, rr = x0 >> 2;
-            uint32_t w[4][G];
-            __half d[4][G];
-            auto fetch = [&](int x) {
-                const int j = j0 + x / 2, t0 = st.at(j), end = j < st.n_first ? min(a.sinks, a.start + a.n) : a.start + a.n;
-                const uint8_t* codes = reinterpret_cast<const uint8_t*>((x & 1) ? a.v : a.k);
-                const __half* scales = (x & 1) ? a.v_scale : a.k_scale;
+            // Two groups of four warps take every other item. A thread unpacks a quarter of a row: the same block of eight
+            // values of every group (cache4.h), 32 rows a pass; the next AHEAD items of its warps are on their way.
+            constexpr int G = HD / kQ4Group, ROWS = 32, PASSES = TK / ROWS, AHEAD = 2;
+            const int x0 = (threadIdx.x - Y::LOAD_WARP * 32) & 127, quarter = x0 & 3, rr = x0 >> 2, group = (warp - Y::LOAD_WARP) >> 2;
+            uint32_t w[AHEAD][PASSES][G];
+            __half d[AHEAD][PASSES][G];
+            const int64_t base = (int64_t)kvh * a.max_seq + rr;
+            auto fetch = [&](int x, uint32_t (&w)[PASSES][G], __half (&d)[PASSES][G]) {
+                const bool v = item_is_v(x);
+                const int j = item_step(x), t0 = st.at(j), end = (j < st.n_first ? min(a.sinks, a.start + a.n) : a.start + a.n) - t0 - rr;
+                const uint8_t* codes = reinterpret_cast<const uint8_t*>(v ? a.v : a.k) + (base + t0) * (HD / 2) + quarter * (HD / 8);
+                const __half* scales = (v ? a.v_scale : a.k_scale) + (base + t0) * G;
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int t = t0 + u * 32 + rr;
-                    const int64_t at = (int64_t)kvh * a.max_seq + t;
-                    if (t < end) {
+                for (int u = 0; u < PASSES; u++) {
+                    if (u * ROWS < end) {
                         if constexpr (G == 4) {
-                            *reinterpret_cast<uint4*>(w[u]) = *reinterpret_cast<const uint4*>(codes + at * 64 + quarter * 16);
-                            *reinterpret_cast<uint2*>(d[u]) = *reinterpret_cast<const uint2*>(scales + at * 4);
+                            *reinterpret_cast<uint4*>(w[u]) = *reinterpret_cast<const uint4*>(codes + u * ROWS * (HD / 2));
+                            *reinterpret_cast<uint2*>(d[u]) = *reinterpret_cast<const uint2*>(scales + u * ROWS * G);
                         } else {
-                            *reinterpret_cast<uint2*>(w[u]) = *reinterpret_cast<const uint2*>(codes + at * 32 + quarter * 8);
-                            *reinterpret_cast<uint32_t*>(d[u]) = *reinterpret_cast<const uint32_t*>(scales + at * 2);
+                            *reinterpret_cast<uint2*>(w[u]) = *reinterpret_cast<const uint2*>(codes + u * ROWS * (HD / 2));
+                            *reinterpret_cast<uint32_t*>(d[u]) = *reinterpret_cast<const uint32_t*>(scales + u * ROWS * G);
                         }
                     } else {
 #pragma unroll
@@ -346,90 +368,178 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
                     }
                 }
             };
-            if (items > 0) fetch(0);
-            for (int x = 0; x < items; x++) {
+            // (row rr + 32 u keeps rr's place in the swizzle pattern, so the four passes store at constant offsets)
+            uint32_t off[G];
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const int chunk = 4 * g + quarter;   // eight values 32 g + 8 quarter ...
+                off[g] = (chunk >> 3) * (TK * 128) + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4);
+            }
+            bool ok = true;
+            auto unpack = [&](int x, uint32_t (&w)[PASSES][G], __half (&d)[PASSES][G]) {
                 const int s = x % STAGES;
-                if (x >= STAGES && !mbar_wait(&empty[s], (x / STAGES - 1) & 1, dead, err)) break;
+                ok = ok && (x < STAGES || warp_wait(&empty[s], (x / STAGES - 1) & 1, dead, err));
+                if (!ok) return;
                 unsigned char* dst = ring + s * Y::STAGE;
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int y = u * 32 + rr;
+                for (int u = 0; u < PASSES; u++) {
 #pragma unroll
                     for (int g = 0; g < G; g++) {
                         const __half2 dd = __half2half2(d[u][g]);
                         __half2 h[4];
+                        q4_pairs(w[u][g], h);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) h[e] = __hmul2(q4_pair(w[u][g], e), dd);
-                        const int chunk = 4 * g + quarter;   // eight values 32 g + 8 quarter ...
-                        *reinterpret_cast<uint4*>(dst + (chunk >> 3) * (TK * 128) + y * 128 + (((chunk & 7) ^ (y & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
+                        for (int e = 0; e < 4; e++) h[e] = __hmul2(h[e], dd);
+                        *reinterpret_cast<uint4*>(dst + off[g] + u * ROWS * 128) = *reinterpret_cast<uint4*>(h);
                     }
                 }
+                if (x + 2 * AHEAD < items) fetch(x + 2 * AHEAD, w, d);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[s]);
-                if (x + 1 < items) fetch(x + 1);
+            };
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+                if (group + 2 * u < items) fetch(group + 2 * u, w[u], d[u]);
+            for (int x = group; x < items && ok; x += 2 * AHEAD) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                    if (x + 2 * u < items) unpack(x + 2 * u, w[u], d[u]);
             }
         }
-    } else if (warp == kMmaWarp) {
+    } else if (warp >= Y::MMA_WARP) {
         // ------------------------------- MMA issuer ------------------------------------------------------------------
-        if (lane == 0) {
+        if constexpr (KIND == CACHE_Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp < Y::MMA_WARP + TILES) {
+            // The whole warp runs this and one thread issues: descriptors then live in uniform registers, and eight MMAs are
+            // issued in 200 cycles (from a branch of one thread it took 600 to 1400, longer than they run). Descriptors are a base plus
+            // a constant (the address is their low bits, in units of 16 bytes), and a step that the tile sees whole goes
+            // through straight-line code.
+            const bool leader = elect_one();
+            const int t = warp - Y::MMA_WARP;
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(QT >> 4) << 24);   // | N / 8 << 17
             const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(QT >> 4) << 24);
-            uint32_t done[2] = {0, 0};   // output products issued
-            auto scores = [&](int t, int j, Cols c) {
-                const uint32_t qa = smem_u32(q_s) + t * Y::Q_BYTES, kb = smem_u32(ring) + (uint32_t)((2 * (j - j0)) % STAGES) * Y::STAGE + c.c0 * 128;
-                const uint32_t id = idesc_s | (uint32_t)((c.c1 - c.c0) >> 3) << 17;
-#pragma unroll
-                for (int k = 0; k < HD / 16; k++)
-                    umma_ss(tmem + t * TK + c.c0, desc_kmajor(qa + (k >> 2) * (QT * 128) + (k & 3) * 32), desc_kmajor(kb + (k >> 2) * (TK * 128) + (k & 3) * 32), id, k > 0);
-                umma_commit(&s_full[t]);
+            const uint64_t q_desc = desc_kmajor(smem_u32(q_s) + t * Y::Q_BYTES);
+            const uint64_t k_desc = desc_kmajor(smem_u32(ring)), v_desc = desc_mnmajor(smem_u32(ring), TK * 128);
+            // Steps that the tile sees whole: from the first that starts at its last row's window to the last that ends at its first row.
+            const int whole0 = st.n_first + max(0, window_low(a, pb[t]) - st.l + TK - 1) / TK, whole1 = t == 0 || two ? st.n_first + (pa[t] + 1 - st.l) / TK : 0;
+            auto cols_at = [&](int j) { return j >= whole0 && j < whole1 ? Cols{0, TK} : cols(t, j); };
+            uint32_t scored = 0, done = 0;       // scores and output products issued; the n-th product takes its weights from buffer n & 1
+            uint32_t stage = 0, phase = 0;       // of the next item; items are used in the order in which they are loaded
+            auto advance = [&]() {
+                if (leader) umma_commit(&empty[stage]);
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
             };
-            auto wait_item = [&](int x) { return mbar_wait(&full[x % STAGES], (x / STAGES) & 1, dead, err); };
-            bool ok = j1 > j0 && wait_item(0);
-            if (ok) {
-                tc_after();
-                for (int t = 0; t < 2; t++)
-                    if (const Cols c = cols(t, j0); c.any()) scores(t, j0, c);
-                umma_commit(&empty[0]);
-            }
-            for (int j = j0; j < j1 && ok; j++) {
-                const int xv = 2 * (j - j0) + 1;
-                for (int t = 0; t < 2 && ok; t++) {
-                    const Cols now = cols(t, j);
-                    if (t == 0) ok = wait_item(xv);
-                    if (now.any() && ok) {
-                        ok = mbar_wait(&p_ready[t], done[t] & 1, dead, err);
-                        if (!ok) break;
-                        tc_after();
-                        const uint32_t vb = smem_u32(ring) + (uint32_t)(xv % STAGES) * Y::STAGE;
-                        for (int k = now.c0 / 16; k < now.c1 / 16; k++)
-                            umma_ts(tmem + O_COL + t * HD, tmem + t * TK + k * 8, desc_mnmajor(vb + k * 2048, TK * 128), idesc_o, done[t] > 0 || k > now.c0 / 16);
-                        umma_commit(&pv_done[t]);
-                        done[t]++;
-                    }
-                    if (t == 1) umma_commit(&empty[xv % STAGES]);
-                    if (j + 1 < j1) {
-                        if (t == 0) ok = ok && wait_item(xv + 1);
-                        // the scores overwrite the weights: the output product that reads them must be complete
-                        if (const Cols next = cols(t, j + 1); ok && next.any()) {
-                            ok = done[t] == 0 || mbar_wait(&pv_done[t], (done[t] - 1) & 1, dead, err);
-                            if (!ok) break;
-                            tc_after();
-                            scores(t, j + 1, next);
-                        }
-                        if (t == 1) umma_commit(&empty[(xv + 1) % STAGES]);
-                    }
+            auto scores = [&](Cols c) {          // K of the next item
+                if (c.any()) {
+                    tc_after();
+                    const uint64_t kb = k_desc + (stage * Y::STAGE + (uint32_t)c.c0 * 128) / 16;
+                    const uint32_t id = idesc_s | (uint32_t)((c.c1 - c.c0) >> 3) << 17, d = tmem + 2 * t * TK + c.c0;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++)
+                        if (leader) umma_ss(d, q_desc + ((k >> 2) * (QT * 128) + (k & 3) * 32) / 16, kb + ((k >> 2) * (TK * 128) + (k & 3) * 32) / 16, id, k > 0);
+                    if (leader) umma_commit(&s_full[t]);
+                    scored++;
                 }
+                advance();
+            };
+            Cols now{0, 0}, next = cols_at(j0);
+            bool ok = warp_wait(&q_ready[t], 0, dead, err);
+            for (int j = j0 - 1; j < j1 && ok; j++) {   // scores of step j + 1, then the output product of step j
+                if (j + 1 < j1) {
+                    ok = warp_wait(&full[stage], phase, dead, err);
+                    if (next.any() && scored > 0) ok = ok && warp_wait(&s_read[t], (scored - 1) & 1, dead, err);
+                    if (!ok) break;
+                    scores(next);
+                }
+                if (j >= j0) {
+                    const uint32_t buf = done & 1;
+                    ok = warp_wait(&full[stage], phase, dead, err);
+                    if (now.any()) ok = ok && warp_wait(&p_ready[2 * t + buf], (done >> 1) & 1, dead, err);
+                    if (!ok) break;
+                    if (now.any()) {
+                        tc_after();
+                        const uint64_t vb = v_desc + stage * Y::STAGE / 16;
+                        const uint32_t d = tmem + O_COL + t * HD, w = tmem + 2 * t * TK + TK + buf * (TK / 2);
+                        if (now.c0 == 0 && now.c1 == TK) {
+#pragma unroll
+                            for (int k = 0; k < TK / 16; k++)
+                                if (leader) umma_ts(d, w + k * 8, vb + k * 2048 / 16, idesc_o, k > 0 || done > 0);
+                        } else {
+                            for (int k = now.c0 / 16; k < now.c1 / 16; k++)
+                                if (leader) umma_ts(d, w + k * 8, vb + k * 2048 / 16, idesc_o, k > now.c0 / 16 || done > 0);
+                        }
+                        if (leader) umma_commit(&pv_done[2 * t + buf]);
+                        done++;
+                    }
+                    advance();
+                }
+                now = next;
+                next = j + 2 < j1 ? cols_at(j + 2) : Cols{0, 0};
             }
-            if (!ok) {  // no product outlives the CTA either (after a full run the softmax warps have waited for the last)
-                umma_commit(&drained);
-                mbar_drain(&drained, 0);
+            if (!ok) {  // no product outlives the CTA (after a full run the softmax warps have waited for the last)
+                if (leader) umma_commit(&drained[t]);
+                mbar_drain(&drained[t], 0);
             }
         }
     } else {
         // ------------------------------- softmax: a thread owns a row ------------------------------------------------
+        if constexpr (KIND == CACHE_Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int tile = warp >> 2, r = threadIdx.x & (QT - 1);   // the thread's tile and row
+        const int row = min(row0 + tile * QT + r, row_last);
+        // First the queries, as f16 in the A operand's layout: row r, 16-byte chunk c of a 64-column block at r * 128 +
+        // ((c ^ (r & 7)) * 16). A warp fetches its 32 rows in batches of eight, lanes across head_dim, one batch ahead. (Straight-line
+        // code for 32 rows is slower: every CTA would fetch it anew.)
+        float c2 = 0.f;                                           // scores are s * c2 in units of log2 e
+        {
+            constexpr int N = HD / 32, B = 8;
+            const int first = tile * QT + (warp & 3) * 32;
+            int i = min(row0 + first, row_last) / a.group, g = min(row0 + first, row_last) - i * a.group, fetched = row0 + first;
+            auto fetch = [&](float (&x)[B][N]) {
+#pragma unroll
+                for (int u = 0; u < B; u++) {
+                    const float* src = a.q + i * a.q_ld + (int64_t)(kvh * a.group + g) * HD + lane * N;
+                    if constexpr (N == 4) *reinterpret_cast<float4*>(x[u]) = *reinterpret_cast<const float4*>(src);
+                    else *reinterpret_cast<float2*>(x[u]) = *reinterpret_cast<const float2*>(src);
+                    if (fetched++ < row_last && ++g == a.group) { g = 0; i++; }   // (behind the last row: that row again)
+                }
+            };
+            float x[B][N], ahead[B][N];
+            fetch(ahead);
+#pragma unroll 1
+            for (int y0 = 0; y0 < 32; y0 += B) {
+#pragma unroll
+                for (int u = 0; u < B; u++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) x[u][e] = ahead[u][e];
+                if (y0 + B < 32) fetch(ahead);
+#pragma unroll
+                for (int u = 0; u < B; u++) {
+                    const int y = y0 + u;
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(x[u][e]));
+                    // the exponent of the largest magnitude, 2^e <= top < 2^(e+1); an infinite one keeps its factor (the row is
+                    // not finite and is computed again)
+                    int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+                    e = e > 127 ? 0 : max(e, -100);
+                    const float up = row0 + first + y <= row_last ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
+                    if (lane == y) c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+                    __half2 h[N / 2];
+#pragma unroll
+                    for (int v = 0; v < N / 2; v++) h[v] = __floats2half2_rn(x[u][2 * v] * up, x[u][2 * v + 1] * up);
+                    const int c = lane * N / 8, yy = (warp & 3) * 32 + y;
+                    unsigned char* dst = q_s + tile * Y::Q_BYTES + (c >> 3) * (QT * 128) + yy * 128 + (((c & 7) ^ u) << 4) + (lane * N % 8) * 2;
+                    if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
+                    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads these through the async proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready[tile]);
+        }
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_addr = tmem + lanes + tile * TK, o_addr = tmem + lanes + O_COL + tile * HD;
+        const uint32_t s_addr = tmem + lanes + 2 * tile * TK, o_addr = tmem + lanes + O_COL + tile * HD;
         const int p = a.start + row / a.group, low = window_low(a, p);
         float m = -FLT_MAX, l = 0.f;
         uint32_t steps = 0;
@@ -437,107 +547,127 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
         const int warp_row = row0 + tile * QT + (warp & 3) * 32;   // the warp's first and last position
         const int wa = a.start + min(warp_row, row_last) / a.group, wb = a.start + min(warp_row + 31, row_last) / a.group;
         const int low_wa = window_low(a, wa), low_wb = window_low(a, wb);
-        for (int j = j0; j < j1 && ok; j++) {
-            const Cols now = cols(tile, j);
-            if (!now.any()) continue;
-            ok = mbar_wait(&s_full[tile], steps & 1, dead, err);
-            if (!ok) break;
-            tc_after();
+        const uint64_t c2_2 = pack2(c2, c2);
+        // One step; `whole`: every row of the warp sees all of it.
+        auto step = [&](auto whole, int j, Cols now) {
+            constexpr bool W = decltype(whole)::value;
+            const uint32_t p_addr = s_addr + TK + (steps & 1) * (TK / 2);
             // columns of the step that the row sees: below `to`, and from `from` on or below `first`
-            const int t0 = st.at(j);
+            const int t0 = W ? 0 : st.at(j);
             const bool in_first = j < st.n_first;
             const int to = (in_first ? st.s : p + 1) - t0, from = (in_first ? 0 : low) - t0, first = (in_first ? 0 : a.sinks) - t0;
-            // 0: nobody in the warp sees any of the block of 32 columns, 2: everybody sees all of it, 1: else
+            // a block of 32 columns is -1: not computed, 0: seen by nobody in the warp, 2: all of it seen by everybody, 1: else
             auto block = [&](int c) {
                 if (c < now.c0 || c >= now.c1) return -1;
                 if (in_first) return c + 32 <= to ? 2 : 1;
                 if (c >= wb + 1 - t0 || (c + 32 <= low_wa - t0 && c >= first)) return 0;
                 return c + 32 <= wa + 1 - t0 && (c >= low_wb - t0 || c + 32 <= first) ? 2 : 1;
             };
-            auto mask = [&](int c, float (&x)[32]) {
-#pragma unroll
-                for (int e = 0; e < 32; e++) x[e] = (c + e < to && (c + e >= from || c + e < first)) ? x[e] : -INFINITY;
-            };
-            float top = -INFINITY;
+            float x[TK];
+            int kind[TK / 32];
 #pragma unroll
             for (int c = 0; c < TK; c += 32) {
-                const int b = block(c);
-                if (b <= 0) continue;
-                float x[32];
-                tmem_ld32(s_addr + c, x);
-                if (b == 1) mask(c, x);
+                kind[c / 32] = W ? 2 : block(c);
+                if (kind[c / 32] > 0) {
+                    tmem_ld32_issue(s_addr + c, x + c);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 32; e++) top = fmaxf(top, x[e]);
+                    for (int e = 0; e < 32; e++) x[c + e] = -INFINITY;
+                }
             }
-            top *= c2;
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < TK; c += 32) tmem_arrived(x + c);
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_read[tile]);   // the next scores may come
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains
+#pragma unroll
+            for (int c = 0; c < TK; c += 32) {
+                if (kind[c / 32] == 1) {
+#pragma unroll
+                    for (int e = c; e < c + 32; e++) x[e] = (e < to && (e >= from || e < first)) ? x[e] : -INFINITY;
+                }
+#pragma unroll
+                for (int e = c; e < c + 32; e++) tops[e & 3] = fmaxf(tops[e & 3], x[e]);
+            }
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * c2;
             const bool move = top > m + kLag;
             if (__any_sync(0xffffffffu, move)) {
                 const float m_new = move ? top : m, scale = ex2_approx(m - m_new);
                 m = m_new;
                 l *= scale;
-                if (steps > 0) {   // (the previous output product is complete: its completion went before these scores)
+                if (steps > 0) {
+                    ok = warp_wait(&pv_done[2 * tile + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, dead, err);   // O is at rest
+                    tc_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        float o[16];
+                        tmem_ld16(o_addr + c, o);
+                        uint32_t y[16];
 #pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        float x[32];
-                        tmem_ld32(o_addr + c, x);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            uint32_t y[16];
-#pragma unroll
-                            for (int e = 0; e < 16; e++) y[e] = __float_as_uint(x[h * 16 + e] * scale);
-                            tmem_st16(o_addr + c + h * 16, y);
-                        }
+                        for (int e = 0; e < 16; e++) y[e] = __float_as_uint(o[e] * scale);
+                        tmem_st16(o_addr + c, y);
                     }
                     tmem_st_wait();
                 }
             }
-            const float shift = kShift - m;
-            const uint64_t c2_2 = pack2(c2, c2), shift_2 = pack2(shift, shift);
-            uint64_t sum = 0;   // (0, 0)
+            const uint64_t shift_2 = pack2(kShift - m, kShift - m);
+            if (steps >= 2) ok = warp_wait(&pv_done[2 * tile + (steps & 1)], ((steps - 2) >> 1) & 1, dead, err) && ok;   // the weights two steps ago are used
+            uint64_t sum[2] = {0, 0};   // two chains of two
 #pragma unroll
             for (int c = 0; c < TK; c += 32) {
-                const int b = block(c);
-                if (b < 0) continue;
+                if (kind[c / 32] < 0) continue;
                 uint32_t y[16];
-                if (b == 0) {
+                if (kind[c / 32] == 0) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) y[e] = 0;
                 } else {
-                    float x[32];
-                    tmem_ld32(s_addr + c, x);
-                    if (b == 1) mask(c, x);
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         float w0, w1;
-                        unpack2(fma2(pack2(x[2 * e], x[2 * e + 1]), c2_2, shift_2), w0, w1);
+                        unpack2(fma2(pack2(x[c + 2 * e], x[c + 2 * e + 1]), c2_2, shift_2), w0, w1);
                         w0 = ex2_approx(w0);
                         w1 = ex2_approx(w1);
-                        sum = add2(sum, pack2(w0, w1));
+                        sum[e & 1] = add2(sum[e & 1], pack2(w0, w1));
                         const __half2 h = __floats2half2_rn(w0, w1);
                         y[e] = *reinterpret_cast<const uint32_t*>(&h);
                     }
                 }
-                tmem_st16(s_addr + c / 2, y);   // over scores that have been read
+                tmem_st16(p_addr + c / 2, y);
             }
             float sum0, sum1;
-            unpack2(sum, sum0, sum1);
+            unpack2(add2(sum[0], sum[1]), sum0, sum1);
             l += sum0 + sum1;
             tmem_st_wait();
+        };
+        // steps that the warp sees whole: from the first that starts at its last row's window to the last that ends at its first row
+        const int whole0 = st.n_first + max(0, low_wb - st.l + TK - 1) / TK, whole1 = tile == 0 || two ? st.n_first + (wa + 1 - st.l) / TK : 0;
+        for (int j = j0; j < j1; j++) {
+            const bool whole = j >= whole0 && j < whole1;
+            const Cols now = whole ? Cols{0, TK} : cols(tile, j);
+            if (!now.any()) continue;
+            ok = warp_wait(&s_full[tile], steps & 1, dead, err);
+            if (!ok) break;
+            tc_after();
+            if (whole) step(std::true_type{}, j, now);
+            else step(std::false_type{}, j, now);
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[tile]);
+            if (lane == 0) mbar_arrive(&p_ready[2 * tile + (steps & 1)]);
             steps++;
+            if (!ok) break;
         }
-        if (ok && steps > 0) ok = mbar_wait(&pv_done[tile], (steps - 1) & 1, dead, err);
+        if (ok && steps > 0) ok = warp_wait(&pv_done[2 * tile + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, dead, err);
         const bool live = row0 + tile * QT + r <= row_last;
         if (ok && __any_sync(0xffffffffu, live)) {
             tc_after();
             const int64_t rec = ((int64_t)row / a.group * a.heads + kvh * a.group + row % a.group) * a.n_split + blockIdx.y;
-            __half* dst = reinterpret_cast<__half*>(a.out) + (int64_t)(row / a.group) * a.out_ld + (int64_t)(kvh * a.group + row % a.group) * HD;
+            unsigned char* turn = q_s + tile * Y::Q_BYTES + (warp & 3) * (32 * HD * 2);   // (the tile's scores are all computed: its queries' room is free)
             const bool empty_row = p + 1 - low + min(a.sinks, low) == 0;
             const float inv = empty_row ? 0.f : 1.0f / l;
             float check = fmaf(l, 0.f, a.n_split == 1 ? inv * 0.f : 0.f);   // a NaN once anything is not finite
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 float x[32];
                 if (steps > 0) {
@@ -551,19 +681,33 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
                 if (live && a.n_split > 1) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(a.rec_o + rec * HD + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                } else if (live) {
+                } else if (a.n_split == 1) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         __half2 h[4];
 #pragma unroll
                         for (int u = 0; u < 4; u++) h[u] = empty_row ? __half2half2(__ushort_as_half(0)) : __floats2half2_rn(x[e + 2 * u] * inv, x[e + 2 * u + 1] * inv);
-                        *reinterpret_cast<uint4*>(dst + c + e) = *reinterpret_cast<uint4*>(h);
+                        *reinterpret_cast<uint4*>(turn + lane * (HD * 2) + ((((c + e) / 8) ^ (lane & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
                     }
                 }
                 __syncwarp();
             }
+            if (a.n_split == 1) {   // out of the warp's rows in shared memory, a row's bytes side by side
+                constexpr int LPR = HD / 8;   // lanes a row
+                int i = min(warp_row, row_last) / a.group, g = min(warp_row, row_last) - i * a.group + lane / LPR;
+#pragma unroll 4
+                for (int y = 0; y < 32; y += 32 / LPR) {
+                    while (g >= a.group) { g -= a.group; i++; }
+                    const int yy = y + lane / LPR, chunk = lane % LPR;
+                    if (warp_row + yy <= row_last)
+                        *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(a.out) + i * a.out_ld + (int64_t)(kvh * a.group + g) * HD + chunk * 8) =
+                            *reinterpret_cast<const uint4*>(turn + yy * (HD * 2) + ((chunk ^ (yy & 7)) << 4));
+                    g += 32 / LPR;
+                }
+            }
             if (live && a.n_split > 1) a.rec_ml[rec] = make_float2(m - kShift, l);
             // rows next to infinite or NaN cache contents, again and one by one
+            __syncwarp();
             uint32_t bad = __ballot_sync(0xffffffffu, live && check != 0.f && !empty_row);
             while (bad) {
                 const int b = __ffs(bad) - 1;
@@ -585,9 +729,9 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 1)
     }
     tc_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == Y::MMA_WARP) {
         __syncwarp();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Y::TMEM_COLS) : "memory");
     }
 }
 
@@ -634,7 +778,7 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
         RLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Y::SMEM));
         attr_mark(set, ctx->device);
     }
-    const int blocks = (a.n * a.group + QB - 1) / QB;
+    const int blocks = (a.n * a.group + Y::ROWS - 1) / Y::ROWS;
     kern<<<dim3((unsigned)(blocks * a.kv_heads), a.n_split), Y::THREADS, Y::SMEM, ctx->stream>>>(mk, mv, mkf, mvf, a, ctx->d_err);
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
@@ -643,12 +787,19 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
 
 }  // namespace
 
-int attn_long_tc_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
-    // one CTA an SM; a split has at least four steps (its own set-up and record cost about two)
-    const int64_t ctas = (int64_t)a.kv_heads * ((a.n * a.group + QB - 1) / QB);
-    const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + QB / a.group, (int64_t)a.start + a.n);
+// Splits of the positions: CTAs run in rounds over the SMs, and a CTA costs its share of the steps and about eight more (set-up,
+// queries, masks, record or result). A split has at least eight steps.
+int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+    const int tiles = kind == CACHE_Q4 ? 2 : 1;
+    const int64_t rows = tiles * QT, ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + rows - 1) / rows), slots = (int64_t)ctx->sm_count * (2 / tiles);
+    const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + rows / a.group, (int64_t)a.start + a.n);
     const int64_t steps = (seen + TK - 1) / TK;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count / std::max<int64_t>(ctas, 1), steps / 4));
+    int64_t best = 1, cost = INT64_MAX;
+    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(steps / 8, 64)); s++) {
+        const int64_t c = ((ctas * s + slots - 1) / slots) * ((steps + s - 1) / s + 8);
+        if (c < cost) { cost = c; best = s; }
+    }
+    return (int)best;
 }
 
 int launch_attn_long_tc(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {

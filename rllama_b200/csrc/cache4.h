@@ -31,6 +31,18 @@ __device__ __forceinline__ __half2 q4_pair(uint32_t word, int j) {
 }
 __host__ __device__ __forceinline__ int q4_word(int e, int groups) { return (e % kQ4Group) / 8 * groups + e / kQ4Group; }
 
+// The four pairs of a word: the nibbles in the upper half of a byte are taken in place, as 1024 + 16 u.
+__device__ __forceinline__ void q4_pairs(uint32_t word, __half2 (&h)[4]) {
+    const uint32_t bias = 0x64086408u, sixteenth = 0x2C002C00u, high_bias = 0xD480D480u;  // 1032, 1/16, -72 = -(1024 / 16 + 8)
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        const uint32_t w = b ? word >> 8 : word;
+        const uint32_t lo = (w & 0x000F000Fu) | 0x64006400u, hi = (w & 0x00F000F0u) | 0x64006400u;
+        h[2 * b] = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&bias));
+        h[2 * b + 1] = __hfma2(*reinterpret_cast<const __half2*>(&hi), *reinterpret_cast<const __half2*>(&sixteenth), *reinterpret_cast<const __half2*>(&high_bias));
+    }
+}
+
 // Scale of a group whose largest magnitude is m.
 __device__ __forceinline__ __half q4_scale(float m) {
     return __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fmul_rn(fminf(m, 65504.f), 1.0f / 7.0f))));

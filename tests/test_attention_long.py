@@ -128,6 +128,7 @@ def attend(cl, q, k, v, heads, kv, hd, start, window, sinks, kind, max_seq, pois
         kc[:, :total], vc[:, :total] = k, v
         k, v = kc[:, :total].clone(), vc[:, :total].clone()
         cl.wrap(out).attention_window(cl.wrap(q), cl.wrap(kc.view(-1, hd)), cl.wrap(vc.view(-1, hd)), heads, kv, max_seq, start, window, sinks)
+    cl.flush()  # raises if a kernel gave up on a wait
     if out_pad:
         assert (wide[:, heads * hd:] == 7.0).all(), "the padding of out was written"
     return out, k, v
