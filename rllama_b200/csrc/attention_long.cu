@@ -16,8 +16,8 @@ using namespace attn_long;
 
 namespace {
 
-// One query row: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
-template <int KIND, int HD>
+// One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
+template <int HD>
 __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a) {
     constexpr int N = HD / 32;
     __shared__ float w_o[8][HD], w_m[8], w_l[8];
@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a
     for (int v = v0 + warp; v < v1; v += 8) {
         const int64_t row = base + run.at(v);
         float k[N], x[N];
-        load_row<KIND, HD>(a.k, a.k_scale, row, lane, k);
-        load_row<KIND, HD>(a.v, a.v_scale, row, lane, x);
+        load_row<CACHE_F32, HD>(a.k, a.k_scale, row, lane, k);
+        load_row<CACHE_F32, HD>(a.v, a.v_scale, row, lane, x);
         float s = 0.f;
 #pragma unroll
         for (int e = 0; e < N; e++) s = fmaf(q[e], k[e], s);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a
         a.rec_o[rec * HD + threadIdx.x] = O;
         if (threadIdx.x == 0) a.rec_ml[rec] = make_float2(M, L);
     } else {
-        store_out(reinterpret_cast<typename Out<KIND>::T*>(a.out) + i * a.out_ld + head * HD + threadIdx.x, run.len > 0 ? O / L : 0.f);
+        store_out(reinterpret_cast<float*>(a.out) + i * a.out_ld + head * HD + threadIdx.x, run.len > 0 ? O / L : 0.f);
     }
 }
 
@@ -85,9 +85,9 @@ __global__ void __launch_bounds__(128) attn_long_merge_kernel(const AttnLongArgs
     store_out(reinterpret_cast<OT*>(a.out) + i * a.out_ld + head * a.hd + threadIdx.x, visible_run(a, p, p).len > 0 ? O / L : 0.f);
 }
 
-template <int KIND, int HD>
+template <int HD>
 int launch_rows(rlb_ctx* ctx, const AttnLongArgs& a) {
-    attn_long_row_kernel<KIND, HD><<<dim3((unsigned)(a.n * a.heads), a.n_split), 256, 0, ctx->stream>>>(a);
+    attn_long_row_kernel<HD><<<dim3((unsigned)(a.n * a.heads), a.n_split), 256, 0, ctx->stream>>>(a);
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
     return RLB_OK;
@@ -134,7 +134,7 @@ int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, i
 int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     AttnLongArgs a = given;
     const bool tiles = kind != CACHE_F32 && (int64_t)a.n * a.group >= 64;
-    a.n_split = tiles ? attn_long_tc_splits(ctx, kind, a) : rows_splits(ctx, a);
+    a.n_split = tiles ? attn_long_tc_splits(ctx, kind, a) : kind != CACHE_F32 ? attn_long_few_splits(ctx, kind, a) : rows_splits(ctx, a);
     const int64_t rows = (int64_t)a.n * a.heads;
     OpWorkspace ws;
     if (a.n_split > 1) {
@@ -144,8 +144,8 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
         a.rec_ml = (float2*)(a.rec_o + recs * a.hd);
     }
     if (tiles) RLB_TRY(launch_attn_long_tc(ctx, kind, a));
-    else if (a.hd == 128) RLB_TRY(kind == CACHE_F32 ? (launch_rows<CACHE_F32, 128>(ctx, a)) : kind == CACHE_F16 ? (launch_rows<CACHE_F16, 128>(ctx, a)) : (launch_rows<CACHE_Q4, 128>(ctx, a)));
-    else RLB_TRY(kind == CACHE_F32 ? (launch_rows<CACHE_F32, 64>(ctx, a)) : kind == CACHE_F16 ? (launch_rows<CACHE_F16, 64>(ctx, a)) : (launch_rows<CACHE_Q4, 64>(ctx, a)));
+    else if (kind != CACHE_F32) RLB_TRY(launch_attn_long_few(ctx, kind, a));
+    else RLB_TRY(a.hd == 128 ? launch_rows<128>(ctx, a) : launch_rows<64>(ctx, a));
     if (a.n_split > 1) {
         if (kind == CACHE_F32) attn_long_merge_kernel<float><<<(unsigned)rows, a.hd, 0, ctx->stream>>>(a);
         else attn_long_merge_kernel<__half><<<(unsigned)rows, a.hd, 0, ctx->stream>>>(a);

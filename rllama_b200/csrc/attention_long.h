@@ -52,13 +52,14 @@ template <int KIND, int HD> __device__ __forceinline__ void load_row(const void*
     }
 }
 
-template <int KIND> struct Out { typedef __half T; };
-template <> struct Out<CACHE_F32> { typedef float T; };
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
 
 }  // namespace attn_long
 
+// attention_long_few.cu
+int attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
+int launch_attn_long_few(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 // attention_long_tc.cu
 int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 int launch_attn_long_tc(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);

@@ -1,0 +1,356 @@
+// Long-context attention of few query rows (a generated token, a handful of drafted ones) over f16 and 4-bit caches:
+// attention_long.cu says what is computed. The time is that of reading the cache, so every K/V row is fetched once for up to eight query rows
+// that share its head (row = i * group + g, as in attention_long_tc.cu), straight from global memory into the registers
+// in which mma.sync takes it; nothing passes through shared memory.
+//
+// A CTA takes eight rows of a K/V head and a share of the positions that they see; each of its eight warps walks tiles of 16
+// positions of that share:
+//  * S (16 x 8 positions, twice) = [q hi; q lo] K^T: the eight queries as two f16 halves each, x = hi + lo, are the 16 rows of
+//    the A operand, so the scores carry 22 bits of the queries at no further MMA. A thread's share of K is 16 contiguous
+//    bytes of a row (or 4-bit words of every group, cache4.h): the contraction index may be ordered freely as long as the queries are
+//    ordered alike.
+//  * the weights 2^(s - m + 7) in f16 are then in the right place for the B operand of O^T = V^T P: there V is A, its rows the values,
+//    its columns the positions; pairs of positions are interleaved with one byte permutation a register.
+// The running maximum m moves only when a score exceeds it by 2^8, as in attention_long_tc.cu, and a row whose result is not
+// finite is computed again from what it sees alone. Scores, maxima, sums and O are f32; rounded to f16: the weights (2^-11) and the result.
+#include <algorithm>
+
+#include "attention_long.h"
+
+using namespace attn_long;
+
+namespace {
+
+constexpr int kRows = 8;    // query rows of a CTA
+constexpr int kWarps = 8;
+constexpr float kShift = 7.f, kLag = 8.f;
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// A thread's share of K in a tile: rows r and r + 8, of each HD / 4 values in chunks of eight, 8 (4 i + c) ...
+template <int KIND, int HD> struct KFrag;
+template <int HD> struct KFrag<CACHE_F16, HD> {
+    uint4 x[2][HD / 32];
+    __device__ __forceinline__ void load(const AttnLongArgs& a, int nt, int64_t row, int c) {
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.k) + row * HD) + c;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) x[nt][i] = __ldg(p + 4 * i);
+    }
+    __device__ __forceinline__ void chunk(int nt, int i, uint32_t (&h)[4]) const { h[0] = x[nt][i].x; h[1] = x[nt][i].y; h[2] = x[nt][i].z; h[3] = x[nt][i].w; }
+};
+template <int HD> struct KFrag<CACHE_Q4, HD> {
+    static constexpr int G = HD / kQ4Group;
+    uint32_t w[2][G];
+    __half d[2][G];
+    __device__ __forceinline__ void load(const AttnLongArgs& a, int nt, int64_t row, int c) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(a.k) + row * (HD / 2) + c * (HD / 8);
+        if constexpr (G == 4) {
+            *reinterpret_cast<uint4*>(w[nt]) = __ldg(reinterpret_cast<const uint4*>(p));
+            *reinterpret_cast<uint2*>(d[nt]) = __ldg(reinterpret_cast<const uint2*>(a.k_scale + row * G));
+        } else {
+            *reinterpret_cast<uint2*>(w[nt]) = __ldg(reinterpret_cast<const uint2*>(p));
+            *reinterpret_cast<uint32_t*>(d[nt]) = __ldg(reinterpret_cast<const uint32_t*>(a.k_scale + row * G));
+        }
+    }
+    __device__ __forceinline__ void chunk(int nt, int i, uint32_t (&h)[4]) const {
+        __half2 v[4];
+        q4_pairs(w[nt][i], v);
+        const __half2 dd = __half2half2(d[nt][i]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = bits(__hmul2(v[e], dd));
+    }
+};
+// A thread's share of V in a tile: positions 2c, 2c + 1, 2c + 8, 2c + 9, of each HD / 64 chunks of eight values. `dim` is a chunk's
+// first value; operand(u, e): pairs of positions of values 2e (a0, a2) and 2e + 1 (a1, a3) of chunk u.
+template <int KIND, int HD> struct VFrag;
+template <int HD> struct VFrag<CACHE_F16, HD> {
+    static constexpr int U = HD / 64;
+    uint4 x[4][U];
+    static __device__ __forceinline__ int dim(int u, int r) { return 8 * (8 * u + r); }
+    __device__ __forceinline__ void load(const AttnLongArgs& a, int i, int64_t row, int r) {
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.v) + row * HD) + r;
+#pragma unroll
+        for (int u = 0; u < U; u++) x[i][u] = __ldg(p + 8 * u);
+    }
+    __device__ __forceinline__ void operands(int u, uint32_t (&f)[4][4]) const {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t* p0 = reinterpret_cast<const uint32_t*>(&x[0][u]);
+            const uint32_t* p1 = reinterpret_cast<const uint32_t*>(&x[1][u]);
+            const uint32_t* p2 = reinterpret_cast<const uint32_t*>(&x[2][u]);
+            const uint32_t* p3 = reinterpret_cast<const uint32_t*>(&x[3][u]);
+            f[e][0] = __byte_perm(p0[e], p1[e], 0x5410);
+            f[e][1] = __byte_perm(p0[e], p1[e], 0x7632);
+            f[e][2] = __byte_perm(p2[e], p3[e], 0x5410);
+            f[e][3] = __byte_perm(p2[e], p3[e], 0x7632);
+        }
+    }
+};
+template <int HD> struct VFrag<CACHE_Q4, HD> {
+    static constexpr int U = HD / 64, G = HD / kQ4Group;
+    uint32_t w[4][U];
+    __half d[4][U];
+    static __device__ __forceinline__ int dim(int u, int r) { const int x = U * r + u; return 32 * (x % G) + 8 * (x / G); }
+    __device__ __forceinline__ void load(const AttnLongArgs& a, int i, int64_t row, int r) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(a.v) + row * (HD / 2)) + U * r;
+        const __half* s = a.v_scale + row * G + (U * r) % G;   // (a thread's words belong to neighbouring groups)
+        if constexpr (U == 2) {
+            *reinterpret_cast<uint2*>(w[i]) = __ldg(reinterpret_cast<const uint2*>(p));
+            *reinterpret_cast<uint32_t*>(d[i]) = __ldg(reinterpret_cast<const uint32_t*>(s));
+        } else {
+            w[i][0] = __ldg(p);
+            d[i][0] = __ldg(s);
+        }
+    }
+    __device__ __forceinline__ void operands(int u, uint32_t (&f)[4][4]) const {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {   // positions 2c, 2c + 1, then 2c + 8, 2c + 9
+            const __half2 dd = __halves2half2(d[2 * h][u], d[2 * h + 1][u]);
+            __half2 even[4], odd[4];
+            q4_pairs(__byte_perm(w[2 * h][u], w[2 * h + 1][u], 0x5410), even);
+            q4_pairs(__byte_perm(w[2 * h][u], w[2 * h + 1][u], 0x7632), odd);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f[e][2 * h] = bits(__hmul2(even[e], dd));
+                f[e][2 * h + 1] = bits(__hmul2(odd[e], dd));
+            }
+        }
+    }
+};
+
+template <int KIND, int HD>
+__global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_long_few_kernel(const __grid_constant__ AttnLongArgs a) {
+    constexpr int KS = HD / 16, U = VFrag<KIND, HD>::U;
+    __shared__ float o_s[kWarps][kRows][HD];
+    __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+    const int n_rows = a.n * a.group, blocks = (n_rows + kRows - 1) / kRows;
+    const int kvh = blockIdx.x / blocks, row0 = (blockIdx.x % blocks) * kRows, rows = min(kRows, n_rows - row0);
+    const int pa = a.start + row0 / a.group, pb = a.start + (row0 + rows - 1) / a.group;
+    const Run run = visible_run(a, pa, pb);
+    int chunk = (run.len + a.n_split - 1) / a.n_split;
+    chunk = (chunk + 15) & ~15;
+    const int v0 = min(run.len, (int)blockIdx.y * chunk), v1 = min(run.len, v0 + chunk);
+    const int64_t base = (int64_t)kvh * a.max_seq;
+
+    KFrag<KIND, HD> kf;
+    VFrag<KIND, HD> vf;
+    const int last = max(v1 - 1, 0);   // (positions behind the share read its last one and weigh nothing)
+    auto load_k = [&](int v) {
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) kf.load(a, nt, base + run.at(min(v + 8 * nt + r, last)), c);
+    };
+    auto load_v = [&](int v) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) vf.load(a, i, base + run.at(min(v + 2 * c + (i & 1) + 8 * (i >> 1), last)), r);
+    };
+    int v = v0 + warp * 16;
+    if (v < v1) load_k(v);
+
+    // the queries: rows r (high halves) and r + 8 (low halves) of the A operand
+    const int row = row0 + min(r, rows - 1), p = a.start + row / a.group, low = window_low(a, p);
+    uint32_t q[KS][4];
+    float c2;
+    {
+        const float* src = a.q + (int64_t)(row / a.group) * a.q_ld + (int64_t)(kvh * a.group + row % a.group) * HD + 8 * c;
+        float x[KS][4], top = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            *reinterpret_cast<float4*>(x[s]) = *reinterpret_cast<const float4*>(src + 32 * (s >> 1) + 4 * (s & 1));
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[s][e]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // scaled by a power of two so that the row's largest element lies in [2^8, 2^9), whatever its magnitude
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = e > 127 ? 0 : max(e, -100);
+        const float up = r < rows ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
+        c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float y0 = x[s][2 * h] * up, y1 = x[s][2 * h + 1] * up;
+                const __half2 hi = __floats2half2_rn(y0, y1);
+                const float2 f = __half22float2(hi);
+                q[s][2 * h] = bits(hi);
+                q[s][2 * h + 1] = bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
+            }
+    }
+    float o[U][4][4] = {}, m = -FLT_MAX, l = 0.f;
+    for (; v < v1; v += kWarps * 16) {
+        load_v(v);
+        float s[2][4] = {};
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                uint32_t h[4];
+                kf.chunk(nt, i, h);
+                mma16816(s[nt], q[2 * i], h[0], h[1]);
+                mma16816(s[nt], q[2 * i + 1], h[2], h[3]);
+            }
+        if (v + kWarps * 16 < v1) load_k(v + kWarps * 16);
+        float x[4];   // scores of the thread's row at positions 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = (s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)]) * c2;
+        const int t0 = run.at(v), t1 = run.at(v + 15);
+        if (!(v + 16 <= v1 && t1 == t0 + 15 && t1 <= pa && (t0 >= window_low(a, pb) || t1 < a.sinks))) {   // some row does not see all of it
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int w = v + 2 * c + (e & 1) + 8 * (e >> 1), t = run.at(w);
+                if (!(w < v1 && t <= p && (t >= low || t < a.sinks))) x[e] = -INFINITY;
+            }
+        }
+        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (__any_sync(0xffffffffu, top > m + kLag)) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m, top), scale = ex2_approx(m - m_new);
+            m = m_new;
+            l *= scale;
+            const float f0 = __shfl_sync(0xffffffffu, scale, 8 * c), f1 = __shfl_sync(0xffffffffu, scale, 8 * c + 4);   // of query rows 2c, 2c + 1
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) { o[u][e][0] *= f0; o[u][e][1] *= f1; o[u][e][2] *= f0; o[u][e][3] *= f1; }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] = ex2_approx(x[e] + (kShift - m));
+            l += x[e];
+        }
+        const uint32_t b0 = bits(__floats2half2_rn(x[0], x[1])), b1 = bits(__floats2half2_rn(x[2], x[3]));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            uint32_t f[4][4];
+            vf.operands(u, f);
+#pragma unroll
+            for (int e = 0; e < 4; e++) mma16816(o[u][e], f[e], b0, b1);
+        }
+    }
+    // the eight warps' shares
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (c == 0) { m_s[warp][r] = m; l_s[warp][r] = l; }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) o_s[warp][2 * c + (x & 1)][VFrag<KIND, HD>::dim(u, r) + 2 * e + (x >> 1)] = o[u][e][x];
+    __syncthreads();
+    constexpr int PER = kRows * HD / (kWarps * 32);   // values of the result a thread joins: one row, PER neighbouring columns
+    const int jr = threadIdx.x * PER / HD, jc = threadIdx.x * PER % HD;
+    float M = -FLT_MAX, L = 0.f, O[PER] = {};
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) M = fmaxf(M, m_s[w][jr]);
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        const float f = ex2_approx(m_s[w][jr] - M);
+        L = fmaf(l_s[w][jr], f, L);
+#pragma unroll
+        for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][jr][jc + e], f, O[e]);
+    }
+    float check = L * 0.f;   // a NaN once anything is not finite
+#pragma unroll
+    for (int e = 0; e < PER; e++) check = fmaf(O[e], 0.f, check);
+    const bool live = jr < rows;
+    M -= kShift;
+    __shared__ uint32_t bad;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    const int jrow = row0 + min(jr, rows - 1), ji = jrow / a.group, jh = kvh * a.group + jrow % a.group;
+    const bool sees = visible_run(a, a.start + ji, a.start + ji).len > 0;
+    // (a row that sees something has a sum above zero somewhere, but perhaps not in this share)
+    if (live && (check != 0.f || (a.n_split == 1 && sees && L == 0.f))) atomicOr(&bad, 1u << jr);
+    __syncthreads();
+    for (uint32_t todo = bad; todo; todo &= todo - 1) {   // uniform: rows next to infinite or NaN cache contents, one by one
+        const int y = __ffs(todo) - 1, again = row0 + y, i = again / a.group, head = kvh * a.group + again % a.group, pp = a.start + i;
+        constexpr int N = HD / 32;
+        const float k2 = rsqrtf((float)HD) * 1.4426950408889634f;
+        float qq[N], oo[N] = {}, mm = -FLT_MAX, ll = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; e++) qq[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * k2;
+        for (int w = v0 + warp; w < v1; w += kWarps) {
+            const int t = run.at(w);
+            if (!visible(a, pp, t)) continue;
+            float k[N], x[N], s = 0.f;
+            load_row<KIND, HD>(a.k, a.k_scale, base + t, lane, k);
+            load_row<KIND, HD>(a.v, a.v_scale, base + t, lane, x);
+#pragma unroll
+            for (int e = 0; e < N; e++) s = fmaf(qq[e], k[e], s);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+            const float m_new = fmaxf(mm, s), wt = exp2f(s - m_new), scale = exp2f(mm - m_new);
+            ll = ll * scale + wt;
+#pragma unroll
+            for (int e = 0; e < N; e++) oo[e] = fmaf(oo[e], scale, wt * x[e]);
+            mm = m_new;
+        }
+        __syncthreads();
+        if (lane == 0) { m_s[warp][0] = mm; l_s[warp][0] = ll; }
+#pragma unroll
+        for (int e = 0; e < N; e++) o_s[warp][0][lane * N + e] = oo[e];
+        __syncthreads();
+        if (jr == y) {
+            M = -FLT_MAX;
+            L = 0.f;
+            for (int w = 0; w < kWarps; w++) M = fmaxf(M, m_s[w][0]);
+#pragma unroll
+            for (int e = 0; e < PER; e++) O[e] = 0.f;
+            for (int w = 0; w < kWarps; w++) {
+                const float f = exp2f(m_s[w][0] - M);
+                L = fmaf(l_s[w][0], f, L);
+#pragma unroll
+                for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][0][jc + e], f, O[e]);
+            }
+        }
+    }
+    if (!live) return;
+    if (a.n_split > 1) {
+        const int64_t rec = ((int64_t)ji * a.heads + jh) * a.n_split + blockIdx.y;
+#pragma unroll
+        for (int e = 0; e < PER; e++) a.rec_o[rec * HD + jc + e] = O[e];
+        if (jc == 0) a.rec_ml[rec] = make_float2(M, L);
+    } else {
+        const float inv = sees ? 1.0f / L : 0.f;
+        __half* dst = reinterpret_cast<__half*>(a.out) + ji * a.out_ld + (int64_t)jh * HD + jc;
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) *reinterpret_cast<__half2*>(dst + e) = sees ? __floats2half2_rn(O[e] * inv, O[e + 1] * inv) : __half2half2(__ushort_as_half(0));
+    }
+}
+
+template <int KIND, int HD>
+int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
+    const int64_t blocks = ((int64_t)a.n * a.group + kRows - 1) / kRows;
+    attn_long_few_kernel<KIND, HD><<<dim3((unsigned)(blocks * a.kv_heads), a.n_split), kWarps * 32, 0, ctx->stream>>>(a);
+    RLB_LAUNCH_CHECK();
+    count_launch(ctx);
+    return RLB_OK;
+}
+
+}  // namespace
+
+int attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+    const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
+    const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + kRows / a.group, (int64_t)a.start + a.n);
+    // at least a tile of 16 positions for every warp
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / ctas, 256), (seen + kWarps * 16 - 1) / (kWarps * 16)));
+}
+
+int launch_attn_long_few(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+    if (kind == CACHE_F16) return a.hd == 128 ? launch<CACHE_F16, 128>(ctx, a) : launch<CACHE_F16, 64>(ctx, a);
+    return a.hd == 128 ? launch<CACHE_Q4, 128>(ctx, a) : launch<CACHE_Q4, 64>(ctx, a);
+}
