@@ -69,20 +69,61 @@ __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a
     }
 }
 
-// Joins the splits of a row; a CTA of HD threads per row.
-template <typename OT>
-__global__ void __launch_bounds__(128) attn_long_merge_kernel(const AttnLongArgs a) {
+// Joins the splits of a row: a CTA a row, its eight warps take every eighth split, a lane HD / 32 columns.
+template <typename OT, int HD>
+__global__ void __launch_bounds__(256) attn_long_merge_kernel(const __grid_constant__ AttnLongArgs a) {
+    constexpr int N = HD / 32;
+    __shared__ float o_s[8][HD], m_s[8], l_s[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = blockIdx.x;
     const int i = (int)(r / a.heads), head = (int)(r % a.heads), p = a.start + i;
-    float M = -FLT_MAX, L = 0.f, O = 0.f;
-    for (int s = 0; s < a.n_split; s++) M = fmaxf(M, a.rec_ml[r * a.n_split + s].x);
-    for (int s = 0; s < a.n_split; s++) {
-        const float2 ml = a.rec_ml[r * a.n_split + s];
-        const float f = exp2f(ml.x - M);
-        L = fmaf(ml.y, f, L);
-        O = fmaf(a.rec_o[(r * a.n_split + s) * a.hd + threadIdx.x], f, O);
+    rlb_pdl_wait();   // launched while the kernel that writes the records drains
+    const float2* ml = a.rec_ml + r * a.n_split;
+    const float* rec = a.rec_o + r * a.n_split * HD + lane * N;
+    float m = -FLT_MAX, l = 0.f, o[N] = {};
+#pragma unroll 4
+    for (int s = warp; s < a.n_split; s += 8) {
+        const float2 x = ml[s];
+        float y[N];
+        if constexpr (N == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(rec + (int64_t)s * HD);
+        else *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(rec + (int64_t)s * HD);
+        const float m_new = fmaxf(m, x.x), f = exp2f(m - m_new), g = exp2f(x.x - m_new);
+        l = l * f + x.y * g;
+#pragma unroll
+        for (int e = 0; e < N; e++) o[e] = o[e] * f + y[e] * g;
+        m = m_new;
     }
-    store_out(reinterpret_cast<OT*>(a.out) + i * a.out_ld + head * a.hd + threadIdx.x, visible_run(a, p, p).len > 0 ? O / L : 0.f);
+    if (lane == 0) { m_s[warp] = m; l_s[warp] = l; }
+#pragma unroll
+    for (int e = 0; e < N; e++) o_s[warp][lane * N + e] = o[e];
+    __syncthreads();
+    if (threadIdx.x >= HD) return;
+    float M = -FLT_MAX, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) M = fmaxf(M, m_s[w]);
+#pragma unroll
+    for (int w = 0; w < 8; w++) {
+        const float f = exp2f(m_s[w] - M);
+        L = fmaf(l_s[w], f, L);
+        O = fmaf(o_s[w][threadIdx.x], f, O);
+    }
+    store_out(reinterpret_cast<OT*>(a.out) + i * a.out_ld + head * HD + threadIdx.x, visible_run(a, p, p).len > 0 ? O / L : 0.f);
+}
+
+template <typename OT, int HD>
+int launch_merge(rlb_ctx* ctx, const AttnLongArgs& a) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(a.n * a.heads));
+    lc.blockDim = dim3(256);
+    lc.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    RLB_CUDA(cudaLaunchKernelEx(&lc, attn_long_merge_kernel<OT, HD>, a));
+    count_launch(ctx);
+    return RLB_OK;
 }
 
 template <int HD>
@@ -134,10 +175,16 @@ int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, i
 int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     AttnLongArgs a = given;
     const bool tiles = kind != CACHE_F32 && (int64_t)a.n * a.group >= 64;
-    a.n_split = tiles ? attn_long_tc_splits(ctx, kind, a) : kind != CACHE_F32 ? attn_long_few_splits(ctx, kind, a) : rows_splits(ctx, a);
+    AttnSplit split;
+    if (kind != CACHE_F32 && !tiles) split = attn_long_few_splits(ctx, kind, a);
+    else {
+        split.n = tiles ? attn_long_tc_splits(ctx, kind, a) : rows_splits(ctx, a);
+        split.records = split.n > 1;
+    }
+    a.n_split = split.n;
     const int64_t rows = (int64_t)a.n * a.heads;
     OpWorkspace ws;
-    if (a.n_split > 1) {
+    if (split.records) {
         const size_t recs = (size_t)rows * a.n_split;
         RLB_TRY(ws.get(ctx, recs * (a.hd * sizeof(float) + sizeof(float2))));
         a.rec_o = (float*)ws.p;
@@ -146,11 +193,9 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     if (tiles) RLB_TRY(launch_attn_long_tc(ctx, kind, a));
     else if (kind != CACHE_F32) RLB_TRY(launch_attn_long_few(ctx, kind, a));
     else RLB_TRY(a.hd == 128 ? launch_rows<128>(ctx, a) : launch_rows<64>(ctx, a));
-    if (a.n_split > 1) {
-        if (kind == CACHE_F32) attn_long_merge_kernel<float><<<(unsigned)rows, a.hd, 0, ctx->stream>>>(a);
-        else attn_long_merge_kernel<__half><<<(unsigned)rows, a.hd, 0, ctx->stream>>>(a);
-        RLB_LAUNCH_CHECK();
-        count_launch(ctx);
+    if (split.records) {
+        if (kind == CACHE_F32) RLB_TRY(a.hd == 128 ? (launch_merge<float, 128>(ctx, a)) : (launch_merge<float, 64>(ctx, a)));
+        else RLB_TRY(a.hd == 128 ? (launch_merge<__half, 128>(ctx, a)) : (launch_merge<__half, 64>(ctx, a)));
     }
     return RLB_OK;
 }

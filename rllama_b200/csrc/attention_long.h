@@ -57,8 +57,13 @@ __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2hal
 
 }  // namespace attn_long
 
+// How many parts the positions of a row block are split into, and whether the parts are joined by a second kernel.
+struct AttnSplit {
+    int n;
+    bool records;
+};
 // attention_long_few.cu
-int attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
+AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 int launch_attn_long_few(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 // attention_long_tc.cu
 int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);

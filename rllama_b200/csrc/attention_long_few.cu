@@ -37,14 +37,21 @@ __device__ __forceinline__ float ex2_approx(float x) {
 }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
-// A thread's share of K in a tile: rows r and r + 8, of each HD / 4 values in chunks of eight, 8 (4 i + c) ...
+// The byte offsets of a cache row t0 in the arrays of a kind (codes or values, scales).
+template <int KIND, int HD> struct Bytes {
+    static constexpr int ROW = KIND == CACHE_Q4 ? HD / 2 : HD * 2, SCALES = KIND == CACHE_Q4 ? HD / 16 : 0;
+};
+template <typename T> __device__ __forceinline__ T fetch(const char* p) { return __ldg(reinterpret_cast<const T*>(p)); }
+
+// A thread's share of K in a tile: rows r and r + 8, of each HD / 4 values in chunks of eight, 8 (4 i + c) ... `row` and `scale` point to
+// the thread's part of a row and to the row's scales.
 template <int KIND, int HD> struct KFrag;
 template <int HD> struct KFrag<CACHE_F16, HD> {
     uint4 x[2][HD / 32];
-    __device__ __forceinline__ void load(const AttnLongArgs& a, int nt, int64_t row, int c) {
-        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.k) + row * HD) + c;
+    static __device__ __forceinline__ int part(int c) { return 16 * c; }
+    __device__ __forceinline__ void load(int nt, const char* row, const char*) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; i++) x[nt][i] = __ldg(p + 4 * i);
+        for (int i = 0; i < HD / 32; i++) x[nt][i] = fetch<uint4>(row + 64 * i);
     }
     __device__ __forceinline__ void chunk(int nt, int i, uint32_t (&h)[4]) const { h[0] = x[nt][i].x; h[1] = x[nt][i].y; h[2] = x[nt][i].z; h[3] = x[nt][i].w; }
 };
@@ -52,14 +59,14 @@ template <int HD> struct KFrag<CACHE_Q4, HD> {
     static constexpr int G = HD / kQ4Group;
     uint32_t w[2][G];
     __half d[2][G];
-    __device__ __forceinline__ void load(const AttnLongArgs& a, int nt, int64_t row, int c) {
-        const uint8_t* p = reinterpret_cast<const uint8_t*>(a.k) + row * (HD / 2) + c * (HD / 8);
+    static __device__ __forceinline__ int part(int c) { return c * (HD / 8); }
+    __device__ __forceinline__ void load(int nt, const char* row, const char* scale) {
         if constexpr (G == 4) {
-            *reinterpret_cast<uint4*>(w[nt]) = __ldg(reinterpret_cast<const uint4*>(p));
-            *reinterpret_cast<uint2*>(d[nt]) = __ldg(reinterpret_cast<const uint2*>(a.k_scale + row * G));
+            *reinterpret_cast<uint4*>(w[nt]) = fetch<uint4>(row);
+            *reinterpret_cast<uint2*>(d[nt]) = fetch<uint2>(scale);
         } else {
-            *reinterpret_cast<uint2*>(w[nt]) = __ldg(reinterpret_cast<const uint2*>(p));
-            *reinterpret_cast<uint32_t*>(d[nt]) = __ldg(reinterpret_cast<const uint32_t*>(a.k_scale + row * G));
+            *reinterpret_cast<uint2*>(w[nt]) = fetch<uint2>(row);
+            *reinterpret_cast<uint32_t*>(d[nt]) = fetch<uint32_t>(scale);
         }
     }
     __device__ __forceinline__ void chunk(int nt, int i, uint32_t (&h)[4]) const {
@@ -71,16 +78,17 @@ template <int HD> struct KFrag<CACHE_Q4, HD> {
     }
 };
 // A thread's share of V in a tile: positions 2c, 2c + 1, 2c + 8, 2c + 9, of each HD / 64 chunks of eight values. `dim` is a chunk's
-// first value; operand(u, e): pairs of positions of values 2e (a0, a2) and 2e + 1 (a1, a3) of chunk u.
+// first value; operands(u): pairs of positions of values 2e (f[e][0], f[e][2]) and 2e + 1 (f[e][1], f[e][3]) of chunk u.
 template <int KIND, int HD> struct VFrag;
 template <int HD> struct VFrag<CACHE_F16, HD> {
     static constexpr int U = HD / 64;
     uint4 x[4][U];
     static __device__ __forceinline__ int dim(int u, int r) { return 8 * (8 * u + r); }
-    __device__ __forceinline__ void load(const AttnLongArgs& a, int i, int64_t row, int r) {
-        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.v) + row * HD) + r;
+    static __device__ __forceinline__ int part(int r) { return 16 * r; }
+    static __device__ __forceinline__ int scale_part(int) { return 0; }
+    __device__ __forceinline__ void load(int i, const char* row, const char*) {
 #pragma unroll
-        for (int u = 0; u < U; u++) x[i][u] = __ldg(p + 8 * u);
+        for (int u = 0; u < U; u++) x[i][u] = fetch<uint4>(row + 128 * u);
     }
     __device__ __forceinline__ void operands(int u, uint32_t (&f)[4][4]) const {
 #pragma unroll
@@ -101,15 +109,15 @@ template <int HD> struct VFrag<CACHE_Q4, HD> {
     uint32_t w[4][U];
     __half d[4][U];
     static __device__ __forceinline__ int dim(int u, int r) { const int x = U * r + u; return 32 * (x % G) + 8 * (x / G); }
-    __device__ __forceinline__ void load(const AttnLongArgs& a, int i, int64_t row, int r) {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(a.v) + row * (HD / 2)) + U * r;
-        const __half* s = a.v_scale + row * G + (U * r) % G;   // (a thread's words belong to neighbouring groups)
+    static __device__ __forceinline__ int part(int r) { return 4 * U * r; }
+    static __device__ __forceinline__ int scale_part(int r) { return 2 * ((U * r) % G); }   // (a thread's words belong to neighbouring groups)
+    __device__ __forceinline__ void load(int i, const char* row, const char* scale) {
         if constexpr (U == 2) {
-            *reinterpret_cast<uint2*>(w[i]) = __ldg(reinterpret_cast<const uint2*>(p));
-            *reinterpret_cast<uint32_t*>(d[i]) = __ldg(reinterpret_cast<const uint32_t*>(s));
+            *reinterpret_cast<uint2*>(w[i]) = fetch<uint2>(row);
+            *reinterpret_cast<uint32_t*>(d[i]) = fetch<uint32_t>(scale);
         } else {
-            w[i][0] = __ldg(p);
-            d[i][0] = __ldg(s);
+            w[i][0] = fetch<uint32_t>(row);
+            d[i][0] = __ushort_as_half(fetch<unsigned short>(scale));
         }
     }
     __device__ __forceinline__ void operands(int u, uint32_t (&f)[4][4]) const {
@@ -128,10 +136,20 @@ template <int HD> struct VFrag<CACHE_Q4, HD> {
     }
 };
 
-template <int KIND, int HD>
+// Shared memory of another CTA of the cluster.
+__device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
+    uint32_t x;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return x;
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// CLUSTER: the splits of a row block form a thread-block cluster (at most kWarps of them) and meet in the first one's shared memory.
+template <int KIND, int HD, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_long_few_kernel(const __grid_constant__ AttnLongArgs a) {
     constexpr int KS = HD / 16, U = VFrag<KIND, HD>::U;
-    __shared__ float o_s[kWarps][kRows][HD];
+    __shared__ __align__(16) float o_s[kWarps][kRows][HD];
     __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
     const int n_rows = a.n * a.group, blocks = (n_rows + kRows - 1) / kRows;
@@ -143,19 +161,37 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
     const int v0 = min(run.len, (int)blockIdx.y * chunk), v1 = min(run.len, v0 + chunk);
     const int64_t base = (int64_t)kvh * a.max_seq;
 
-    KFrag<KIND, HD> kf;
-    VFrag<KIND, HD> vf;
+    typedef Bytes<KIND, HD> Y;
+    KFrag<KIND, HD> kf, kn;   // this tile's and the next one's
+    VFrag<KIND, HD> vf, vn;
+    const char* k_p = reinterpret_cast<const char*>(a.k) + base * Y::ROW + KFrag<KIND, HD>::part(c);
+    const char* v_p = reinterpret_cast<const char*>(a.v) + base * Y::ROW + VFrag<KIND, HD>::part(r);
+    const char* k_d = reinterpret_cast<const char*>(a.k_scale) + base * Y::SCALES;
+    const char* v_d = reinterpret_cast<const char*>(a.v_scale) + base * Y::SCALES + VFrag<KIND, HD>::scale_part(r);
     const int last = max(v1 - 1, 0);   // (positions behind the share read its last one and weigh nothing)
-    auto load_k = [&](int v) {
+    auto load = [&](int v, KFrag<KIND, HD>& kf, VFrag<KIND, HD>& vf) {
+        if (v + 16 <= v1 && (v >= run.s || v + 16 <= run.s)) {   // 16 neighbouring rows
+            const int64_t t = run.at(v), tr = t + r, tc = t + 2 * c;
+            const char *kr = k_p + tr * Y::ROW, *kd = k_d + tr * Y::SCALES, *vr = v_p + tc * Y::ROW, *vd = v_d + tc * Y::SCALES;
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) kf.load(a, nt, base + run.at(min(v + 8 * nt + r, last)), c);
-    };
-    auto load_v = [&](int v) {
+            for (int nt = 0; nt < 2; nt++) kf.load(nt, kr + nt * 8 * Y::ROW, kd + nt * 8 * Y::SCALES);
 #pragma unroll
-        for (int i = 0; i < 4; i++) vf.load(a, i, base + run.at(min(v + 2 * c + (i & 1) + 8 * (i >> 1), last)), r);
+            for (int i = 0; i < 4; i++) vf.load(i, vr + ((i & 1) + 8 * (i >> 1)) * Y::ROW, vd + ((i & 1) + 8 * (i >> 1)) * Y::SCALES);
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                const int64_t t = run.at(min(v + 8 * nt + r, last));
+                kf.load(nt, k_p + t * Y::ROW, k_d + t * Y::SCALES);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t t = run.at(min(v + 2 * c + (i & 1) + 8 * (i >> 1), last));
+                vf.load(i, v_p + t * Y::ROW, v_d + t * Y::SCALES);
+            }
+        }
     };
     int v = v0 + warp * 16;
-    if (v < v1) load_k(v);
+    if (v < v1) load(v, kn, vn);
 
     // the queries: rows r (high halves) and r + 8 (low halves) of the A operand
     const int row = row0 + min(r, rows - 1), p = a.start + row / a.group, low = window_low(a, p);
@@ -190,7 +226,9 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
     }
     float o[U][4][4] = {}, m = -FLT_MAX, l = 0.f;
     for (; v < v1; v += kWarps * 16) {
-        load_v(v);
+        kf = kn;
+        vf = vn;
+        if (v + kWarps * 16 < v1) load(v + kWarps * 16, kn, vn);
         float s[2][4] = {};
 #pragma unroll
         for (int i = 0; i < HD / 32; i++)
@@ -201,7 +239,6 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
                 mma16816(s[nt], q[2 * i], h[0], h[1]);
                 mma16816(s[nt], q[2 * i + 1], h[2], h[3]);
             }
-        if (v + kWarps * 16 < v1) load_k(v + kWarps * 16);
         float x[4];   // scores of the thread's row at positions 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
         for (int e = 0; e < 4; e++) x[e] = (s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)]) * c2;
@@ -318,8 +355,31 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
             }
         }
     }
+    if constexpr (CLUSTER) {
+        cluster_sync();   // every CTA has joined its warps: the first one's shared memory may be written
+        const uint32_t to = blockIdx.y;
+#pragma unroll
+        for (int e = 0; e < PER; e++) cluster_store(cluster_map(&o_s[to][jr][jc + e], 0), O[e]);
+        if (jc == 0) {
+            cluster_store(cluster_map(&m_s[to][jr], 0), M);
+            cluster_store(cluster_map(&l_s[to][jr], 0), L);
+        }
+        cluster_sync();
+        if (blockIdx.y != 0) return;
+        M = -FLT_MAX;
+        for (int w = 0; w < a.n_split; w++) M = fmaxf(M, m_s[w][jr]);
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; e++) O[e] = 0.f;
+        for (int w = 0; w < a.n_split; w++) {
+            const float f = ex2_approx(m_s[w][jr] - M);
+            L = fmaf(l_s[w][jr], f, L);
+#pragma unroll
+            for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][jr][jc + e], f, O[e]);
+        }
+    }
     if (!live) return;
-    if (a.n_split > 1) {
+    if (!CLUSTER && a.n_split > 1) {
         const int64_t rec = ((int64_t)ji * a.heads + jh) * a.n_split + blockIdx.y;
 #pragma unroll
         for (int e = 0; e < PER; e++) a.rec_o[rec * HD + jc + e] = O[e];
@@ -335,19 +395,36 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
 template <int KIND, int HD>
 int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
     const int64_t blocks = ((int64_t)a.n * a.group + kRows - 1) / kRows;
-    attn_long_few_kernel<KIND, HD><<<dim3((unsigned)(blocks * a.kv_heads), a.n_split), kWarps * 32, 0, ctx->stream>>>(a);
-    RLB_LAUNCH_CHECK();
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(blocks * a.kv_heads), a.n_split);
+    lc.blockDim = dim3(kWarps * 32);
+    lc.stream = ctx->stream;
+    if (a.n_split > 1 && a.rec_o == nullptr) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1;
+        attr[0].val.clusterDim.y = (unsigned)a.n_split;
+        attr[0].val.clusterDim.z = 1;
+        lc.attrs = attr;
+        lc.numAttrs = 1;
+        RLB_CUDA(cudaLaunchKernelEx(&lc, attn_long_few_kernel<KIND, HD, true>, a));
+    } else {
+        RLB_CUDA(cudaLaunchKernelEx(&lc, attn_long_few_kernel<KIND, HD, false>, a));
+    }
     count_launch(ctx);
     return RLB_OK;
 }
 
 }  // namespace
 
-int attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + kRows / a.group, (int64_t)a.start + a.n);
     // at least a tile of 16 positions for every warp
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / ctas, 256), (seen + kWarps * 16 - 1) / (kWarps * 16)));
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / ctas, 256), (seen + kWarps * 16 - 1) / (kWarps * 16)));
+    // a cluster joins its splits without a second kernel
+    if (most <= kWarps) return {(int)most, false};
+    return {(int)most, true};
 }
 
 int launch_attn_long_few(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
