@@ -1,18 +1,24 @@
 // Long-context attention of few query rows (a generated token, a handful of drafted ones) over f16 and 4-bit caches:
-// attention_long.cu says what is computed. The time is that of reading the cache, so every K/V row is fetched once for up to eight query rows
-// that share its head (row = i * group + g, as in attention_long_tc.cu), straight from global memory into the registers
-// in which mma.sync takes it; nothing passes through shared memory.
+// attention_long.cu says what is computed. The time is that of reading the cache, so every K/V row is fetched once for up to
+// eight query rows that share its head (row = i * group + g, as in attention_long_tc.cu).
 //
-// A CTA takes eight rows of a K/V head and a share of the positions that they see; each of its eight warps walks tiles of 16
-// positions of that share:
-//  * S (16 x 8 positions, twice) = [q hi; q lo] K^T: the eight queries as two f16 halves each, x = hi + lo, are the 16 rows of
-//    the A operand, so the scores carry 22 bits of the queries at no further MMA. A thread's share of K is 16 contiguous
-//    bytes of a row (or 4-bit words of every group, cache4.h): the contraction index may be ordered freely as long as the queries are
-//    ordered alike.
-//  * the weights 2^(s - m + 7) in f16 are then in the right place for the B operand of O^T = V^T P: there V is A, its rows the values,
-//    its columns the positions; pairs of positions are interleaved with one byte permutation a register.
+// A CTA takes eight rows of a K/V head and a share of the positions that they see. A warp of its own keeps a ring of stages
+// of 128 positions full with bulk copies (neighbouring rows are one piece of memory); each of eight warps takes 16
+// positions of a stage:
+//  * S (16 x 8 positions, twice) = [q hi; q lo] K^T with mma.sync: the eight queries as two f16 halves each, x = hi + lo, are
+//    the 16 rows of the A operand, so the scores carry 22 bits of the queries at no further MMA. A thread's share of K is
+//    16 contiguous bytes of a row (or one 4-bit word of every group, cache4.h): the contraction index may be ordered
+//    freely as long as the queries are ordered alike.
+//  * the weights 2^(s - m + 7) in f16 are then in the right place for the B operand of O^T = V^T P: there V is A, its rows the
+//    values, its columns the positions; pairs of positions are interleaved with one byte permutation a register.
+// The positions of a tile are dealt to the 2 x 8 columns of S so that a thread's four scores belong to positions c, 4 + c, 8 + c, 12 + c: the
+// rows of V that the four threads of a column read side by side are then neighbours in shared memory.
 // The running maximum m moves only when a score exceeds it by 2^8, as in attention_long_tc.cu, and a row whose result is not
-// finite is computed again from what it sees alone. Scores, maxima, sums and O are f32; rounded to f16: the weights (2^-11) and the result.
+// finite is computed again from what it sees alone. Scores, maxima, sums and O are f32; rounded to f16: the weights
+// (2^-11) and the result.
+//
+// Loads straight into registers (two tiles ahead: 141 us, one: 107, of 65536 positions, 32 heads, 4 bits) wait for one another: a warp
+// tells its outstanding loads apart by six counters only.
 #include <algorithm>
 
 #include "attention_long.h"
@@ -25,59 +31,68 @@ constexpr int kRows = 8;    // query rows of a CTA
 constexpr int kWarps = 8;
 constexpr float kShift = 7.f, kLag = 8.f;
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+// d = a b + c with another c than d.
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, float c01, float c23) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %11, %11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(c01), "f"(c23));
 }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
-// The byte offsets of a cache row t0 in the arrays of a kind (codes or values, scales).
-template <int KIND, int HD> struct Bytes {
-    static constexpr int ROW = KIND == CACHE_Q4 ? HD / 2 : HD * 2, SCALES = KIND == CACHE_Q4 ? HD / 16 : 0;
+// The ring: stages of POS positions, [K rows][V rows][K scales][V scales]; 4 bits: two CTAs share an SM.
+template <int KIND, int HD> struct Ring {
+    static constexpr int POS = kWarps * 16, ROW = KIND == CACHE_Q4 ? HD / 2 : HD * 2, SCALES = KIND == CACHE_Q4 ? HD / 16 : 0;
+    static constexpr int V = POS * ROW, KD = 2 * POS * ROW, VD = KD + POS * SCALES, STAGE = KD + 2 * POS * SCALES;
+    static constexpr int STAGES = KIND == CACHE_Q4 ? (HD == 128 ? 4 : 8) : (HD == 128 ? 3 : 6);
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE;
 };
-template <typename T> __device__ __forceinline__ T fetch(const char* p) { return __ldg(reinterpret_cast<const T*>(p)); }
+template <typename T> __device__ __forceinline__ T fetch(const char* p) { return *reinterpret_cast<const T*>(p); }
 
-// A thread's share of K in a tile: rows r and r + 8, of each HD / 4 values in chunks of eight, 8 (4 i + c) ... `row` and `scale` point to
-// the thread's part of a row and to the row's scales.
+// A thread's share of K in a tile: two rows, of each HD / 4 values in chunks of eight, 8 (4 i + c) ... `row` points to
+// the thread's part of a row.
 template <int KIND, int HD> struct KFrag;
 template <int HD> struct KFrag<CACHE_F16, HD> {
     uint4 x[2][HD / 32];
     static __device__ __forceinline__ int part(int c) { return 16 * c; }
-    __device__ __forceinline__ void load(int nt, const char* row, const char*) {
+    __device__ __forceinline__ void load(int nt, const char* row) {
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) x[nt][i] = fetch<uint4>(row + 64 * i);
     }
     __device__ __forceinline__ void chunk(int nt, int i, uint32_t (&h)[4]) const { h[0] = x[nt][i].x; h[1] = x[nt][i].y; h[2] = x[nt][i].z; h[3] = x[nt][i].w; }
 };
+// Of a 4-bit row only the codes: a nibble alone in the low bits of an f16 IS a number, u + 8 times 2^-24 (or 2^-20 for the upper
+// nibble of a byte), so one AND makes a pair of operands. The factor 16 goes into the queries, the 8 into the accumulator's
+// start, and the scales, one for 32 values, multiply each group's sum afterwards.
 template <int HD> struct KFrag<CACHE_Q4, HD> {
     static constexpr int G = HD / kQ4Group;
     uint32_t w[2][G];
-    __half d[2][G];
     static __device__ __forceinline__ int part(int c) { return c * (HD / 8); }
-    __device__ __forceinline__ void load(int nt, const char* row, const char* scale) {
-        if constexpr (G == 4) {
-            *reinterpret_cast<uint4*>(w[nt]) = fetch<uint4>(row);
-            *reinterpret_cast<uint2*>(d[nt]) = fetch<uint2>(scale);
-        } else {
-            *reinterpret_cast<uint2*>(w[nt]) = fetch<uint2>(row);
-            *reinterpret_cast<uint32_t*>(d[nt]) = fetch<uint32_t>(scale);
-        }
+    __device__ __forceinline__ void load(int nt, const char* row) {
+        if constexpr (G == 4) *reinterpret_cast<uint4*>(w[nt]) = fetch<uint4>(row);
+        else *reinterpret_cast<uint2*>(w[nt]) = fetch<uint2>(row);
     }
     __device__ __forceinline__ void chunk(int nt, int i, uint32_t (&h)[4]) const {
-        __half2 v[4];
-        q4_pairs(w[nt][i], v);
-        const __half2 dd = __half2half2(d[nt][i]);
-#pragma unroll
-        for (int e = 0; e < 4; e++) h[e] = bits(__hmul2(v[e], dd));
+        const uint32_t x = w[nt][i], y = x >> 8;
+        h[0] = x & 0x000F000Fu; h[1] = x & 0x00F000F0u; h[2] = y & 0x000F000Fu; h[3] = y & 0x00F000F0u;
     }
 };
-// A thread's share of V in a tile: positions 2c, 2c + 1, 2c + 8, 2c + 9, of each HD / 64 chunks of eight values. `dim` is a chunk's
+// The scales of K at positions c, 4 + c, 8 + c, 12 + c of a tile, where the scores are.
+template <int KIND, int HD> struct KScales {
+    __device__ __forceinline__ void load(int, const char*) {}
+};
+template <int HD> struct KScales<CACHE_Q4, HD> {
+    __half d[4][HD / kQ4Group];
+    __device__ __forceinline__ void load(int i, const char* p) {
+        if constexpr (HD == 128) *reinterpret_cast<uint2*>(d[i]) = fetch<uint2>(p);
+        else *reinterpret_cast<uint32_t*>(d[i]) = fetch<uint32_t>(p);
+    }
+};
+// A thread's share of V in a tile: positions c, 4 + c, 8 + c, 12 + c, of each HD / 64 chunks of eight values. `dim` is a chunk's
 // first value; operands(u): pairs of positions of values 2e (f[e][0], f[e][2]) and 2e + 1 (f[e][1], f[e][3]) of chunk u.
 template <int KIND, int HD> struct VFrag;
 template <int HD> struct VFrag<CACHE_F16, HD> {
@@ -122,7 +137,7 @@ template <int HD> struct VFrag<CACHE_Q4, HD> {
     }
     __device__ __forceinline__ void operands(int u, uint32_t (&f)[4][4]) const {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {   // positions 2c, 2c + 1, then 2c + 8, 2c + 9
+        for (int h = 0; h < 2; h++) {   // positions c, 4 + c, then 8 + c, 12 + c
             const __half2 dd = __halves2half2(d[2 * h][u], d[2 * h + 1][u]);
             __half2 even[4], odd[4];
             q4_pairs(__byte_perm(w[2 * h][u], w[2 * h + 1][u], 0x5410), even);
@@ -145,13 +160,33 @@ __device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+template <int N> __device__ __forceinline__ void async_copy(void* dst, const void* src) {   // 4 or 8 bytes
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(N) : "memory");
+}
+__device__ __forceinline__ void async_arrive(uint64_t* bar) {   // once the thread's copies are there
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // CLUSTER: the splits of a row block form a thread-block cluster (at most kWarps of them) and meet in the first one's shared memory.
 template <int KIND, int HD, bool CLUSTER>
-__global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_long_few_kernel(const __grid_constant__ AttnLongArgs a) {
-    constexpr int KS = HD / 16, U = VFrag<KIND, HD>::U;
-    __shared__ __align__(16) float o_s[kWarps][kRows][HD];
+__global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) attn_long_few_kernel(const __grid_constant__ AttnLongArgs a, int* err) {
+    typedef Ring<KIND, HD> Y;
+    constexpr int KS = HD / 16, U = VFrag<KIND, HD>::U, STAGES = Y::STAGES;
+    extern __shared__ __align__(128) char ring[];
+    float (*o_s)[kRows][HD] = reinterpret_cast<float (*)[kRows][HD]>(ring);   // [warp], after the loop
+    static_assert(kWarps * kRows * HD * 4 <= STAGES * Y::STAGE, "the warps' results fit in the ring");
     __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+    __shared__ uint4 q_s[HD / 16][32];   // the queries as A operands, a lane's four registers of a product side by side
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
+    __shared__ int dead_flag;
+    __shared__ uint32_t bad;
+    volatile int* dead = &dead_flag;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), r = lane >> 2, c = lane & 3;   // (warp: known to be uniform)
     const int n_rows = a.n * a.group, blocks = (n_rows + kRows - 1) / kRows;
     const int kvh = blockIdx.x / blocks, row0 = (blockIdx.x % blocks) * kRows, rows = min(kRows, n_rows - row0);
     const int pa = a.start + row0 / a.group, pb = a.start + (row0 + rows - 1) / a.group;
@@ -161,153 +196,251 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
     const int v0 = min(run.len, (int)blockIdx.y * chunk), v1 = min(run.len, v0 + chunk);
     const int64_t base = (int64_t)kvh * a.max_seq;
 
-    typedef Bytes<KIND, HD> Y;
-    KFrag<KIND, HD> kf, kn;   // this tile's and the next one's
-    VFrag<KIND, HD> vf, vn;
-    const char* k_p = reinterpret_cast<const char*>(a.k) + base * Y::ROW + KFrag<KIND, HD>::part(c);
-    const char* v_p = reinterpret_cast<const char*>(a.v) + base * Y::ROW + VFrag<KIND, HD>::part(r);
-    const char* k_d = reinterpret_cast<const char*>(a.k_scale) + base * Y::SCALES;
-    const char* v_d = reinterpret_cast<const char*>(a.v_scale) + base * Y::SCALES + VFrag<KIND, HD>::scale_part(r);
-    const int last = max(v1 - 1, 0);   // (positions behind the share read its last one and weigh nothing)
-    auto load = [&](int v, KFrag<KIND, HD>& kf, VFrag<KIND, HD>& vf) {
-        if (v + 16 <= v1 && (v >= run.s || v + 16 <= run.s)) {   // 16 neighbouring rows
-            const int64_t t = run.at(v), tr = t + r, tc = t + 2 * c;
-            const char *kr = k_p + tr * Y::ROW, *kd = k_d + tr * Y::SCALES, *vr = v_p + tc * Y::ROW, *vd = v_d + tc * Y::SCALES;
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) kf.load(nt, kr + nt * 8 * Y::ROW, kd + nt * 8 * Y::SCALES);
-#pragma unroll
-            for (int i = 0; i < 4; i++) vf.load(i, vr + ((i & 1) + 8 * (i >> 1)) * Y::ROW, vd + ((i & 1) + 8 * (i >> 1)) * Y::SCALES);
-        } else {
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                const int64_t t = run.at(min(v + 8 * nt + r, last));
-                kf.load(nt, k_p + t * Y::ROW, k_d + t * Y::SCALES);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t t = run.at(min(v + 2 * c + (i & 1) + 8 * (i >> 1), last));
-                vf.load(i, v_p + t * Y::ROW, v_d + t * Y::SCALES);
-            }
+    if (threadIdx.x == 0) {
+        dead_flag = 0;
+        bad = 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], KIND == CACHE_Q4 ? 33 : 1);   // the announced bytes, and the scales' 32 threads
+            mbar_init(&empty[s], kWarps);
         }
-    };
-    int v = v0 + warp * 16;
-    if (v < v1) load(v, kn, vn);
-
-    // the queries: rows r (high halves) and r + 8 (low halves) of the A operand
-    const int row = row0 + min(r, rows - 1), p = a.start + row / a.group, low = window_low(a, p);
-    uint32_t q[KS][4];
-    float c2;
-    {
-        const float* src = a.q + (int64_t)(row / a.group) * a.q_ld + (int64_t)(kvh * a.group + row % a.group) * HD + 8 * c;
-        float x[KS][4], top = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            *reinterpret_cast<float4*>(x[s]) = *reinterpret_cast<const float4*>(src + 32 * (s >> 1) + 4 * (s & 1));
-#pragma unroll
-            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[s][e]));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // scaled by a power of two so that the row's largest element lies in [2^8, 2^9), whatever its magnitude
-        int e = (int)(__float_as_uint(top) >> 23) - 127;
-        e = e > 127 ? 0 : max(e, -100);
-        const float up = r < rows ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
-        c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float y0 = x[s][2 * h] * up, y1 = x[s][2 * h + 1] * up;
-                const __half2 hi = __floats2half2_rn(y0, y1);
-                const float2 f = __half22float2(hi);
-                q[s][2 * h] = bits(hi);
-                q[s][2 * h + 1] = bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
-            }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncthreads();
     float o[U][4][4] = {}, m = -FLT_MAX, l = 0.f;
-    for (; v < v1; v += kWarps * 16) {
-        kf = kn;
-        vf = vn;
-        if (v + kWarps * 16 < v1) load(v + kWarps * 16, kn, vn);
-        float s[2][4] = {};
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++)
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                uint32_t h[4];
-                kf.chunk(nt, i, h);
-                mma16816(s[nt], q[2 * i], h[0], h[1]);
-                mma16816(s[nt], q[2 * i + 1], h[2], h[3]);
+    if (warp == kWarps) {
+        // ------------------------------- keeps the ring full ---------------------------------------------------------
+        const char *k = reinterpret_cast<const char*>(a.k) + base * Y::ROW, *v = reinterpret_cast<const char*>(a.v) + base * Y::ROW;
+        uint32_t s = 0, phase = 1;
+        int p0 = v0, issued = 0;
+        for (; p0 < v1; p0 += Y::POS, issued++) {
+            if (issued >= STAGES && !warp_wait(&empty[s], phase, dead, err)) break;
+            char* dst = ring + s * Y::STAGE;
+            const int p1 = min(p0 + Y::POS, v1), cut = min(max(run.s, p0), p1);   // [p0, cut) of the first run, [cut, p1) of the second
+            if (lane == 0) {
+                mbar_expect_tx(&full[s], (uint32_t)(p1 - p0) * 2 * Y::ROW);
+                if (cut > p0) {
+                    bulk_load(dst, k + (int64_t)p0 * Y::ROW, (cut - p0) * Y::ROW, &full[s]);
+                    bulk_load(dst + Y::V, v + (int64_t)p0 * Y::ROW, (cut - p0) * Y::ROW, &full[s]);
+                }
+                if (p1 > cut) {
+                    const int64_t t = run.at(cut);
+                    bulk_load(dst + (cut - p0) * Y::ROW, k + t * Y::ROW, (p1 - cut) * Y::ROW, &full[s]);
+                    bulk_load(dst + Y::V + (cut - p0) * Y::ROW, v + t * Y::ROW, (p1 - cut) * Y::ROW, &full[s]);
+                }
             }
-        float x[4];   // scores of the thread's row at positions 2c, 2c + 1, 2c + 8, 2c + 9
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = (s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)]) * c2;
-        const int t0 = run.at(v), t1 = run.at(v + 15);
-        if (!(v + 16 <= v1 && t1 == t0 + 15 && t1 <= pa && (t0 >= window_low(a, pb) || t1 < a.sinks))) {   // some row does not see all of it
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int w = v + 2 * c + (e & 1) + 8 * (e >> 1), t = run.at(w);
-                if (!(w < v1 && t <= p && (t >= low || t < a.sinks))) x[e] = -INFINITY;
+            if constexpr (KIND == CACHE_Q4) {   // (8 or 4 bytes a row: no 16-byte boundary for a bulk copy to start at)
+                for (int x = lane; x < p1 - p0; x += 32) {
+                    const int64_t t = base + run.at(p0 + x);
+                    async_copy<Y::SCALES>(dst + Y::KD + x * Y::SCALES, reinterpret_cast<const char*>(a.k_scale) + t * Y::SCALES);
+                    async_copy<Y::SCALES>(dst + Y::VD + x * Y::SCALES, reinterpret_cast<const char*>(a.v_scale) + t * Y::SCALES);
+                }
+                async_arrive(&full[s]);
             }
+            if (++s == STAGES) { s = 0; phase ^= 1; }
         }
-        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        if (__any_sync(0xffffffffu, top > m + kLag)) {
+        for (int x = max(0, issued - STAGES); x < issued; x++) mbar_drain(&full[x % STAGES], (x / STAGES) & 1);   // no copy outlives the ring
+    } else {
+        // the queries: rows r (high halves) and r + 8 (low halves) of the A operand
+        const int row = row0 + min(r, rows - 1), p = a.start + row / a.group, low = window_low(a, p);
+        float k0[KIND == CACHE_Q4 ? HD / kQ4Group : 1][2] = {};   // -8 times a group's sum of the row's high and low halves, times 2^-24
+        float c2;
+        {
+            const float* src = a.q + (int64_t)(row / a.group) * a.q_ld + (int64_t)(kvh * a.group + row % a.group) * HD + 8 * c;
+            float x[KS][4], top = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                *reinterpret_cast<float4*>(x[s]) = *reinterpret_cast<const float4*>(src + 32 * (s >> 1) + 4 * (s & 1));
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[s][e]));
+            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m, top), scale = ex2_approx(m - m_new);
-            m = m_new;
-            l *= scale;
-            const float f0 = __shfl_sync(0xffffffffu, scale, 8 * c), f1 = __shfl_sync(0xffffffffu, scale, 8 * c + 4);   // of query rows 2c, 2c + 1
+            // scaled by a power of two so that the row's largest element lies in [2^8, 2^9), whatever its magnitude
+            int e = (int)(__float_as_uint(top) >> 23) - 127;
+            e = e > 127 ? 0 : max(e, -100);
+            const float up = r < rows ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
+            c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int s = 0; s < KS; s++) {
+                uint32_t q[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) { o[u][e][0] *= f0; o[u][e][1] *= f1; o[u][e][2] *= f0; o[u][e][3] *= f1; }
+                for (int h = 0; h < 2; h++) {
+                    const float y0 = x[s][2 * h] * up, y1 = x[s][2 * h + 1] * up;
+                    const __half2 hi = __floats2half2_rn(y0, y1);
+                    const float2 f = __half22float2(hi);
+                    const __half2 lo = __floats2half2_rn(y0 - f.x, y1 - f.y);
+                    if constexpr (KIND == CACHE_Q4) {
+                        const float2 g = __half22float2(lo);
+                        k0[s >> 1][0] += f.x + f.y;
+                        k0[s >> 1][1] += g.x + g.y;
+                        const __half2 k = __floats2half2_rn(h ? 0.0625f : 1.f, h ? 0.0625f : 1.f);   // (upper nibbles come 16 times as large)
+                        q[2 * h] = bits(__hmul2(hi, k));
+                        q[2 * h + 1] = bits(__hmul2(lo, k));
+                    } else {
+                        q[2 * h] = bits(hi);
+                        q[2 * h + 1] = bits(lo);
+                    }
+                }
+                if (warp == s % kWarps) q_s[s][lane] = make_uint4(q[0], q[1], q[2], q[3]);
+            }
+            if constexpr (KIND == CACHE_Q4) {
+#pragma unroll
+                for (int g = 0; g < HD / kQ4Group; g++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        k0[g][h] += __shfl_xor_sync(0xffffffffu, k0[g][h], 1);
+                        k0[g][h] += __shfl_xor_sync(0xffffffffu, k0[g][h], 2);
+                        k0[g][h] *= -8.f / 16777216.f;
+                    }
+                c2 *= 16777216.f;
+            }
         }
+        // the thread's places in a stage
+        const int kp = (warp * 16 + (r >> 1) + 4 * (r & 1)) * Y::ROW + KFrag<KIND, HD>::part(c), kd = Y::KD + (warp * 16 + c) * Y::SCALES;
+        const int vp = Y::V + (warp * 16 + c) * Y::ROW + VFrag<KIND, HD>::part(r), vd = Y::VD + (warp * 16 + c) * Y::SCALES + VFrag<KIND, HD>::scale_part(r);
+        // One tile, at virtual position v; `there`: how many of its positions are in the stage (those behind them read the last one
+        // and weigh nothing).
+        auto tile = [&](int v, const char* stage, int there) {
+            KFrag<KIND, HD> kf;
+            KScales<KIND, HD> ks;
+            VFrag<KIND, HD> vf;
+            if (there >= 16) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[e] = ex2_approx(x[e] + (kShift - m));
-            l += x[e];
-        }
-        const uint32_t b0 = bits(__floats2half2_rn(x[0], x[1])), b1 = bits(__floats2half2_rn(x[2], x[3]));
+                for (int nt = 0; nt < 2; nt++) kf.load(nt, stage + kp + nt * 8 * Y::ROW);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            uint32_t f[4][4];
-            vf.operands(u, f);
+                for (int e = 0; e < 4; e++) {
+                    ks.load(e, stage + kd + e * 4 * Y::SCALES);
+                    vf.load(e, stage + vp + e * 4 * Y::ROW, stage + vd + e * 4 * Y::SCALES);
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) mma16816(o[u][e], f[e], b0, b1);
+                for (int nt = 0; nt < 2; nt++) {
+                    const int x = (r >> 1) + 4 * (r & 1);
+                    kf.load(nt, stage + kp + (min(x + 8 * nt, there - 1) - x) * Y::ROW);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int x = min(4 * e + c, there - 1) - c;
+                    ks.load(e, stage + kd + x * Y::SCALES);
+                    vf.load(e, stage + vp + x * Y::ROW, stage + vd + x * Y::SCALES);
+                }
+            }
+            float x[4] = {};   // scores of the thread's row at positions c, 4 + c, 8 + c, 12 + c
+            if constexpr (KIND == CACHE_Q4) {
+#pragma unroll
+                for (int g = 0; g < HD / kQ4Group; g++)
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {
+                        uint32_t h[4];
+                        float s[4];
+                        kf.chunk(nt, g, h);
+                        mma16816(s, q_s[2 * g][lane], h[0], h[1], k0[g][0], k0[g][1]);
+                        mma16816(s, q_s[2 * g + 1][lane], h[2], h[3]);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) x[2 * nt + e] = fmaf(__half2float(ks.d[2 * nt + e][g]), s[e] + s[2 + e], x[2 * nt + e]);
+                    }
+            } else {
+                float s[2][4] = {};
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {
+                        uint32_t h[4];
+                        kf.chunk(nt, i, h);
+                        mma16816(s[nt], q_s[2 * i][lane], h[0], h[1]);
+                        mma16816(s[nt], q_s[2 * i + 1][lane], h[2], h[3]);
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] *= c2;
+            // (a block of one position sees all of its share)
+            bool whole = v + 16 <= v1 && (v >= run.s || v + 16 <= run.s);
+            if (pa != pb) { const int t0 = run.at(v); whole = whole && t0 + 15 <= pa && (t0 >= window_low(a, pb) || t0 + 15 < a.sinks); }
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int w = v + 4 * e + c, t = run.at(w);
+                    if (!(w < v1 && t <= p && (t >= low || t < a.sinks))) x[e] = -INFINITY;
+                }
+            }
+            float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            if (__any_sync(0xffffffffu, top > m + kLag)) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float m_new = fmaxf(m, top), scale = ex2_approx(m - m_new);
+                m = m_new;
+                l *= scale;
+                const float f0 = __shfl_sync(0xffffffffu, scale, 8 * c), f1 = __shfl_sync(0xffffffffu, scale, 8 * c + 4);   // of query rows 2c, 2c + 1
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { o[u][e][0] *= f0; o[u][e][1] *= f1; o[u][e][2] *= f0; o[u][e][3] *= f1; }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[e] = ex2_approx(x[e] + (kShift - m));
+                l += x[e];
+            }
+            const uint32_t b0 = bits(__floats2half2_rn(x[0], x[1])), b1 = bits(__floats2half2_rn(x[2], x[3]));
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                uint32_t f[4][4];
+                vf.operands(u, f);
+#pragma unroll
+                for (int e = 0; e < 4; e++) mma16816(o[u][e], make_uint4(f[e][0], f[e][1], f[e][2], f[e][3]), b0, b1);
+            }
+        };
+        asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");   // q_s
+        uint32_t s = 0, phase = 0;
+        for (int p0 = v0; p0 < v1; p0 += Y::POS) {
+            if (!warp_wait(&full[s], phase, dead, err)) break;
+            const int v = p0 + warp * 16;   // the warp's tile
+            if (v < v1) tile(v, ring + s * Y::STAGE, v1 - v);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+            if (++s == STAGES) { s = 0; phase ^= 1; }
         }
     }
-    // the eight warps' shares
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (c == 0) { m_s[warp][r] = m; l_s[warp][r] = l; }
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) o_s[warp][2 * c + (x & 1)][VFrag<KIND, HD>::dim(u, r) + 2 * e + (x >> 1)] = o[u][e][x];
+    // the eight warps' shares, in the ring's room
     __syncthreads();
-    constexpr int PER = kRows * HD / (kWarps * 32);   // values of the result a thread joins: one row, PER neighbouring columns
-    const int jr = threadIdx.x * PER / HD, jc = threadIdx.x * PER % HD;
-    float M = -FLT_MAX, L = 0.f, O[PER] = {};
+    if (warp < kWarps) {
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (c == 0) { m_s[warp][r] = m; l_s[warp][r] = l; }
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) M = fmaxf(M, m_s[w][jr]);
+        for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-        const float f = ex2_approx(m_s[w][jr] - M);
-        L = fmaf(l_s[w][jr], f, L);
+            for (int e = 0; e < 4; e++)
 #pragma unroll
-        for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][jr][jc + e], f, O[e]);
+                for (int x = 0; x < 4; x++) o_s[warp][2 * c + (x & 1)][VFrag<KIND, HD>::dim(u, r) + 2 * e + (x >> 1)] = o[u][e][x];
     }
+    __syncthreads();
+    constexpr int PER = kRows * HD / (kWarps * 32);   // values of the result a thread joins: of one row, PER neighbouring columns
+    const bool joins = warp < kWarps;
+    const int jr = joins ? threadIdx.x * PER / HD : 0, jc = threadIdx.x * PER % HD;
+    float M = -FLT_MAX, L = 0.f, O[PER] = {};
+    // Joins n partial results of a row.
+    auto join = [&](int n, int from) {
+        M = -FLT_MAX;
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; e++) O[e] = 0.f;
+        for (int w = 0; w < n; w++) M = fmaxf(M, m_s[w][from]);
+        for (int w = 0; w < n; w++) {
+            const float f = ex2_approx(m_s[w][from] - M);
+            L = fmaf(l_s[w][from], f, L);
+#pragma unroll
+            for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][from][jc + e], f, O[e]);
+        }
+    };
+    join(kWarps, jr);
+    M -= kShift;
     float check = L * 0.f;   // a NaN once anything is not finite
 #pragma unroll
     for (int e = 0; e < PER; e++) check = fmaf(O[e], 0.f, check);
-    const bool live = jr < rows;
-    M -= kShift;
-    __shared__ uint32_t bad;
-    if (threadIdx.x == 0) bad = 0;
-    __syncthreads();
+    const bool live = joins && jr < rows;
     const int jrow = row0 + min(jr, rows - 1), ji = jrow / a.group, jh = kvh * a.group + jrow % a.group;
     const bool sees = visible_run(a, a.start + ji, a.start + ji).len > 0;
     // (a row that sees something has a sum above zero somewhere, but perhaps not in this share)
@@ -320,7 +453,7 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
         float qq[N], oo[N] = {}, mm = -FLT_MAX, ll = 0.f;
 #pragma unroll
         for (int e = 0; e < N; e++) qq[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * k2;
-        for (int w = v0 + warp; w < v1; w += kWarps) {
+        for (int w = v0 + warp; joins && w < v1; w += kWarps) {
             const int t = run.at(w);
             if (!visible(a, pp, t)) continue;
             float k[N], x[N], s = 0.f;
@@ -337,46 +470,28 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
             mm = m_new;
         }
         __syncthreads();
-        if (lane == 0) { m_s[warp][0] = mm; l_s[warp][0] = ll; }
+        if (joins) {
+            if (lane == 0) { m_s[warp][0] = mm; l_s[warp][0] = ll; }
 #pragma unroll
-        for (int e = 0; e < N; e++) o_s[warp][0][lane * N + e] = oo[e];
-        __syncthreads();
-        if (jr == y) {
-            M = -FLT_MAX;
-            L = 0.f;
-            for (int w = 0; w < kWarps; w++) M = fmaxf(M, m_s[w][0]);
-#pragma unroll
-            for (int e = 0; e < PER; e++) O[e] = 0.f;
-            for (int w = 0; w < kWarps; w++) {
-                const float f = exp2f(m_s[w][0] - M);
-                L = fmaf(l_s[w][0], f, L);
-#pragma unroll
-                for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][0][jc + e], f, O[e]);
-            }
+            for (int e = 0; e < N; e++) o_s[warp][0][lane * N + e] = oo[e];
         }
+        __syncthreads();
+        if (jr == y) join(kWarps, 0);
     }
     if constexpr (CLUSTER) {
         cluster_sync();   // every CTA has joined its warps: the first one's shared memory may be written
         const uint32_t to = blockIdx.y;
+        if (joins) {
 #pragma unroll
-        for (int e = 0; e < PER; e++) cluster_store(cluster_map(&o_s[to][jr][jc + e], 0), O[e]);
-        if (jc == 0) {
-            cluster_store(cluster_map(&m_s[to][jr], 0), M);
-            cluster_store(cluster_map(&l_s[to][jr], 0), L);
+            for (int e = 0; e < PER; e++) cluster_store(cluster_map(&o_s[to][jr][jc + e], 0), O[e]);
+            if (jc == 0) {
+                cluster_store(cluster_map(&m_s[to][jr], 0), M);
+                cluster_store(cluster_map(&l_s[to][jr], 0), L);
+            }
         }
         cluster_sync();
         if (blockIdx.y != 0) return;
-        M = -FLT_MAX;
-        for (int w = 0; w < a.n_split; w++) M = fmaxf(M, m_s[w][jr]);
-        L = 0.f;
-#pragma unroll
-        for (int e = 0; e < PER; e++) O[e] = 0.f;
-        for (int w = 0; w < a.n_split; w++) {
-            const float f = ex2_approx(m_s[w][jr] - M);
-            L = fmaf(l_s[w][jr], f, L);
-#pragma unroll
-            for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][jr][jc + e], f, O[e]);
-        }
+        join(a.n_split, jr);
     }
     if (!live) return;
     if (!CLUSTER && a.n_split > 1) {
@@ -395,22 +510,26 @@ __global__ void __launch_bounds__(kWarps * 32, KIND == CACHE_Q4 ? 2 : 1) attn_lo
 template <int KIND, int HD>
 int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
     const int64_t blocks = ((int64_t)a.n * a.group + kRows - 1) / kRows;
+    const bool cluster = a.n_split > 1 && a.rec_o == nullptr;
+    auto kern = cluster ? attn_long_few_kernel<KIND, HD, true> : attn_long_few_kernel<KIND, HD, false>;
+    static std::atomic<uint64_t> set[2];
+    if (!attr_done(set[cluster], ctx->device)) {
+        RLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Ring<KIND, HD>::SMEM));
+        attr_mark(set[cluster], ctx->device);
+    }
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(blocks * a.kv_heads), a.n_split);
-    lc.blockDim = dim3(kWarps * 32);
+    lc.blockDim = dim3((kWarps + 1) * 32);
+    lc.dynamicSmemBytes = Ring<KIND, HD>::SMEM;
     lc.stream = ctx->stream;
-    if (a.n_split > 1 && a.rec_o == nullptr) {
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 1;
-        attr[0].val.clusterDim.y = (unsigned)a.n_split;
-        attr[0].val.clusterDim.z = 1;
-        lc.attrs = attr;
-        lc.numAttrs = 1;
-        RLB_CUDA(cudaLaunchKernelEx(&lc, attn_long_few_kernel<KIND, HD, true>, a));
-    } else {
-        RLB_CUDA(cudaLaunchKernelEx(&lc, attn_long_few_kernel<KIND, HD, false>, a));
-    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)a.n_split;
+    attr[0].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = cluster ? 1 : 0;
+    RLB_CUDA(cudaLaunchKernelEx(&lc, kern, a, ctx->d_err));
     count_launch(ctx);
     return RLB_OK;
 }

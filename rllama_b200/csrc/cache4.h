@@ -37,7 +37,9 @@ __device__ __forceinline__ void q4_pairs(uint32_t word, __half2 (&h)[4]) {
 #pragma unroll
     for (int b = 0; b < 2; b++) {
         const uint32_t w = b ? word >> 8 : word;
-        const uint32_t lo = (w & 0x000F000Fu) | 0x64006400u, hi = (w & 0x00F000F0u) | 0x64006400u;
+        uint32_t lo, hi;   // (w & mask) | 0x64006400
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(lo) : "r"(w), "r"(0x000F000Fu), "r"(0x64006400u));
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(hi) : "r"(w), "r"(0x00F000F0u), "r"(0x64006400u));
         h[2 * b] = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&bias));
         h[2 * b + 1] = __hfma2(*reinterpret_cast<const __half2*>(&hi), *reinterpret_cast<const __half2*>(&sixteenth), *reinterpret_cast<const __half2*>(&high_bias));
     }
