@@ -8,9 +8,9 @@
 // All of it is f32; a cache row is rounded once, to the cache's dtype.
 #include "internal.h"
 
+#include <algorithm>
 #include <cmath>
 #include <new>
-#include <vector>
 
 namespace {
 
@@ -41,54 +41,65 @@ template <typename CT, int N> __device__ __forceinline__ void store_cache(CT* p,
     }
 }
 
-// A warp per (token, slot); slots are the q heads, the k heads and the v heads. A lane holds HD / 32 neighbouring values,
-// i.e. whole pairs, and the norm's sum is one reduction over the warp.
+// grid (slots / 8, tokens): a warp per slot (the q heads, the k heads, the v heads) and U tokens, whose loads are all in flight. A lane
+// holds HD / 32 neighbouring values, i.e. whole pairs, and the norm's sum is one reduction over the warp.
+constexpr int U = 4;
+
 template <typename CT, int HD>
-__global__ void __launch_bounds__(256) norm_rope_append_kernel(const RotateArgs a) {
+__global__ void __launch_bounds__(256) norm_rope_append_kernel(const __grid_constant__ RotateArgs a) {
     constexpr int N = HD / 32;
     typedef typename Vec<N>::T V;
-    const int slots = a.heads + 2 * a.kv_heads;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (w >= (int64_t)a.n * slots) return;
-    const int i = (int)(w / slots), slot = (int)(w % slots), c = (threadIdx.x & 31) * N;
+    const int slot = blockIdx.x * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * N;
+    if (slot >= a.heads + 2 * a.kv_heads) return;
     const int kind = slot < a.heads ? 0 : slot < a.heads + a.kv_heads ? 1 : 2;
     const int head = kind == 0 ? slot : kind == 1 ? slot - a.heads : slot - a.heads - a.kv_heads;
-    const float* src = kind == 0 ? a.q + i * a.q_ld : kind == 1 ? a.k + i * a.k_ld : a.v + i * a.v_ld;
-    float x[N];
-    *reinterpret_cast<V*>(x) = *reinterpret_cast<const V*>(src + head * HD + c);
-    const int pos = a.start + i;
-    const int64_t row = ((int64_t)head * a.max_seq + pos) * HD + c;
-    if (kind == 2) {
-        store_cache<CT, N>(reinterpret_cast<CT*>(a.vcache) + row, x);
-        return;
+    const float* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + head * HD + c;
+    const int64_t ld = kind == 0 ? a.q_ld : kind == 1 ? a.k_ld : a.v_ld;
+    const float* gain = kind == 0 ? a.q_gain : kind == 1 ? a.k_gain : nullptr;
+    float g[N];
+    if (gain) *reinterpret_cast<V*>(g) = *reinterpret_cast<const V*>(gain + c);
+    for (int i0 = blockIdx.y * U; i0 < a.n; i0 += gridDim.y * U) {
+        float x[U][N], f[U][N];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = min(i0 + u, a.n - 1);
+            *reinterpret_cast<V*>(x[u]) = *reinterpret_cast<const V*>(src + i * ld);
+            if (kind != 2) *reinterpret_cast<V*>(f[u]) = *reinterpret_cast<const V*>(a.table + (a.start + i) * a.table_ld + c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u;
+            if (i >= a.n) break;
+            const int64_t row = ((int64_t)head * a.max_seq + a.start + i) * HD + c;
+            if (kind == 2) {
+                store_cache<CT, N>(reinterpret_cast<CT*>(a.vcache) + row, x[u]);
+                continue;
+            }
+            if (gain) {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < N; e++) ss = fmaf(x[u][e], x[u][e], ss);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float s = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+                for (int e = 0; e < N; e++) x[u][e] = x[u][e] * s * g[e];
+            }
+            float y[N];
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                y[e] = __fsub_rn(__fmul_rn(x[u][e], f[u][e]), __fmul_rn(x[u][e + 1], f[u][e + 1]));
+                y[e + 1] = __fadd_rn(__fmul_rn(x[u][e], f[u][e + 1]), __fmul_rn(x[u][e + 1], f[u][e]));
+            }
+            if (kind == 0) *reinterpret_cast<V*>(a.q_out + i * a.qo_ld + head * HD + c) = *reinterpret_cast<const V*>(y);
+            else store_cache<CT, N>(reinterpret_cast<CT*>(a.kcache) + row, y);
+        }
     }
-    float f[N];
-    *reinterpret_cast<V*>(f) = *reinterpret_cast<const V*>(a.table + pos * a.table_ld + c);
-    const float* gain = kind == 0 ? a.q_gain : a.k_gain;
-    if (gain) {
-        float g[N];
-        *reinterpret_cast<V*>(g) = *reinterpret_cast<const V*>(gain + c);
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; e++) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float s = 1.0f / sqrtf(ss / (float)HD + a.eps);
-#pragma unroll
-        for (int e = 0; e < N; e++) x[e] = x[e] * s * g[e];
-    }
-    float y[N];
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-        y[e] = __fsub_rn(__fmul_rn(x[e], f[e]), __fmul_rn(x[e + 1], f[e + 1]));
-        y[e + 1] = __fadd_rn(__fmul_rn(x[e], f[e + 1]), __fmul_rn(x[e + 1], f[e]));
-    }
-    if (kind == 0) *reinterpret_cast<V*>(a.q_out + i * a.qo_ld + head * HD + c) = *reinterpret_cast<const V*>(y);
-    else store_cache<CT, N>(reinterpret_cast<CT*>(a.kcache) + row, y);
 }
 
 template <typename CT>
-void launch(const RotateArgs& a, int hd, unsigned grid, cudaStream_t s) {
+void launch(const RotateArgs& a, int hd, cudaStream_t s) {
+    const dim3 grid((unsigned)((a.heads + 2 * a.kv_heads + 7) / 8), (unsigned)std::min((a.n + U - 1) / U, 65535));
     if (hd == 128) norm_rope_append_kernel<CT, 128><<<grid, 256, 0, s>>>(a);
     else norm_rope_append_kernel<CT, 64><<<grid, 256, 0, s>>>(a);
 }
@@ -151,8 +162,6 @@ extern "C" int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_t
     if (rope->dtype != RLB_F32 || rope->cols != hd || rope->rows < start_pos + n)
         return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: the rope table must be f32, head_dim wide and cover position %lld", (long long)(start_pos + n - 1));
     if (!(eps >= 0.f)) return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: eps must not be negative");
-    const int64_t warps = n * ((int64_t)heads + 2 * (int64_t)kv_heads);
-    if ((warps + 7) / 8 > 0x7fffffffll) return rlb_fail(RLB_ERR_LIMIT, "norm_rope_append: %lld rows of %d heads are more than one launch takes", (long long)n, heads);
     if (n == 0) return RLB_OK;
     rlb_ctx* ctx = q_out->ctx;
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
@@ -165,9 +174,8 @@ extern "C" int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_t
     a.table = (const float*)rope->d; a.table_ld = rope->cap;
     a.kcache = kcache->d; a.vcache = vcache->d;
     a.n = (int)n; a.heads = heads; a.kv_heads = kv_heads; a.max_seq = max_seq_len; a.start = start_pos; a.eps = eps;
-    const unsigned grid = (unsigned)((warps + 7) / 8);
-    if (kcache->dtype == RLB_F16) launch<__half>(a, (int)hd, grid, ctx->stream);
-    else launch<float>(a, (int)hd, grid, ctx->stream);
+    if (kcache->dtype == RLB_F16) launch<__half>(a, (int)hd, ctx->stream);
+    else launch<float>(a, (int)hd, ctx->stream);
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
     RLB_TRY(tensor_mark_ready(q_out));
