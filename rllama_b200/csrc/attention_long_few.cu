@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kRows = 8;    // query rows of a CTA
 constexpr int kWarps = 8;
+constexpr int kMaxCluster = 8;   // (clusters of 16 find room on few SMs: 35 us where two kernels take 21)
 constexpr float kShift = 7.f, kLag = 8.f;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -45,11 +46,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
 // The ring: stages of POS positions, [K rows][V rows][K scales][V scales]; 4 bits: two CTAs share an SM.
-template <int KIND, int HD> struct Ring {
+template <int KIND, int HD, bool CLUSTER> struct Ring {
     static constexpr int POS = kWarps * 16, ROW = KIND == CACHE_Q4 ? HD / 2 : HD * 2, SCALES = KIND == CACHE_Q4 ? HD / 16 : 0;
+    static constexpr int THREADS = (kWarps + 1) * 32;
     static constexpr int V = POS * ROW, KD = 2 * POS * ROW, VD = KD + POS * SCALES, STAGE = KD + 2 * POS * SCALES;
-    static constexpr int STAGES = KIND == CACHE_Q4 ? (HD == 128 ? 4 : 8) : (HD == 128 ? 3 : 6);
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE;
+    static constexpr int STAGES = (KIND == CACHE_Q4 ? 4 : CLUSTER ? 2 : 3) * 128 / HD;
+    static constexpr int MOST = CLUSTER ? kMaxCluster : 1;
+    static constexpr size_t RECORD = kRows * HD * 4;                       // [split][row][HD] behind the ring, written by the cluster
+    static size_t smem(int splits) { return (size_t)STAGES * STAGE + (CLUSTER ? splits * RECORD : 0); }
 };
 template <typename T> __device__ __forceinline__ T fetch(const char* p) { return *reinterpret_cast<const T*>(p); }
 
@@ -157,8 +161,6 @@ __device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
     return x;
 }
-__device__ __forceinline__ void cluster_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
@@ -172,15 +174,18 @@ __device__ __forceinline__ void async_arrive(uint64_t* bar) {   // once the thre
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// CLUSTER: the splits of a row block form a thread-block cluster (at most kWarps of them) and meet in the first one's shared memory.
+// CLUSTER: the splits of a row block form a thread-block cluster and meet in the first one's shared memory.
 template <int KIND, int HD, bool CLUSTER>
-__global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) attn_long_few_kernel(const __grid_constant__ AttnLongArgs a, int* err) {
-    typedef Ring<KIND, HD> Y;
+__global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACHE_Q4 ? 2 : 1) attn_long_few_kernel(const __grid_constant__ AttnLongArgs a, int* err) {
+    typedef Ring<KIND, HD, CLUSTER> Y;
     constexpr int KS = HD / 16, U = VFrag<KIND, HD>::U, STAGES = Y::STAGES;
     extern __shared__ __align__(128) char ring[];
-    float (*o_s)[kRows][HD] = reinterpret_cast<float (*)[kRows][HD]>(ring);   // [warp], after the loop
-    static_assert(kWarps * kRows * HD * 4 <= STAGES * Y::STAGE, "the warps' results fit in the ring");
+    constexpr int LD = HD + 1;   // (a thread's neighbours in a store are 2 rows or 8 columns away)
+    float (*o_s)[kRows][LD] = reinterpret_cast<float (*)[kRows][LD]>(ring);   // [warp], after the loop
+    static_assert(kWarps * kRows * LD * 4 <= STAGES * Y::STAGE, "the warps' results fit in the ring");
+    float* rec_o = reinterpret_cast<float*>(ring + STAGES * Y::STAGE);
     __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
+    __shared__ float2 rec_ml[Y::MOST][kRows];
     __shared__ uint4 q_s[HD / 16][32];   // the queries as A operands, a lane's four registers of a product side by side
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
     __shared__ int dead_flag;
@@ -196,19 +201,22 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) a
     const int v0 = min(run.len, (int)blockIdx.y * chunk), v1 = min(run.len, v0 + chunk);
     const int64_t base = (int64_t)kvh * a.max_seq;
 
-    if (threadIdx.x == 0) {
-        dead_flag = 0;
-        bad = 0;
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(&full[s], KIND == CACHE_Q4 ? 33 : 1);   // the announced bytes, and the scales' 32 threads
-            mbar_init(&empty[s], kWarps);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
+    // (a CTA's shared memory may be written by its cluster only once that CTA is running)
+    if constexpr (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     float o[U][4][4] = {}, m = -FLT_MAX, l = 0.f;
     if (warp == kWarps) {
         // ------------------------------- keeps the ring full ---------------------------------------------------------
+        if (lane == 0) {
+            dead_flag = 0;
+            bad = 0;
+            for (int s = 0; s < STAGES; s++) {
+                mbar_init(&full[s], KIND == CACHE_Q4 ? 33 : 1);   // the announced bytes, and the scales' 32 threads
+                mbar_init(&empty[s], kWarps);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("bar.arrive 1, %0;" ::"n"(Y::THREADS) : "memory");   // the barriers are there; the first copies go out at once
         const char *k = reinterpret_cast<const char*>(a.k) + base * Y::ROW, *v = reinterpret_cast<const char*>(a.v) + base * Y::ROW;
         uint32_t s = 0, phase = 1;
         int p0 = v0, issued = 0;
@@ -392,7 +400,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) a
                 for (int e = 0; e < 4; e++) mma16816(o[u][e], make_uint4(f[e][0], f[e][1], f[e][2], f[e][3]), b0, b1);
             }
         };
-        asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");   // q_s
+        asm volatile("bar.sync 1, %0;" ::"n"(Y::THREADS) : "memory");   // q_s, and the barriers
         uint32_t s = 0, phase = 0;
         for (int p0 = v0; p0 < v1; p0 += Y::POS) {
             if (!warp_wait(&full[s], phase, dead, err)) break;
@@ -403,7 +411,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) a
             if (++s == STAGES) { s = 0; phase ^= 1; }
         }
     }
-    // the eight warps' shares, in the ring's room
+    // the warps' shares, in the ring's room
     __syncthreads();
     if (warp < kWarps) {
         l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -414,7 +422,8 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) a
 #pragma unroll
             for (int e = 0; e < 4; e++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) o_s[warp][2 * c + (x & 1)][VFrag<KIND, HD>::dim(u, r) + 2 * e + (x >> 1)] = o[u][e][x];
+                for (int x = 0; x < 4; x++)
+                    if (2 * c + (x & 1) < rows) o_s[warp][2 * c + (x & 1)][VFrag<KIND, HD>::dim(u, r) + 2 * e + (x >> 1)] = o[u][e][x];
     }
     __syncthreads();
     constexpr int PER = kRows * HD / (kWarps * 32);   // values of the result a thread joins: of one row, PER neighbouring columns
@@ -435,12 +444,12 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) a
             for (int e = 0; e < PER; e++) O[e] = fmaf(o_s[w][from][jc + e], f, O[e]);
         }
     };
-    join(kWarps, jr);
+    const bool live = joins && jr < rows;
+    if (live) join(kWarps, jr);
     M -= kShift;
     float check = L * 0.f;   // a NaN once anything is not finite
 #pragma unroll
     for (int e = 0; e < PER; e++) check = fmaf(O[e], 0.f, check);
-    const bool live = joins && jr < rows;
     const int jrow = row0 + min(jr, rows - 1), ji = jrow / a.group, jh = kvh * a.group + jrow % a.group;
     const bool sees = visible_run(a, a.start + ji, a.start + ji).len > 0;
     // (a row that sees something has a sum above zero somewhere, but perhaps not in this share)
@@ -479,48 +488,63 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, KIND == CACHE_Q4 ? 2 : 1) a
         if (jr == y) join(kWarps, 0);
     }
     if constexpr (CLUSTER) {
-        cluster_sync();   // every CTA has joined its warps: the first one's shared memory may be written
-        const uint32_t to = blockIdx.y;
-        if (joins) {
-#pragma unroll
-            for (int e = 0; e < PER; e++) cluster_store(cluster_map(&o_s[to][jr][jc + e], 0), O[e]);
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // every CTA of the cluster is running
+        if (live) {
+            const uint32_t to = cluster_map(rec_o + ((blockIdx.y * kRows + jr) * HD + jc), 0);
+            if constexpr (PER == 4)
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(O[0]), "f"(O[1]), "f"(O[PER - 2]), "f"(O[PER - 1]) : "memory");
+            else
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(O[0]), "f"(O[1]) : "memory");
             if (jc == 0) {
-                cluster_store(cluster_map(&m_s[to][jr], 0), M);
-                cluster_store(cluster_map(&l_s[to][jr], 0), L);
+                const uint32_t ml = cluster_map(&rec_ml[blockIdx.y][jr], 0);
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(ml), "f"(M), "f"(L) : "memory");
             }
         }
-        cluster_sync();
-        if (blockIdx.y != 0) return;
-        join(a.n_split, jr);
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (blockIdx.y != 0 || !live) return;
+        M = -FLT_MAX;
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; e++) O[e] = 0.f;
+        for (int w = 0; w < a.n_split; w++) M = fmaxf(M, rec_ml[w][jr].x);
+        for (int w = 0; w < a.n_split; w++) {
+            const float2 ml = rec_ml[w][jr];
+            const float f = ex2_approx(ml.x - M);
+            L = fmaf(ml.y, f, L);
+#pragma unroll
+            for (int e = 0; e < PER; e++) O[e] = fmaf(rec_o[(w * kRows + jr) * HD + jc + e], f, O[e]);
+        }
     }
     if (!live) return;
     if (!CLUSTER && a.n_split > 1) {
         const int64_t rec = ((int64_t)ji * a.heads + jh) * a.n_split + blockIdx.y;
-#pragma unroll
-        for (int e = 0; e < PER; e++) a.rec_o[rec * HD + jc + e] = O[e];
+        if constexpr (PER == 4) *reinterpret_cast<float4*>(a.rec_o + rec * HD + jc) = make_float4(O[0], O[1], O[PER - 2], O[PER - 1]);
+        else *reinterpret_cast<float2*>(a.rec_o + rec * HD + jc) = make_float2(O[0], O[1]);
         if (jc == 0) a.rec_ml[rec] = make_float2(M, L);
-    } else {
-        const float inv = sees ? 1.0f / L : 0.f;
-        __half* dst = reinterpret_cast<__half*>(a.out) + ji * a.out_ld + (int64_t)jh * HD + jc;
-#pragma unroll
-        for (int e = 0; e < PER; e += 2) *reinterpret_cast<__half2*>(dst + e) = sees ? __floats2half2_rn(O[e] * inv, O[e + 1] * inv) : __half2half2(__ushort_as_half(0));
+        return;
     }
+    const float inv = sees ? 1.0f / L : 0.f;
+    __half* dst = reinterpret_cast<__half*>(a.out) + ji * a.out_ld + (int64_t)jh * HD + jc;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) *reinterpret_cast<__half2*>(dst + e) = sees ? __floats2half2_rn(O[e] * inv, O[e + 1] * inv) : __half2half2(__ushort_as_half(0));
 }
 
 template <int KIND, int HD>
 int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
     const int64_t blocks = ((int64_t)a.n * a.group + kRows - 1) / kRows;
     const bool cluster = a.n_split > 1 && a.rec_o == nullptr;
+    typedef Ring<KIND, HD, true> YC;
+    const size_t smem = cluster ? YC::smem(a.n_split) : Ring<KIND, HD, false>::smem(1), most = cluster ? YC::smem(YC::MOST) : smem;
     auto kern = cluster ? attn_long_few_kernel<KIND, HD, true> : attn_long_few_kernel<KIND, HD, false>;
     static std::atomic<uint64_t> set[2];
     if (!attr_done(set[cluster], ctx->device)) {
-        RLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Ring<KIND, HD>::SMEM));
+        RLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
         attr_mark(set[cluster], ctx->device);
     }
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(blocks * a.kv_heads), a.n_split);
-    lc.blockDim = dim3((kWarps + 1) * 32);
-    lc.dynamicSmemBytes = Ring<KIND, HD>::SMEM;
+    lc.blockDim = dim3(YC::THREADS);
+    lc.dynamicSmemBytes = smem;
     lc.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -539,10 +563,15 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
 AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + kRows / a.group, (int64_t)a.start + a.n);
-    // at least a tile of 16 positions for every warp
+    // as many as fill the SMs, but at least a tile of 16 positions for every warp
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / ctas, 256), (seen + kWarps * 16 - 1) / (kWarps * 16)));
-    // a cluster joins its splits without a second kernel
-    if (most <= kWarps) return {(int)most, false};
+    // A cluster joins its splits through shared memory; more of them need records and a second kernel, which costs about 2 us more, the
+    // time of 13 MB. That is weighed against the SMs that a cluster's eight splits leave empty. (One token, 32 heads, 384
+    // 4-bit positions: three splits in a cluster 6.8 us, through records 10.6. The last CTA to arrive joining the
+    // records, without a second kernel, was no faster than it.)
+    const int64_t cluster = std::min<int64_t>(most, kMaxCluster);
+    const double bytes = 2.0 * (double)seen * a.kv_heads * (kind == CACHE_Q4 ? a.hd / 2 + a.hd / 16 : a.hd * 2);
+    if (bytes * ((double)most / cluster - 1) < 13e6) return {(int)cluster, false};
     return {(int)most, true};
 }
 
