@@ -16,6 +16,8 @@ using namespace attn_long;
 
 namespace {
 
+constexpr int kTileRows = 64;
+
 // One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
 template <int HD>
 __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a) {
@@ -194,11 +196,14 @@ int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, i
 
 int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     AttnLongArgs a = given;
-    const bool tiles = kind != CACHE_F32 && (int64_t)a.n * a.group >= 64;
+    // Rows that share a K/V head: from kTileRows on tiles of rows on the tensor cores (f16, 4 bits), from 16 on tiles of 64 rows (f32); below, every
+    // fetched cache row serves up to eight query rows (f16, 4 bits) or one (f32).
+    const int64_t shared = (int64_t)a.n * a.group;
+    const bool f32 = kind == CACHE_F32, tiles = shared >= (f32 ? 16 : kTileRows), few = !f32 && !tiles;
     AttnSplit split;
-    if (kind != CACHE_F32 && !tiles) split = attn_long_few_splits(ctx, kind, a);
+    if (few) split = attn_long_few_splits(ctx, kind, a);
     else {
-        split.n = tiles ? attn_long_tc_splits(ctx, kind, a) : rows_splits(ctx, a);
+        split.n = !tiles ? rows_splits(ctx, a) : f32 ? attn_long_f32_splits(ctx, a) : attn_long_tc_splits(ctx, kind, a);
         split.records = split.n > 1;
     }
     a.n_split = split.n;
@@ -210,11 +215,12 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
         a.rec_o = (float*)ws.p;
         a.rec_ml = (float2*)(a.rec_o + recs * a.hd);
     }
-    if (tiles) RLB_TRY(launch_attn_long_tc(ctx, kind, a));
-    else if (kind != CACHE_F32) RLB_TRY(launch_attn_long_few(ctx, kind, a));
+    if (few) RLB_TRY(launch_attn_long_few(ctx, kind, a));
+    else if (!f32) RLB_TRY(launch_attn_long_tc(ctx, kind, a));
+    else if (tiles) RLB_TRY(launch_attn_long_f32(ctx, a));
     else RLB_TRY(a.hd == 128 ? launch_rows<128>(ctx, a) : launch_rows<64>(ctx, a));
     if (split.records) {
-        if (kind == CACHE_F32) RLB_TRY(a.hd == 128 ? (launch_merge<float, 128>(ctx, a)) : (launch_merge<float, 64>(ctx, a)));
+        if (f32) RLB_TRY(a.hd == 128 ? (launch_merge<float, 128>(ctx, a)) : (launch_merge<float, 64>(ctx, a)));
         else RLB_TRY(a.hd == 128 ? (launch_merge<__half, 128>(ctx, a)) : (launch_merge<__half, 64>(ctx, a)));
     }
     return RLB_OK;

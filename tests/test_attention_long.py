@@ -341,7 +341,9 @@ def test_attention_a_bad_row_reaches_only_the_rows_that_see_it(cl, kind, n):
     total = start + n
     g = gen(6)
     q, k, v = normal(g, n, heads * hd), normal(g, kv, total, hd), normal(g, kv, total, hd)
-    clean, _, _ = attend(cl, q, k, v, heads, kv, hd, start, window, sinks, kind, total)
+    clean, k, v = attend(cl, q, k, v, heads, kv, hd, start, window, sinks, kind, total)
+    want, spread, top = attention64(q, k, v, heads, kv, hd, start, window, sinks)
+    tol = tolerance(want, spread, top, clean.dtype, hd, window + sinks)
     for which in (0, 1):
         at = start + n // 2
         k2, v2 = k.clone(), v.clone()
@@ -350,8 +352,10 @@ def test_attention_a_bad_row_reaches_only_the_rows_that_see_it(cl, kind, n):
         sees = visible(start, n, window, sinks, total)[:, at]
         assert not torch.isfinite(out[sees]).any()
         assert torch.isfinite(out[~sees]).all()
-        # rows that do not see it: the same numbers up to the order of their sums
-        assert ((out[~sees].double() - clean[~sees].double()).abs() <= 4 * HALF[out.dtype] * (1 + clean[~sees].double().abs())).all()
+        # The formula's result for rows that do not see it has not changed, so the bound of every result holds for theirs, whichever way they
+        # were computed. (Two ways differ by up to the sum of their bounds, in f32 hd + 8 steps times the scores' terms among them, not by the four
+        # steps of the result that this test asked for at first.)
+        assert ((out[~sees].double() - want[~sees]).abs() <= tol[~sees]).all()
 
 
 @pytest.mark.gpu
