@@ -16,8 +16,6 @@ using namespace attn_long;
 
 namespace {
 
-constexpr int kTileRows = 64;
-
 // One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
 template <int HD>
 __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a) {
@@ -196,15 +194,24 @@ int run(CacheKind kind, AttnLongArgs& a, rlb_tensor* out, const rlb_tensor* q, i
 
 int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     AttnLongArgs a = given;
-    // Rows that share a K/V head: from kTileRows on tiles of rows on the tensor cores (f16, 4 bits), from 16 on tiles of 64 rows (f32); below, every
-    // fetched cache row serves up to eight query rows (f16, 4 bits) or one (f32).
-    const int64_t shared = (int64_t)a.n * a.group;
-    const bool f32 = kind == CACHE_F32, tiles = shared >= (f32 ? 16 : kTileRows), few = !f32 && !tiles;
+    const bool f32 = kind == CACHE_F32;
     AttnSplit split;
-    if (few) split = attn_long_few_splits(ctx, kind, a);
-    else {
-        split.n = !tiles ? rows_splits(ctx, a) : f32 ? attn_long_f32_splits(ctx, a) : attn_long_tc_splits(ctx, kind, a);
+    bool tiles, few = false;
+    if (f32) {
+        // Rows that share a K/V head: from 16 on they go through tiles of 64 (32 heads, 10000 positions: 285 us at 16 rows), below row by row (306 us at 8).
+        tiles = (int64_t)a.n * a.group >= 16;
+        split.n = tiles ? attn_long_f32_splits(ctx, a) : rows_splits(ctx, a);
         split.records = split.n > 1;
+    } else {
+        // The kernel for few rows reads the cache once for every eight of them, the one for many rows has tiles of 128 (256 in 4 bits) that cost
+        // the same however many of their rows there are. Each says what it expects to take, from what was measured; e.g. 32
+        // heads, 8000 positions, us with few / tiles: f16 8 rows 31 / 31, 16 rows 50 / 32, 64 rows 163 / 39; 4 bits 8 rows 21 / 52, 24 rows 62 / 52, 64
+        // rows 104 / 53; 300 positions: f16 32 rows 10 / 15, 64 rows 17 / 15; 4 bits 64 rows 13 / 21, 128 rows 23 / 21.
+        const AttnSplit s = attn_long_few_splits(ctx, kind, a);
+        const int t = attn_long_tc_splits(ctx, kind, a);
+        few = attn_long_few_us(ctx, kind, a, s) <= attn_long_tc_us(ctx, kind, a, t);
+        tiles = !few;
+        split = few ? s : AttnSplit{t, t > 1};
     }
     a.n_split = split.n;
     const int64_t rows = (int64_t)a.n * a.heads;

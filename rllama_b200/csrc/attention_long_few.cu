@@ -560,9 +560,14 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
 
 }  // namespace
 
+// Positions that some row of a block of `rows` rows sees, at most.
+static int64_t positions_seen(const AttnLongArgs& a, int rows) {
+    return std::min<int64_t>((int64_t)a.window + a.sinks + rows / a.group, (int64_t)a.start + a.n);
+}
+
 AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
-    const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + kRows / a.group, (int64_t)a.start + a.n);
+    const int64_t seen = positions_seen(a, kRows);
     // as many as fill the SMs, but at least a tile of 16 positions for every warp
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / ctas, 256), (seen + kWarps * 16 - 1) / (kWarps * 16)));
     // A cluster joins its splits through shared memory; more of them need records and a second kernel, which costs about 2 us more, the
@@ -573,6 +578,14 @@ AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs&
     const double bytes = 2.0 * (double)seen * a.kv_heads * (kind == CACHE_Q4 ? a.hd / 2 + a.hd / 16 : a.hd * 2);
     if (bytes * ((double)most / cluster - 1) < 13e6) return {(int)cluster, false};
     return {(int)most, true};
+}
+
+// 6 us, 2 more for a second kernel, and the rounds of CTAs over the SMs, a CTA reading 44 KB a us (f16: an SM's share of the memory's rate) or,
+// with 4 bits and two CTAs an SM, 9.8 KB (what their arithmetic allows).
+double attn_long_few_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, AttnSplit s) {
+    const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
+    const double row = kind == CACHE_Q4 ? a.hd + a.hd / 8 : a.hd * 4, rate = kind == CACHE_Q4 ? 9.8e3 : 44e3;
+    return 6 + (s.records ? 2 : 0) + (double)((ctas * s.n + slots - 1) / slots) * (double)positions_seen(a, kRows) / s.n * row / rate;
 }
 
 int launch_attn_long_few(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {

@@ -761,6 +761,15 @@ int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     return (int)best;
 }
 
+// 14 us (20 with the unpacking of 4-bit rows), and the longer of the CTAs' steps, 1.2 us each, and the reading of the cache.
+double attn_long_tc_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, int splits) {
+    const int tiles = kind == CACHE_Q4 ? 2 : 1;
+    const int64_t rows = tiles * QT, ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + rows - 1) / rows), slots = (int64_t)ctx->sm_count * (2 / tiles);
+    const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + rows / a.group, (int64_t)a.start + a.n), steps = (seen + TK - 1) / TK;
+    const double bytes = (double)seen * a.kv_heads * (kind == CACHE_Q4 ? a.hd + a.hd / 8 : a.hd * 4);
+    return (kind == CACHE_Q4 ? 20 : 14) + std::max(1.2 * (double)((ctas * splits + slots - 1) / slots) * (double)((steps + splits - 1) / splits), bytes / 6.5e6);
+}
+
 int launch_attn_long_tc(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     if (kind == CACHE_F16) return a.hd == 128 ? launch<CACHE_F16, 128>(ctx, a) : launch<CACHE_F16, 64>(ctx, a);
     return a.hd == 128 ? launch<CACHE_Q4, 128>(ctx, a) : launch<CACHE_Q4, 64>(ctx, a);
