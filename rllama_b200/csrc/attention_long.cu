@@ -198,9 +198,13 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     AttnSplit split;
     bool tiles, few = false;
     if (f32) {
-        // Rows that share a K/V head: from 16 on they go through tiles of 64 (32 heads, 10000 positions: 285 us at 16 rows), below row by row (306 us at 8).
-        tiles = (int64_t)a.n * a.group >= 16;
-        split.n = tiles ? attn_long_f32_splits(ctx, a) : rows_splits(ctx, a);
+        // Tiles of 64 rows of a K/V head, 15 us (head_dim 128) for 64 positions of two of them an SM, or row by row, 0.12 us for 1000 scores. (32 heads,
+        // 10000 positions: 8 rows 306 us row by row, 16 rows 285 in tiles; 8 heads of 64 on 4 K/V heads, 77 rows, window 100: 10 row by row, 20 in tiles.)
+        const int t = attn_long_f32_splits(ctx, a), r = rows_splits(ctx, a);
+        const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks, (int64_t)a.start + a.n);
+        const double row_us = 5 + 0.12e-3 * (double)a.n * a.heads * (double)seen * (a.hd == 128 ? 1 : 0.7);
+        tiles = attn_long_f32_us(ctx, a, t) < row_us;
+        split.n = tiles ? t : r;
         split.records = split.n > 1;
     } else {
         // The kernel for few rows reads the cache once for every eight of them, the one for many rows has tiles of 128 (256 in 4 bits) that cost

@@ -105,10 +105,11 @@ struct AttnSplit {
 };
 // attention_long_few.cu
 AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
-double attn_long_few_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, AttnSplit s);   // the time it will take, roughly
+double attn_long_few_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, AttnSplit s);
 int launch_attn_long_few(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 // attention_long_f32.cu
 int attn_long_f32_splits(rlb_ctx* ctx, const AttnLongArgs& a);
+double attn_long_f32_us(rlb_ctx* ctx, const AttnLongArgs& a, int splits);   // the time it will take, roughly
 int launch_attn_long_f32(rlb_ctx* ctx, const AttnLongArgs& a);
 // attention_long_tc.cu
 int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);

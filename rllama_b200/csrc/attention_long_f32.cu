@@ -221,4 +221,10 @@ int attn_long_f32_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
     return (int)best;
 }
 
+double attn_long_f32_us(rlb_ctx* ctx, const AttnLongArgs& a, int splits) {
+    const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + QT - 1) / QT), slots = (int64_t)ctx->sm_count * 2;
+    const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + QT / a.group, (int64_t)a.start + a.n), steps = (seen + TK - 1) / TK;
+    return (splits > 1 ? 10 : 6) + 15.0 * a.hd / 128 * (double)((ctas * splits + slots - 1) / slots) * (double)((steps + splits - 1) / splits);
+}
+
 int launch_attn_long_f32(rlb_ctx* ctx, const AttnLongArgs& a) { return a.hd == 128 ? launch<128>(ctx, a) : launch<64>(ctx, a); }

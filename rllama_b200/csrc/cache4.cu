@@ -38,35 +38,42 @@ struct AppendArgs {
     int kv_heads, max_seq, start, n;
 };
 
-// Both kernels: grid (words of a row / 256 threads and U rows, K and V); a thread takes a word (eight neighbouring values) of U rows, with
-// the loads of all of them in flight; four threads make a group. No thread divides by a runtime size.
-// (One word of one row a thread, found by 64-bit division: 51 us for 1792 rows of 64 heads, 49 us to read them back.)
-constexpr int U = 4;
+// Both kernels: grid (4 kv_heads / 128, rows, K and V). A thread takes the same block of eight values of every group of a head's row, HD / 4
+// values, which is a quarter of the row's codes side by side (cache4.h); four threads make a row. No thread divides by a runtime size. (1792 rows
+// of 64 heads of 128, f32, written and read back: one word a thread, found by 64-bit division: 51 + 49 us; this: 28 + 13 us, of 20 + 11 that the
+// bytes take; two rows a thread, or CTAs of 256: 4 to 10 us more.)
+constexpr int kThreads = 128;
+template <int G> struct Words;   // a quarter of a row's codes, and its scales
+template <> struct Words<4> { typedef uint4 T; typedef uint2 D; };
+template <> struct Words<2> { typedef uint2 T; typedef uint32_t D; };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) append4_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int WORDS = HD / 8, GROUPS = HD / kQ4Group;
-    const int x = blockIdx.x * 256 + threadIdx.x, which = blockIdx.z;
-    const bool live = x < a.kv_heads * WORDS;   // (a multiple of 8: a group's four threads are all live or none is)
-    const int word = x % WORDS, head = live ? x / WORDS : 0, group = word / 4, block = word % 4;
-    const T* src = reinterpret_cast<const T*>(a.src[which]) + head * HD + word * 8;
-    for (int i0 = blockIdx.y * U; i0 < a.n; i0 += gridDim.y * U) {
-        float x8[U][8];
+__global__ void __launch_bounds__(kThreads) append4_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int G = HD / kQ4Group;
+    const int x = blockIdx.x * kThreads + threadIdx.x, which = blockIdx.z, block = x & 3;
+    const bool live = x < a.kv_heads * 4;   // (a row's four threads are all live or none is)
+    const int head = live ? x >> 2 : 0;
+    const T* src = reinterpret_cast<const T*>(a.src[which]) + head * HD + block * 8;
+    for (int i = blockIdx.y; i < a.n; i += gridDim.y) {
+        float y[G][8];
 #pragma unroll
-        for (int u = 0; u < U; u++) load8<T>(src + (int64_t)min(i0 + u, a.n - 1) * a.ld[which], x8[u]);
+        for (int g = 0; g < G; g++) load8<T>(src + i * a.ld[which] + g * kQ4Group, y[g]);
+        uint32_t w[G];
+        __half d[G];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
+        for (int g = 0; g < G; g++) {
             float m = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(x8[u][e]));
+            for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(y[g][e]));
             m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const __half d = m != m ? __ushort_as_half(0x7fff) : q4_scale(m);
-            if (!live || i0 + u >= a.n) continue;
-            const int64_t row = (int64_t)head * a.max_seq + a.start + i0 + u;
-            reinterpret_cast<uint32_t*>(a.codes[which] + row * (HD / 2))[block * GROUPS + group] = q4_pack(x8[u], __half2float(d));
-            if (block == 0) a.scales[which][row * GROUPS + group] = d;
+            d[g] = m != m ? __ushort_as_half(0x7fff) : q4_scale(m);
+            w[g] = q4_pack(y[g], __half2float(d[g]));
         }
+        if (!live) continue;
+        const int64_t row = (int64_t)head * a.max_seq + a.start + i;
+        *reinterpret_cast<typename Words<G>::T*>(a.codes[which] + row * (HD / 2) + block * (HD / 8)) = *reinterpret_cast<const typename Words<G>::T*>(w);
+        if (block == 0) *reinterpret_cast<typename Words<G>::D*>(a.scales[which] + row * G) = *reinterpret_cast<const typename Words<G>::D*>(d);
     }
 }
 
@@ -79,29 +86,25 @@ struct ReadArgs {
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) read4_kernel(const __grid_constant__ ReadArgs a) {
-    constexpr int WORDS = HD / 8, GROUPS = HD / kQ4Group;
-    const int x = blockIdx.x * 256 + threadIdx.x, which = blockIdx.z;
-    if (x >= a.kv_heads * WORDS || a.dst[which] == nullptr) return;
-    const int word = x % WORDS, head = x / WORDS, group = word / 4, block = word % 4;
+__global__ void __launch_bounds__(kThreads) read4_kernel(const __grid_constant__ ReadArgs a) {
+    constexpr int G = HD / kQ4Group;
+    const int x = blockIdx.x * kThreads + threadIdx.x, which = blockIdx.z, block = x & 3, head = x >> 2;
+    if (x >= a.kv_heads * 4 || a.dst[which] == nullptr) return;
     const int64_t base = (int64_t)head * a.max_seq + a.start;
-    for (int i0 = blockIdx.y * U; i0 < a.n; i0 += gridDim.y * U) {
-        uint32_t w[U];
-        __half2 d[U];
+    for (int i = blockIdx.y; i < a.n; i += gridDim.y) {
+        const int64_t row = base + i;
+        uint32_t w[G];
+        __half d[G];
+        *reinterpret_cast<typename Words<G>::T*>(w) = *reinterpret_cast<const typename Words<G>::T*>(a.codes[which] + row * (HD / 2) + block * (HD / 8));
+        *reinterpret_cast<typename Words<G>::D*>(d) = *reinterpret_cast<const typename Words<G>::D*>(a.scales[which] + row * G);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + min(i0 + u, a.n - 1);
-            w[u] = reinterpret_cast<const uint32_t*>(a.codes[which] + row * (HD / 2))[block * GROUPS + group];
-            d[u] = __half2half2(a.scales[which][row * GROUPS + group]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (i0 + u >= a.n) break;
+        for (int g = 0; g < G; g++) {
             __half2 v[4];
-            q4_pairs(w[u], v);
+            q4_pairs(w[g], v);
+            const __half2 dd = __half2half2(d[g]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = __hmul2(v[j], d[u]);
-            T* dst = reinterpret_cast<T*>(a.dst[which]) + (int64_t)(i0 + u) * a.ld[which] + head * HD + word * 8;
+            for (int j = 0; j < 4; j++) v[j] = __hmul2(v[j], dd);
+            T* dst = reinterpret_cast<T*>(a.dst[which]) + i * a.ld[which] + head * HD + g * kQ4Group + block * 8;
             if constexpr (sizeof(T) == 2) {
                 *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
             } else {
@@ -113,8 +116,8 @@ __global__ void __launch_bounds__(256) read4_kernel(const __grid_constant__ Read
     }
 }
 
-dim3 rows_grid(int64_t n, int kv_heads, int hd) {
-    return dim3((unsigned)((kv_heads * (hd / 8) + 255) / 256), (unsigned)std::min<int64_t>((n + U - 1) / U, 65535), 2);
+dim3 rows_grid(int64_t n, int kv_heads) {
+    return dim3((unsigned)((kv_heads * 4 + kThreads - 1) / kThreads), (unsigned)std::min<int64_t>(n, 65535), 2);
 }
 
 int check_dims(const char* who, int32_t kv_heads, int32_t max_seq_len, int32_t head_dim) {
@@ -210,13 +213,13 @@ int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, i
     for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
     a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos;
     a.n = (int)k->rows;
-    const dim3 grid = rows_grid(k->rows, c->kv_heads, c->hd);
+    const dim3 grid = rows_grid(k->rows, c->kv_heads);
     if (k->dtype == RLB_F16) {
-        if (c->hd == 128) append4_kernel<__half, 128><<<grid, 256, 0, ctx->stream>>>(a);
-        else append4_kernel<__half, 64><<<grid, 256, 0, ctx->stream>>>(a);
+        if (c->hd == 128) append4_kernel<__half, 128><<<grid, kThreads, 0, ctx->stream>>>(a);
+        else append4_kernel<__half, 64><<<grid, kThreads, 0, ctx->stream>>>(a);
     } else {
-        if (c->hd == 128) append4_kernel<float, 128><<<grid, 256, 0, ctx->stream>>>(a);
-        else append4_kernel<float, 64><<<grid, 256, 0, ctx->stream>>>(a);
+        if (c->hd == 128) append4_kernel<float, 128><<<grid, kThreads, 0, ctx->stream>>>(a);
+        else append4_kernel<float, 64><<<grid, kThreads, 0, ctx->stream>>>(a);
     }
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
@@ -240,13 +243,13 @@ int rlb_cache4_read(rlb_cache4* c, rlb_tensor* k_out, rlb_tensor* v_out, int32_t
     for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
     a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos;
     a.n = (int)any->rows;
-    const dim3 grid = rows_grid(any->rows, c->kv_heads, c->hd);
+    const dim3 grid = rows_grid(any->rows, c->kv_heads);
     if (any->dtype == RLB_F16) {
-        if (c->hd == 128) read4_kernel<__half, 128><<<grid, 256, 0, ctx->stream>>>(a);
-        else read4_kernel<__half, 64><<<grid, 256, 0, ctx->stream>>>(a);
+        if (c->hd == 128) read4_kernel<__half, 128><<<grid, kThreads, 0, ctx->stream>>>(a);
+        else read4_kernel<__half, 64><<<grid, kThreads, 0, ctx->stream>>>(a);
     } else {
-        if (c->hd == 128) read4_kernel<float, 128><<<grid, 256, 0, ctx->stream>>>(a);
-        else read4_kernel<float, 64><<<grid, 256, 0, ctx->stream>>>(a);
+        if (c->hd == 128) read4_kernel<float, 128><<<grid, kThreads, 0, ctx->stream>>>(a);
+        else read4_kernel<float, 64><<<grid, kThreads, 0, ctx->stream>>>(a);
     }
     RLB_LAUNCH_CHECK();
     count_launch(ctx);

@@ -49,16 +49,22 @@ __device__ __forceinline__ void q4_pairs(uint32_t word, __half2 (&h)[4]) {
 __device__ __forceinline__ __half q4_scale(float m) {
     return __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fmul_rn(fminf(m, 65504.f), 1.0f / 7.0f))));
 }
-// Nibble of x under the scale d.
-__device__ __forceinline__ uint32_t q4_code(float x, float d) {
-    if (!(d > 0.f)) return 8u;
-    return (uint32_t)((int)rintf(fminf(fmaxf(__fdiv_rn(x, d), -7.f), 7.f)) + 8);
+// Nibble of x under the scale d: rint(x / d), clamped. x * (1 / d) is within 2e-6 of x / d below 8, so it rounds to the same integer unless it
+// lies next to a half; only then is the quotient itself needed. (A correctly rounded division for every value is most of the arithmetic of an
+// append, which is then bound by it.)
+__device__ __forceinline__ uint32_t q4_code(float x, float d, float inv) {
+    const float t = x * inv;
+    float n = rintf(t);
+    if (fabsf(t - n) > 0.49999f) n = rintf(__fdiv_rn(x, d));
+    return (uint32_t)((int)fminf(fmaxf(n, -7.f), 7.f) + 8);
 }
 // Eight values into a word.
 __device__ __forceinline__ uint32_t q4_pack(const float (&x)[8], float d) {
+    if (!(d > 0.f)) return 0x88888888u;
+    const float inv = __fdiv_rn(1.0f, d);
     uint32_t w = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) w |= q4_code(x[e], d) << (4 * ((e >> 1) + (e & 1) * 4));
+    for (int e = 0; e < 8; e++) w |= q4_code(x[e], d, inv) << (4 * ((e >> 1) + (e & 1) * 4));
     return w;
 }
 #endif
