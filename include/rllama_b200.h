@@ -86,7 +86,8 @@ int rlb_tensor_zeros(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t capacity_
 /* A tensor over memory that the caller owns and keeps alive (no copy; no counterpart in the
  * reference): device memory of the context's device, 16-byte aligned, rows a multiple of 16 bytes
  * apart. On a context with a stream of its own the caller orders its accesses itself, e.g. with
- * rlb_tensor_wait, which waits for the context's stream here. rlb_tensor_free drops the view only. */
+ * rlb_tensor_wait, which waits for the context's stream here, and keeps the memory until then.
+ * rlb_tensor_free drops the view only.                                                   */
 int rlb_tensor_wrap(rlb_ctx* ctx, void* device, int64_t rows, int64_t cols, int64_t capacity_cols,
                     rlb_dtype dtype, rlb_tensor** out);
 /* OpenCLTensor::wait_until_ready (src/tensor_opencl_support.rs:177-196).              */
@@ -151,11 +152,13 @@ int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q, const rlb_
  * Tier 1, long contexts: what lies between the q/k/v projection and wo, for caches in f16, f32
  * or 4 bits, a sliding window with first tokens that stay visible, and K/V heads shared by
  * heads / kv_heads query heads each (query head h reads K/V head h / (heads / kv_heads)).
- * head_dim is 64 or 128. Rows may be padded (capacity_cols), caches may not. A call with no rows
- * does nothing. On a context of the caller's stream these ops may be captured into a CUDA graph
- * (rlb_cache4_create excepted): a graph then owns the scratch of its calls, so graphs may be
- * replayed in any order and next to one another. The shapes, pointers and positions are fixed at
- * the time of capture.
+ * head_dim is 64 or 128; caches have up to 2^30 positions (RLB_ERR_LIMIT). Rows may be padded
+ * (capacity_cols), caches may not. A call with no rows does nothing. What a call writes overlaps
+ * none of its other arguments, unless said otherwise. On a context of the caller's stream these
+ * ops may be captured into a CUDA graph (rlb_cache4_create and rlb_rope_table excepted): a graph
+ * then owns the scratch of its calls, so graphs may be replayed in any order and next to one
+ * another. The shapes, pointers and positions are fixed at the time of capture. The context
+ * outlives the graphs captured on it.
  * ---------------------------------------------------------------------------------- */
 
 /* compute_freqs_cis (src/transformer.rs:858-885) as a tensor: max_seq_len x head_dim f32, row p

@@ -780,7 +780,8 @@ extern "C" int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q,
                         heads, n_split, hd, need, kStaticRecordFloats);
     rlb_ctx* ctx = out->ctx;
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
-    RLB_CUDA(cudaSetDevice(ctx->device));
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
     if (ctx_capturing(ctx))
         return rlb_fail(RLB_ERR_STATE, "attention_decode_static cannot be captured into a graph on a borrowed stream: its scratch is shared by the process");
     float* base = nullptr;

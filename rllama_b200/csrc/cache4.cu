@@ -122,6 +122,7 @@ dim3 rows_grid(int64_t n, int kv_heads) {
 
 int check_dims(const char* who, int32_t kv_heads, int32_t max_seq_len, int32_t head_dim) {
     if (kv_heads < 1 || kv_heads > 65536 || max_seq_len < 1) return rlb_fail(RLB_ERR_INVALID, "%s: bad kv_heads %d or max_seq_len %d", who, kv_heads, max_seq_len);
+    if (max_seq_len > kMaxPositions) return rlb_fail(RLB_ERR_LIMIT, "%s: max_seq_len %d is more than %d", who, max_seq_len, kMaxPositions);
     if (head_dim != 64 && head_dim != 128) return rlb_fail(RLB_ERR_INVALID, "%s: head_dim %d is not supported (64 or 128)", who, head_dim);
     return RLB_OK;
 }
@@ -153,7 +154,6 @@ int rlb_cache4_create(rlb_ctx* ctx, int32_t kv_heads, int32_t max_seq_len, int32
     cudaError_t e = cudaMalloc(&c->owned, 2 * (codes + scales));
     if (e != cudaSuccess) {
         delete c;
-        cudaGetLastError();
         return rlb_fail(RLB_ERR_OOM, "rlb_cache4_create: cudaMalloc(%zu): %s", 2 * (codes + scales), cudaGetErrorString(e));
     }
     e = cudaMemsetAsync(c->owned, 0, 2 * (codes + scales), ctx->stream);  // scale 0: every value is zero
@@ -175,9 +175,13 @@ int rlb_cache4_wrap(rlb_ctx* ctx, void* k_codes, void* k_scales, void* v_codes, 
     if (!ctx || !out) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_wrap: null pointer");
     *out = nullptr;
     RLB_TRY(check_dims("rlb_cache4_wrap", kv_heads, max_seq_len, head_dim));
-    for (const void* p : {k_codes, k_scales, v_codes, v_scales}) {
-        if (!p || ((uintptr_t)p & 15)) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_wrap: the four arrays must be 16-byte aligned");
-        RLB_TRY(check_device_memory(ctx, p, "rlb_cache4_wrap"));
+    const size_t rows = (size_t)kv_heads * max_seq_len;
+    const struct { const void* p; size_t bytes; } parts[] = {{k_codes, rows * (head_dim / 2)}, {k_scales, rows * (head_dim / kQ4Group) * 2},
+                                                             {v_codes, rows * (head_dim / 2)}, {v_scales, rows * (head_dim / kQ4Group) * 2}};
+    for (const auto& part : parts) {
+        if (!part.p || ((uintptr_t)part.p & 15)) return rlb_fail(RLB_ERR_INVALID, "rlb_cache4_wrap: the four arrays must be 16-byte aligned");
+        RLB_TRY(check_device_memory(ctx, part.p, "rlb_cache4_wrap"));
+        RLB_TRY(check_device_memory(ctx, (const char*)part.p + part.bytes - 1, "rlb_cache4_wrap: the last element"));
     }
     rlb_cache4* c = new (std::nothrow) rlb_cache4();
     if (!c) return rlb_fail(RLB_ERR_OOM, "rlb_cache4_wrap: out of host memory");

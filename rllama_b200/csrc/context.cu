@@ -17,6 +17,8 @@ int rlb_fail(int code, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
+    // the caller has it from us: its own next cudaGetLastError is not to find it again
+    if (code == RLB_ERR_CUDA || code == RLB_ERR_OOM) cudaGetLastError();
     return code;
 }
 
@@ -168,7 +170,7 @@ int rlb_ctx_create_on_stream(int verbose, int nth_device, void* cuda_stream, rlb
 
 int rlb_ctx_destroy(rlb_ctx* ctx) {
     if (!ctx) return RLB_OK;
-    cudaSetDevice(ctx->device);
+    DeviceScope dev(ctx->device);
     cudaStreamSynchronize(ctx->stream);
     if (ctx->op_scratch) cudaFree(ctx->op_scratch);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
@@ -181,7 +183,8 @@ int rlb_ctx_destroy(rlb_ctx* ctx) {
 int rlb_ctx_flush(rlb_ctx* ctx) {
     if (!ctx) return rlb_fail(RLB_ERR_INVALID, "rlb_ctx_flush: null context");
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
-    RLB_CUDA(cudaSetDevice(ctx->device));
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
     RLB_CUDA(cudaStreamSynchronize(ctx->stream));
     return ctx_check_error_word(ctx);
 }
@@ -202,8 +205,8 @@ static int tensor_new(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t cap, rlb
     if ((cap * (int64_t)dtype_size(dtype)) % 16 != 0)
         return rlb_fail(RLB_ERR_INVALID, "tensor: capacity_cols %lld does not give 16-byte aligned rows", (long long)cap);
     rlb_tensor* t = new rlb_tensor();
-    t->ctx = ctx; t->rows = rows; t->cols = cols; t->cap = cap; t->dtype = dtype;
-    cudaSetDevice(ctx->device);
+    t->ctx = ctx; t->device = ctx->device; t->rows = rows; t->cols = cols; t->cap = cap; t->dtype = dtype;
+    DeviceScope dev(ctx->device);
     size_t bytes = t->bytes();
     cudaError_t e = cudaMalloc(&t->d, bytes ? bytes : 16);
     if (e != cudaSuccess) {
@@ -258,18 +261,24 @@ int rlb_tensor_wrap(rlb_ctx* ctx, void* device, int64_t rows, int64_t cols, int6
                         (long long)capacity_cols, (int)dtype);
     if (((uintptr_t)device & 15) || (capacity_cols * (int64_t)dtype_size(dtype)) % 16 != 0)
         return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wrap: the memory and its rows (capacity_cols %lld) must be 16-byte aligned", (long long)capacity_cols);
-    if (rows > 0 && cols > 0) RLB_TRY(check_device_memory(ctx, device, "rlb_tensor_wrap"));
+    if (rows > 0 && cols > 0) {
+        const int64_t es = (int64_t)dtype_size(dtype);
+        if (rows > INT64_MAX / es / capacity_cols)
+            return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wrap: %lld rows of capacity %lld pass 63 bits", (long long)rows, (long long)capacity_cols);
+        RLB_TRY(check_device_memory(ctx, device, "rlb_tensor_wrap"));
+        RLB_TRY(check_device_memory(ctx, (const char*)device + ((rows - 1) * capacity_cols + cols) * es - 1, "rlb_tensor_wrap: the last element"));
+    }
     rlb_tensor* t = new (std::nothrow) rlb_tensor();
     if (!t) return rlb_fail(RLB_ERR_OOM, "rlb_tensor_wrap: out of host memory");
-    t->ctx = ctx; t->d = device; t->rows = rows; t->cols = cols; t->cap = capacity_cols; t->dtype = dtype; t->wrapped = true;
+    t->ctx = ctx; t->device = ctx->device; t->d = device; t->rows = rows; t->cols = cols; t->cap = capacity_cols; t->dtype = dtype; t->wrapped = true;
     *out = t;
     return RLB_OK;
 }
 
 int rlb_tensor_wait(rlb_tensor* t) {
     if (!t) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wait: null tensor");
-    if (t->ready) RLB_CUDA(cudaEventSynchronize(t->ready));
-    else RLB_CUDA(cudaStreamSynchronize(t->ctx->stream));
+    if (t->ready && !t->ctx->borrowed_stream) RLB_CUDA(cudaEventSynchronize(t->ready));
+    else RLB_CUDA(cudaStreamSynchronize(t->ctx->stream));  // (a graph that was replayed there has recorded no event)
     return ctx_check_error_word(t->ctx);
 }
 
@@ -277,7 +286,8 @@ int rlb_tensor_download(rlb_tensor* t, void* host, rlb_event** out_event) {
     if (!t || !host || !out_event) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_download: null pointer");
     rlb_ctx* ctx = t->ctx;
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
-    RLB_CUDA(cudaSetDevice(ctx->device));
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
     rlb_event* ev = new rlb_event();
     ev->ctx = ctx;
     cudaError_t e = cudaEventCreateWithFlags(&ev->ev, cudaEventDisableTiming);
@@ -314,7 +324,7 @@ int rlb_tensor_free(rlb_tensor* t) {
         delete t;
         return RLB_OK;
     }
-    cudaSetDevice(t->ctx->device);
+    DeviceScope dev(t->device);  // (the context may be gone by now)
     if (t->ready) {
         cudaEventSynchronize(t->ready);  // the reference also waits for the initial write before dropping
         cudaEventDestroy(t->ready);
@@ -334,7 +344,8 @@ static int refuse_capture(const rlb_ctx* ctx, const char* op) {
 #define OP_PROLOGUE(ctxvar, t)                              \
     rlb_ctx* ctxvar = (t)->ctx;                             \
     std::lock_guard<std::recursive_mutex> _g(ctxvar->mu);   \
-    RLB_CUDA(cudaSetDevice(ctxvar->device));
+    DeviceScope _dev(ctxvar->device);                       \
+    RLB_CUDA(_dev.err);
 
 int rlb_copy_inplace(rlb_tensor* dst, const rlb_tensor* src) {
     RLB_TRY(same_ctx(dst, src));

@@ -62,6 +62,7 @@ int ctx_check_error_word(rlb_ctx* ctx);  // after a synchronisation: RLB_ERR_CUD
 
 struct rlb_tensor {
     rlb_ctx* ctx = nullptr;
+    int device = 0;
     void* d = nullptr;
     int64_t rows = 0, cols = 0, cap = 0;
     rlb_dtype dtype = RLB_F32;
@@ -227,6 +228,7 @@ struct rlb_cache4 {
     void* owned = nullptr;                    // the allocation behind the four arrays, when the library made it
 };
 
+constexpr int kMaxPositions = 1 << 30;   // of a long-context cache: positions and the ends of tiles behind them are ints
 struct AttnLongArgs {
     const float* q = nullptr;                 // n rows of heads * hd f32, row stride q_ld
     int64_t q_ld = 0;
