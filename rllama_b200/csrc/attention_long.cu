@@ -167,6 +167,7 @@ int check(const char* who, const rlb_tensor* out, const rlb_tensor* q, rlb_dtype
     if (hd != 64 && hd != 128) return rlb_fail(RLB_ERR_INVALID, "%s: head_dim %lld is not supported (64 or 128)", who, (long long)hd);
     if (max_seq < 1 || start < 0 || start + q->rows > max_seq)
         return rlb_fail(RLB_ERR_INVALID, "%s: bad max_seq_len %d, start_pos %d or %lld rows", who, max_seq, start, (long long)q->rows);
+    if (max_seq > kMaxPositions) return rlb_fail(RLB_ERR_LIMIT, "%s: max_seq_len %d is more than %d", who, max_seq, kMaxPositions);
     if (window < 0 || sinks < 0) return rlb_fail(RLB_ERR_INVALID, "%s: window %d and sinks %d must not be negative", who, window, sinks);
     if (q->dtype != RLB_F32 || q->cols != heads * hd) return rlb_fail(RLB_ERR_INVALID, "%s: q must be n x heads*head_dim f32", who);
     if (out->dtype != out_dtype || out->rows != q->rows || out->cols != q->cols)
@@ -217,15 +218,21 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
         tiles = !few;
         split = few ? s : AttnSplit{t, t > 1};
     }
-    a.n_split = split.n;
     const int64_t rows = (int64_t)a.n * a.heads;
     OpWorkspace ws;
     if (split.records) {
-        const size_t recs = (size_t)rows * a.n_split;
-        RLB_TRY(ws.get(ctx, recs * (a.hd * sizeof(float) + sizeof(float2))));
-        a.rec_o = (float*)ws.p;
-        a.rec_ml = (float2*)(a.rec_o + recs * a.hd);
+        const size_t recs = (size_t)rows * split.n;
+        const int got = ws.get(ctx, recs * (a.hd * sizeof(float) + sizeof(float2)));
+        if (got == RLB_OK) {
+            a.rec_o = (float*)ws.p;
+            a.rec_ml = (float2*)(a.rec_o + recs * a.hd);
+        } else if (got == RLB_ERR_OOM && !ctx_capturing(ctx)) {
+            split = {1, false};   // no memory for records: slower without them
+        } else {
+            return got;
+        }
     }
+    a.n_split = split.n;
     if (few) RLB_TRY(launch_attn_long_few(ctx, kind, a));
     else if (!f32) RLB_TRY(launch_attn_long_tc(ctx, kind, a));
     else if (tiles) RLB_TRY(launch_attn_long_f32(ctx, a));

@@ -1,6 +1,7 @@
 // Device helpers shared by the long-context attention kernels: the visible set, cache rows as f32, the plain form of a row.
 #pragma once
 
+#include <algorithm>
 #include <cfloat>
 
 #include "cache4.h"
@@ -103,6 +104,9 @@ struct AttnSplit {
     int n;
     bool records;
 };
+// Splits whose records take up to 64 MB: scratch is memory that the caller's caches do not get.
+inline int64_t record_limit(const AttnLongArgs& a) { return std::max<int64_t>(1, (64ll << 20) / ((int64_t)a.n * a.heads * (a.hd * 4 + 8))); }
+
 // attention_long_few.cu
 AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a);
 double attn_long_few_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, AttnSplit s);

@@ -214,7 +214,7 @@ int attn_long_f32_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + QT - 1) / QT), slots = (int64_t)ctx->sm_count * 2;
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + QT / a.group, (int64_t)a.start + a.n), steps = (seen + TK - 1) / TK;
     int64_t best = 1, cost = INT64_MAX;
-    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(steps / 2, 64)); s++) {
+    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(steps / 2, std::min<int64_t>(64, record_limit(a)))); s++) {
         const int64_t c = ((ctas * s + slots - 1) / slots) * ((steps + s - 1) / s + 2);
         if (c < cost) { cost = c; best = s; }
     }

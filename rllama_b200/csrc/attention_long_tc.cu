@@ -754,7 +754,7 @@ int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + rows / a.group, (int64_t)a.start + a.n);
     const int64_t steps = (seen + TK - 1) / TK;
     int64_t best = 1, cost = INT64_MAX;
-    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(steps / 8, 64)); s++) {
+    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(steps / 8, std::min<int64_t>(64, record_limit(a)))); s++) {
         const int64_t c = ((ctas * s + slots - 1) / slots) * ((steps + s - 1) / s + 8);
         if (c < cost) { cost = c; best = s; }
     }

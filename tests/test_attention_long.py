@@ -298,6 +298,48 @@ def test_attention(cl, heads, kv, hd, n, start, window, sinks, kind):
     check_attention(cl, heads, kv, hd, n, start, window, sinks, kind)
 
 
+LONG = [
+    # enough positions that a row's splits are joined by a second kernel, or within a cluster, or not at all
+    (2, 1, 128, 1, 40000, 100000, 0),
+    (3, 1, 64, 3, 50000, 45000, 9),
+    (16, 2, 128, 1, 30000, 29000, 70),
+    (6, 6, 128, 1, 2000, 3000, 0),
+    (40, 40, 128, 1, 1500, 3000, 0),
+    (2, 1, 128, 150, 9000, 100000, 0),
+    (8, 8, 64, 70, 6000, 5000, 40),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "q4"])
+@pytest.mark.parametrize("heads,kv,hd,n,start,window,sinks", LONG)
+def test_attention_long_contexts(cl, heads, kv, hd, n, start, window, sinks, kind):
+    check_attention(cl, heads, kv, hd, n, start, window, sinks, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "q4"])
+@pytest.mark.parametrize("window", [0, 1, 31, 32, 33, 64, 65, 127, 128, 129])
+def test_attention_window_and_tile_edges(cl, kind, window):
+    """Windows, first tokens and row counts around the kernels' tiles of 16, 32, 64 and 128."""
+    for i, (n, start, sinks) in enumerate([(1, 128, 0), (8, 56, 1), (9, 0, 16), (63, 1, 31), (64, 64, 32), (65, 63, 33), (127, 130, 64), (128, 0, 65),
+                                           (129, 127, 128), (256, 0, 129)]):
+        if window or sinks:
+            check_attention(cl, 2, 1 + i % 2, 64 if i % 3 else 128, n, start, window, sinks, kind, seed=i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_random_shapes(cl, seed):
+    import random
+    r = random.Random(seed)
+    kv = r.choice([1, 2, 3, 5, 8])
+    heads, n = kv * r.choice([1, 1, 2, 3, 7, 8, 16]), r.choice([1, 1, 2, 7, 20, 55, 100, 190, 333])
+    start = int(2 ** r.uniform(0, 11.5)) - 1
+    check_attention(cl, heads, kv, r.choice([64, 128]), n, start, r.choice([10 ** 9, r.randrange(1, start + n + 1), r.randrange(1, start + n + 1)]),
+                    r.choice([0, 0, 1, 4, 50, 10 ** 9]), r.choice(["f16", "q4", "f32"]), seed=seed, max_seq=start + n + r.randrange(3))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f32", "f16", "q4"])
 def test_attention_strided_rows(cl, kind):
@@ -380,6 +422,52 @@ def test_attention_magnitudes(cl, kind, n):
     out, k, v = attend(cl, q, k, v, heads, kv, hd, start, 200, 3, kind, total)
     want, spread, top = attention64(q, k, v, heads, kv, hd, start, 200, 3)
     assert ((out.double() - want).abs() <= tolerance(want, spread, top, out.dtype, hd, 203)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "q4"])
+@pytest.mark.parametrize("n", [1, 5, 150])
+@pytest.mark.parametrize("size", [1e30, 1e36])
+def test_attention_of_huge_queries_is_the_best_row(cl, kind, n, size):
+    """Scores further apart than f32 can weigh: the result is the value of the largest score, or the mean of equal ones."""
+    heads, kv, hd, start, window = 2, 1, 64, 200 - n, 90
+    g = gen(17)
+    key = torch.arange(200, device=DEV)[torch.randperm(200, generator=g, device=DEV)]
+    k, v = torch.zeros(kv, 200, hd, device=DEV), normal(g, kv, 200, hd)
+    k[0, :, 0] = torch.where(key < 128, 1 + key / 128, 2 + (key - 128) / 64)
+    q = torch.zeros(n, heads, hd, device=DEV)
+    q[:, 0, 0], q[:, 1, 0] = size, -size
+    out, k, v = attend(cl, q.view(n, -1), k, v, heads, kv, hd, start, window, 3, kind, 210)
+    sees = visible(start, n, window, 3, 200)
+    # In 4 bits neighbours from 1.75 on can share a scale (the step of an eight-bit scale next to 1/4 is 2^-9, theirs 2^-7 / 7): equal rows have equal
+    # scores and weigh the same. The sum of c of them and the division are off by c + 2 half steps of f32, the result by half a step of its type.
+    half = torch.finfo(out.dtype).eps / 2
+    for h, sign in ((0, 1), (1, -1)):
+        s = (sign * k[0, :, 0].double()).expand(n, 200).masked_fill(~sees, -math.inf)
+        best = (s == s.amax(1, keepdim=True)).double()
+        count = best.sum(1, keepdim=True)
+        want, size = (best @ x / count for x in (v[0].double(), v[0].double().abs()))
+        off = (out.view(n, heads, hd)[:, h].double() - want).abs()
+        assert (off <= half * want.abs() + (count + 2) * 2.0 ** -24 * size + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "q4"])
+@pytest.mark.parametrize("n", [5, 150])
+def test_attention_a_bad_query_reaches_only_its_row(cl, kind, n):
+    heads, kv, hd, start, window, sinks = 4, 2, 128, 30, 60, 2
+    total = start + n
+    g = gen(18)
+    q, k, v = normal(g, n, heads * hd), normal(g, kv, total, hd), normal(g, kv, total, hd)
+    bad = q.clone()
+    bad[1, 3], bad[3, 2 * hd + 5] = math.nan, math.inf   # rows 1 and 3, heads 0 and 2
+    out, k, v = attend(cl, bad, k, v, heads, kv, hd, start, window, sinks, kind, total)
+    want, spread, top = attention64(q, k, v, heads, kv, hd, start, window, sinks)
+    good = torch.ones(n, heads, dtype=torch.bool, device=DEV)
+    good[1, 0] = good[3, 2] = False
+    good = good.repeat_interleave(hd, 1)
+    assert out[~good].isnan().all()
+    assert ((out.double() - want).abs() <= tolerance(want, spread, top, out.dtype, hd, window + sinks))[good].all()
 
 
 @pytest.mark.gpu
@@ -553,6 +641,82 @@ def test_two_captured_graphs_side_by_side(kind):
 
 
 @pytest.mark.gpu
+def test_a_captured_step_follows_its_inputs():
+    """rotate, append to both kinds of cache, read back and attend, in one graph that is replayed with new inputs in place."""
+    from rllama_b200 import Cache4, Cuda
+    side = torch.cuda.Stream()
+    on = Cuda(stream=side.cuda_stream)
+    heads, kv, hd, max_seq, pos = 8, 2, 64, 3000, 2900
+    g = gen(15)
+    q, k, v = normal(g, 1, heads * hd), normal(g, 1, kv * hd), normal(g, 1, kv * hd)
+    kc, vc = (normal(g, kv * max_seq, hd).half() for _ in range(2))
+    qr, out, out4 = torch.empty_like(q), torch.empty(1, heads * hd, dtype=torch.float16, device=DEV), torch.empty(1, heads * hd, dtype=torch.float16, device=DEV)
+    held = [torch.empty(1, kv * hd, device=DEV) for _ in range(2)]
+    torch.cuda.synchronize()
+    table, cache, W = on.rope_table(max_seq, hd), Cache4(on, kv, max_seq, hd), on.wrap
+
+    def step():
+        W(qr).norm_rope_append(W(kc), W(vc), W(q), W(k), W(v), table, heads, kv, max_seq, pos)
+        W(out).attention_window(W(qr), W(kc), W(vc), heads, kv, max_seq, pos, 2500, 4)
+        cache.append(W(k), W(v), pos)
+        cache.read(W(held[0]), W(held[1]), pos)
+        cache.attention(W(out4), W(qr), heads, pos, 5)
+
+    step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for _ in range(3):
+        for x in (q, k, v):
+            x.copy_(normal(g, *x.shape))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in (qr, out, *held, out4)]
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (qr, out, *held, out4)))
+        assert torch.equal(held[0], values4(k.view(-1, hd)).view(1, -1)) and torch.equal(held[1], values4(v.view(-1, hd)).view(1, -1))
+    del graph
+    cache.free()
+    on.close()
+
+
+@pytest.mark.gpu
+def test_two_threads_on_one_context(cl):
+    """Calls from two host threads: each thread's results are those of its own inputs."""
+    import threading
+    g = gen(16)
+    heads, kv, hd, max_seq = 8, 1, 128, 20000
+    kc, vc = (normal(g, kv * max_seq, hd).half() for _ in range(2))
+    qs = [normal(g, n, heads * hd) for n in (1, 40)]
+    outs = [[torch.empty(q.shape, dtype=torch.float16, device=DEV) for _ in range(20)] for q in qs]
+    W = cl.wrap
+    args = [[(W(o), W(q)) for o in os] for os, q in zip(outs, qs)]
+    wk, wv = W(kc), W(vc)
+    torch.cuda.synchronize()
+
+    def work(i):
+        for o, q in args[i]:
+            o.attention_window(q, wk, wv, heads, kv, max_seq, 19000 - i * 7000, 18000, 3)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        k, v = (x.view(kv, max_seq, hd)[:, :19000 - i * 7000 + len(qs[i])] for x in (kc, vc))
+        want, spread, top = attention64(qs[i], k, v, heads, kv, hd, 19000 - i * 7000, 18000, 3)
+        tol = tolerance(want, spread, top, torch.float16, hd, 18003)
+        for o in outs[i]:
+            assert ((o.double() - want).abs() <= tol).all() and torch.equal(o, outs[i][0])
+
+
+@pytest.mark.gpu
 def test_ops_with_scratch_of_the_context_refuse_capture():
     from rllama_b200 import Cuda, RllamaError
     side = torch.cuda.Stream()
@@ -602,17 +766,26 @@ def test_wrapped_tensors_in_the_older_ops(cl):
     g = gen(14)
     for dt, tol in ((torch.float16, 2.0 ** -10), (torch.float32, 1e-5)):
         for rows in (1, 5, 40):
+            t = torch.full((rows, 64), 7.0, dtype=dt, device=DEV)
+            part = t[:, :21]
+            part.copy_(normal(g, rows, 21))
+            before = part.clone()
+            cl.wrap(part).silu_inplace()
+            cl.wrap(part).hadamard_product_inplace(cl.wrap(part))
+            want = torch.nn.functional.silu(before.double()).to(dt).double().square()
+            assert ((part.double() - want).abs() <= 4 * tol * (1 + want.abs())).all() and (t[:, 21:] == 7.0).all()
             wide = torch.full((rows, 64), math.nan, dtype=dt, device=DEV)
             x = wide[:, :19]
             x.copy_(normal(g, rows, 19))
             wide_w = torch.full((24, 48), math.nan, dtype=dt, device=DEV)
             w = wide_w[:, :19]
             w.copy_(normal(g, 24, 19))
-            y = torch.full((rows, 32), 7.0, dtype=dt, device=DEV)
-            cl.wrap(y[:, :24]).matrix_mul_inplace_transposed(cl.wrap(x), cl.wrap(w))
-            want = x.double() @ w.double().T
-            assert ((y[:, :24].double() - want).abs() <= tol * (1 + want.abs()) * 4).all()
-            assert (y[:, 24:] == 7.0).all()
+            for m in (24, 21):   # rows of w, i.e. columns of the product
+                y = torch.full((rows, 32), 7.0, dtype=dt, device=DEV)
+                cl.wrap(y[:, :m]).matrix_mul_inplace_transposed(cl.wrap(x), cl.wrap(w[:m]))
+                want = x.double() @ w[:m].double().T
+                assert ((y[:, :m].double() - want).abs() <= tol * (1 + want.abs()) * 4).all()
+                assert (y[:, m:] == 7.0).all()
             assert (cl.wrap(x).to_numpy() == x.cpu().numpy()).all()
 
 
@@ -706,6 +879,24 @@ def test_refusals(cl):
     lib, h = _ffi.lib(), ctypes.c_void_p()
     host = torch.zeros(64)
     assert lib.rlb_tensor_wrap(cl._h, ctypes.c_void_p(host.data_ptr() // 16 * 16), 1, 8, 8, 0, ctypes.byref(h)) == 1  # host memory
+    here = ctypes.c_void_p(base.data_ptr())
+    assert lib.rlb_tensor_wrap(cl._h, here, 1 << 44, 8, 8, 0, ctypes.byref(h)) == 1   # an end that is no memory
+    assert lib.rlb_tensor_wrap(cl._h, here, 1 << 62, 8, 8, 0, ctypes.byref(h)) == 1
+    assert lib.rlb_cache4_wrap(cl._h, here, here, here, here, 60000, 1 << 30, 128, ctypes.byref(h)) == 1
+    assert lib.rlb_cache4_create(cl._h, 1, (1 << 30) + 1, 128, ctypes.byref(h)) == 7
+    refused(lambda: Cache4(cl, 65536, 1 << 30, 128), 4)   # more than there is
+    assert torch.zeros(4, device=DEV).add_(1).sum().item() == 4   # none of these is an error of the caller's next call
+
+
+@pytest.mark.gpu
+def test_handles_may_outlive_their_context():
+    from rllama_b200 import Cache4, Cuda
+    on = Cuda(stream=torch.cuda.current_stream().cuda_stream)
+    table, cache, view, zeros = on.rope_table(16, 64), Cache4(on, 1, 16, 64), on.wrap(torch.zeros(4, 8, device=DEV)), on.zeros(4, 8, 0)
+    on.close()
+    for x in (table, cache, view, zeros):
+        x.free()
+    assert torch.zeros(4, device=DEV).add_(1).sum().item() == 4
 
 
 @pytest.mark.gpu
