@@ -83,8 +83,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     *reinterpret_cast<volatile int*>(err) = 4;
     return false;
 }
-// The same for a whole warp, with one answer for all of its lanes (they go on together or not at all).
+// The same for a whole warp, with one answer for all of its lanes (they go on together or not at all). What is there
+// already costs one look (512-row 4-bit chunk 150 us with the loop alone, 142 with it).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, dead, err));
 }
 // Waits, with the same limit, for work of the CTA's own that is in flight, whether or not the CTA gave up.

@@ -208,14 +208,17 @@ template <int KIND, int HD> struct Layout {
     static constexpr uint32_t STAGE = TK * HD * 2;
     static constexpr int STAGES = (TILES == 2 ? 8 : 4) * 128 / HD;
     static constexpr uint32_t TMEM_COLS = TILES * 256;
-    // warps: four a tile for the softmax, one a tile for its MMAs, then one that loads, or eight that unpack
-    static constexpr int SOFTMAX_WARPS = 4 * TILES, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = KIND == CACHE_Q4 ? 12 : MMA_WARP + TILES;
-    static constexpr int THREADS = (LOAD_WARP + (KIND == CACHE_Q4 ? 8 : 1)) * 32;
+    // warps: four a tile for the softmax, two a tile for its MMAs, then one that loads (and an idle one: registers are dealt to four warps
+    // at a time), or eight that unpack
+    static constexpr int SOFTMAX_WARPS = 4 * TILES, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = MMA_WARP + 2 * TILES;
+    static constexpr int THREADS = (LOAD_WARP + (KIND == CACHE_Q4 ? 8 : 2)) * 32;
     static constexpr size_t SMEM = TILES * Q_BYTES + STAGES * STAGE + 1024;
+    // A thread is launched with LAUNCH_REGS registers (65536 over the threads of an SM, in eights); the MMA and loading warps give theirs to the
+    // softmax warps, whose sum with what is left is what was launched: 128 * 160 + 128 * 96 = 256 * 128 (f16), 256 * 144 + 384 * 64 = 640 * 96.
+    static constexpr int LAUNCH_REGS = KIND == CACHE_Q4 ? 96 : 128, SOFTMAX_REGS = KIND == CACHE_Q4 ? 144 : 160, OTHER_REGS = KIND == CACHE_Q4 ? 64 : 96;
+    static_assert(SOFTMAX_WARPS * SOFTMAX_REGS + (THREADS / 32 - SOFTMAX_WARPS) * OTHER_REGS <= THREADS / 32 * LAUNCH_REGS, "the shares fit in the launch's registers");
+    static_assert((2 / TILES) * THREADS * LAUNCH_REGS <= 65536, "the CTAs of an SM fit in its registers");
 };
-// 4-bit: 640 threads are launched with 96 registers each. The MMA and unpacking warps give 32 of theirs to the softmax warps:
-// 8 * 32 * 144 + 12 * 32 * 64 = 61440 = 640 * 96.
-constexpr int kSoftmaxRegs = 144, kOtherRegs = 64;
 
 template <int KIND, int HD>
 __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD>::TILES)
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     extern __shared__ unsigned char smem_raw[];
     unsigned char* q_s = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // [tile][HD/64][128][64]
     unsigned char* ring = q_s + TILES * Y::Q_BYTES;                                                              // [stage][HD/64][128][64]
-    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], q_ready[2], drained[2];
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], q_ready[2], drained[4];
     __shared__ __align__(8) uint64_t p_ready[4], pv_done[4];   // [tile][buffer]: a phase is seen before the next one begins
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_flag;
@@ -259,12 +262,12 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         for (int b = 0; b < 4; b++) {
             mbar_init(&p_ready[b], 4);
             mbar_init(&pv_done[b], 1);
+            mbar_init(&drained[b], 1);
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
             mbar_init(&s_read[t], 4);
             mbar_init(&q_ready[t], 4);
-            mbar_init(&drained[t], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -280,12 +283,12 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
 
     if (warp >= Y::LOAD_WARP) {
         // ------------------------------- K and V steps into the ring -------------------------------------------------
-        if constexpr (KIND == CACHE_Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
         const int items = 2 * (j1 - j0);
         auto item_is_v = [&](int x) { return x > 0 && (x % 2 == 0 || x == items - 1); };
         auto item_step = [&](int x) { return j0 + (x == items - 1 ? x / 2 : item_is_v(x) ? x / 2 - 1 : (x + 1) / 2); };
         if constexpr (KIND == CACHE_F16) {
-            if (lane == 0) {
+            if (warp == Y::LOAD_WARP && lane == 0) {
                 int x = 0;
                 for (; x < items; x++) {
                     const int s = x % STAGES, j = item_step(x), t0 = st.at(j);
@@ -367,29 +370,31 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             }
         }
     } else if (warp >= Y::MMA_WARP) {
-        // ------------------------------- MMA issuer ------------------------------------------------------------------
-        if constexpr (KIND == CACHE_Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        // ------------------------------- MMA issuers -----------------------------------------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
+        // A warp for a tile's scores and one for its output products: a wait, a commit or the issue of eight MMAs costs 100 to 300 cycles each, and
+        // one warp with all of a step's was busy for 1800 cycles, about as long as the softmax (512-row 4-bit chunk 153 us, with two warps 149; 8192-row prompt 278 and
+        // 274).
+        // The whole warp runs this and one thread issues: descriptors then live in uniform registers (from a branch of one
+        // thread eight MMAs took 600 to 1400 cycles, longer than they run). Descriptors are a base plus a constant (the address is their low bits, in
+        // units of 16 bytes), and a step that the tile sees whole goes through straight-line code.
+        const int t = (warp - Y::MMA_WARP) % TILES;
+        const bool leader = elect_one();
+        // Steps that the tile sees whole: from the first that starts at its last row's window to the last that ends at its first row.
+        const int whole0 = st.n_first + max(0, window_low(a, pb[t]) - st.l + TK - 1) / TK, whole1 = t == 0 || two ? st.n_first + (pa[t] + 1 - st.l) / TK : 0;
+        auto cols_at = [&](int j) { return j >= whole0 && j < whole1 ? Cols{0, TK} : cols(t, j); };
+        uint32_t done = 0;   // products issued
+        bool ok = true;
         if (warp < Y::MMA_WARP + TILES) {
-            // The whole warp runs this and one thread issues: descriptors then live in uniform registers, and eight MMAs are
-            // issued in 200 cycles (from a branch of one thread it took 600 to 1400, longer than they run). Descriptors are a base plus
-            // a constant (the address is their low bits, in units of 16 bytes), and a step that the tile sees whole goes
-            // through straight-line code.
-            const bool leader = elect_one();
-            const int t = warp - Y::MMA_WARP;
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(QT >> 4) << 24);   // | N / 8 << 17
-            const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(QT >> 4) << 24);
-            const uint64_t q_desc = desc_kmajor(smem_u32(q_s) + t * Y::Q_BYTES);
-            const uint64_t k_desc = desc_kmajor(smem_u32(ring)), v_desc = desc_mnmajor(smem_u32(ring), TK * 128);
-            // Steps that the tile sees whole: from the first that starts at its last row's window to the last that ends at its first row.
-            const int whole0 = st.n_first + max(0, window_low(a, pb[t]) - st.l + TK - 1) / TK, whole1 = t == 0 || two ? st.n_first + (pa[t] + 1 - st.l) / TK : 0;
-            auto cols_at = [&](int j) { return j >= whole0 && j < whole1 ? Cols{0, TK} : cols(t, j); };
-            uint32_t scored = 0, done = 0;       // scores and output products issued; the n-th product takes its weights from buffer n & 1
-            uint32_t stage = 0, phase = 0;       // of the next item; items are used in the order in which they are loaded
-            auto advance = [&]() {
-                if (leader) umma_commit(&empty[stage]);
-                if (++stage == STAGES) { stage = 0; phase ^= 1; }
-            };
-            auto scores = [&](Cols c) {          // K of the next item
+            const uint64_t q_desc = desc_kmajor(smem_u32(q_s) + t * Y::Q_BYTES), k_desc = desc_kmajor(smem_u32(ring));
+            ok = warp_wait(&q_ready[t], 0, dead, err);
+            for (int j = j0; j < j1 && ok; j++) {
+                const uint32_t x = j == j0 ? 0 : 2 * (j - j0) - 1, stage = x % STAGES;   // the step's place among the items
+                const Cols c = cols_at(j);
+                ok = warp_wait(&full[stage], (x / STAGES) & 1, dead, err);
+                if (c.any() && done > 0) ok = ok && warp_wait(&s_read[t], (done - 1) & 1, dead, err);
+                if (!ok) break;
                 if (c.any()) {
                     tc_after();
                     const uint64_t kb = k_desc + (stage * Y::STAGE + (uint32_t)c.c0 * 128) / 16;
@@ -398,52 +403,44 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                     for (int k = 0; k < HD / 16; k++)
                         if (leader) umma_ss(d, q_desc + ((k >> 2) * (QT * 128) + (k & 3) * 32) / 16, kb + ((k >> 2) * (TK * 128) + (k & 3) * 32) / 16, id, k > 0);
                     if (leader) umma_commit(&s_full[t]);
-                    scored++;
+                    done++;
                 }
-                advance();
-            };
-            Cols now{0, 0}, next = cols_at(j0);
-            bool ok = warp_wait(&q_ready[t], 0, dead, err);
-            for (int j = j0 - 1; j < j1 && ok; j++) {   // scores of step j + 1, then the output product of step j
-                if (j + 1 < j1) {
-                    ok = warp_wait(&full[stage], phase, dead, err);
-                    if (next.any() && scored > 0) ok = ok && warp_wait(&s_read[t], (scored - 1) & 1, dead, err);
-                    if (!ok) break;
-                    scores(next);
-                }
-                if (j >= j0) {
-                    const uint32_t buf = done & 1;
-                    ok = warp_wait(&full[stage], phase, dead, err);
-                    if (now.any()) ok = ok && warp_wait(&p_ready[2 * t + buf], (done >> 1) & 1, dead, err);
-                    if (!ok) break;
-                    if (now.any()) {
-                        tc_after();
-                        const uint64_t vb = v_desc + stage * Y::STAGE / 16;
-                        const uint32_t d = tmem + O_COL + t * HD, w = tmem + 2 * t * TK + TK + buf * (TK / 2);
-                        if (now.c0 == 0 && now.c1 == TK) {
+                if (leader) umma_commit(&empty[stage]);
+            }
+        } else if (warp < Y::MMA_WARP + 2 * TILES) {
+            const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(QT >> 4) << 24);
+            const uint64_t v_desc = desc_mnmajor(smem_u32(ring), TK * 128);
+            for (int j = j0; j < j1; j++) {   // the n-th product takes its weights from buffer n & 1
+                const uint32_t x = j == j1 - 1 ? 2 * (j - j0) + 1 : 2 * (j - j0) + 2, stage = x % STAGES, buf = done & 1;
+                const Cols c = cols_at(j);
+                ok = warp_wait(&full[stage], (x / STAGES) & 1, dead, err);
+                if (c.any()) ok = ok && warp_wait(&p_ready[2 * t + buf], (done >> 1) & 1, dead, err);
+                if (!ok) break;
+                if (c.any()) {
+                    tc_after();
+                    const uint64_t vb = v_desc + stage * Y::STAGE / 16;
+                    const uint32_t d = tmem + O_COL + t * HD, w = tmem + 2 * t * TK + TK + buf * (TK / 2);
+                    if (c.c0 == 0 && c.c1 == TK) {
 #pragma unroll
-                            for (int k = 0; k < TK / 16; k++)
-                                if (leader) umma_ts(d, w + k * 8, vb + k * 2048 / 16, idesc_o, k > 0 || done > 0);
-                        } else {
-                            for (int k = now.c0 / 16; k < now.c1 / 16; k++)
-                                if (leader) umma_ts(d, w + k * 8, vb + k * 2048 / 16, idesc_o, k > now.c0 / 16 || done > 0);
-                        }
-                        if (leader) umma_commit(&pv_done[2 * t + buf]);
-                        done++;
+                        for (int k = 0; k < TK / 16; k++)
+                            if (leader) umma_ts(d, w + k * 8, vb + k * 2048 / 16, idesc_o, k > 0 || done > 0);
+                    } else {
+                        for (int k = c.c0 / 16; k < c.c1 / 16; k++)
+                            if (leader) umma_ts(d, w + k * 8, vb + k * 2048 / 16, idesc_o, k > c.c0 / 16 || done > 0);
                     }
-                    advance();
+                    if (leader) umma_commit(&pv_done[2 * t + buf]);
+                    done++;
                 }
-                now = next;
-                next = j + 2 < j1 ? cols_at(j + 2) : Cols{0, 0};
+                if (leader) umma_commit(&empty[stage]);
             }
-            if (!ok) {  // no product outlives the CTA (after a full run the softmax warps have waited for the last)
-                if (leader) umma_commit(&drained[t]);
-                mbar_drain(&drained[t], 0);
-            }
+        }
+        if (!ok) {  // no product outlives the CTA (after a full run the softmax warps have waited for the last)
+            if (leader) umma_commit(&drained[warp - Y::MMA_WARP]);
+            mbar_drain(&drained[warp - Y::MMA_WARP], 0);
         }
     } else {
         // ------------------------------- softmax: a thread owns a row ------------------------------------------------
-        if constexpr (KIND == CACHE_Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Y::SOFTMAX_REGS));
         const int tile = warp >> 2, r = threadIdx.x & (QT - 1);   // the thread's tile and row
         const int row = min(row0 + tile * QT + r, row_last);
         // First the queries, as f16 in the A operand's layout: row r, 16-byte chunk c of a 64-column block at r * 128 +
