@@ -49,6 +49,12 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
                  "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
 }
+// A thread's own 16-byte aligned piece of shared memory to global memory; the piece is free again on return.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("fence.proxy.async.shared::cta;\n cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n cp.async.bulk.commit_group;\n cp.async.bulk.wait_group.read 0;" ::"l"(dst),
+                 "r"(smem_u32(src)), "r"(bytes)
+                 : "memory");
+}
 // Shared-memory operand descriptors, 128-byte swizzle, groups of 8 rows 1024 bytes apart. K-major: a row is 128 bytes of the
 // contraction index. MN-major: a row is 64 output columns of one contraction index; the next 64 columns follow at lead_bytes.
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
@@ -204,7 +210,9 @@ template <int KIND, int HD> struct Layout {
     static constexpr int TILES = KIND == CACHE_Q4 ? 2 : 1;
     static constexpr int ROWS = TILES * QT;                  // rows of a CTA
     static constexpr int NB = HD / 64;                       // 64-column blocks of a row
-    static constexpr uint32_t Q_BYTES = QT * HD * 2;
+    // A tile's queries, 128 rows of f16 one after the other, and in the end its results, in rows that are 16 bytes longer (32 lanes that store
+    // 16 bytes of a row each then meet no bank twice).
+    static constexpr uint32_t OUT_ROW = HD * 2 + 16, Q_ROOM = QT * OUT_ROW;
     static constexpr uint32_t STAGE = TK * HD * 2;
     static constexpr int STAGES = (TILES == 2 ? 8 : 4) * 128 / HD;
     static constexpr uint32_t TMEM_COLS = TILES * 256;
@@ -212,7 +220,7 @@ template <int KIND, int HD> struct Layout {
     // at a time), or eight that unpack
     static constexpr int SOFTMAX_WARPS = 4 * TILES, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = MMA_WARP + 2 * TILES;
     static constexpr int THREADS = (LOAD_WARP + (KIND == CACHE_Q4 ? 8 : 2)) * 32;
-    static constexpr size_t SMEM = TILES * Q_BYTES + STAGES * STAGE + 1024;
+    static constexpr size_t SMEM = TILES * Q_ROOM + STAGES * STAGE + 1024;
     // A thread is launched with LAUNCH_REGS registers (65536 over the threads of an SM, in eights); the MMA and loading warps give theirs to the
     // softmax warps, whose sum with what is left is what was launched: 128 * 160 + 128 * 96 = 256 * 128 (f16), 256 * 144 + 384 * 64 = 640 * 96.
     static constexpr int LAUNCH_REGS = KIND == CACHE_Q4 ? 96 : 128, SOFTMAX_REGS = KIND == CACHE_Q4 ? 144 : 160, OTHER_REGS = KIND == CACHE_Q4 ? 64 : 96;
@@ -229,9 +237,10 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     constexpr uint32_t O_COL = TILES * 2 * TK;   // [tile]: S [TK], P [buffer][TK / 2]; then [tile]: O [HD]
     extern __shared__ unsigned char smem_raw[];
     unsigned char* q_s = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // [tile][HD/64][128][64]
-    unsigned char* ring = q_s + TILES * Y::Q_BYTES;                                                              // [stage][HD/64][128][64]
-    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], q_ready[2], drained[4];
+    unsigned char* ring = q_s + TILES * Y::Q_ROOM;                                                               // [stage][HD/64][128][64]
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], drained[4];
     __shared__ __align__(8) uint64_t p_ready[4], pv_done[4];   // [tile][buffer]: a phase is seen before the next one begins
+    __shared__ float c2_s[QB];   // a row's scores are s * c2 in units of log2 e
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_flag;
     volatile int* dead = &dead_flag;
@@ -253,7 +262,19 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     const bool two = TILES == 2 && row0 + QT <= row_last;  // the second tile has rows
     auto cols = [&](int t, int j) { return t == 0 || two ? step_cols(a, st, j, pa[t], pb[t]) : Cols{0, 0}; };
 
-    if (threadIdx.x == 0) {
+    // K and V steps pass through the ring as items K0 K1 V0 K2 V1 ...
+    const int items = 2 * (j1 - j0);
+    auto item_is_v = [&](int x) { return x > 0 && (x % 2 == 0 || x == items - 1); };
+    auto item_step = [&](int x) { return j0 + (x == items - 1 ? x / 2 : item_is_v(x) ? x / 2 - 1 : (x + 1) / 2); };
+    auto load = [&](int x) {   // f16, one thread
+        const int s = x % STAGES, j = item_step(x), t0 = st.at(j);
+        const bool v = item_is_v(x);
+        const CUtensorMap* map = j < st.n_first ? (v ? &tm_v_first : &tm_k_first) : (v ? &tm_v : &tm_k);
+        mbar_expect_tx(&full[s], Y::STAGE);
+#pragma unroll
+        for (int b = 0; b < NB; b++) tma_load_3d(ring + s * Y::STAGE + b * (TK * 128), map, b * 64, t0, kvh, &full[s]);
+    };
+    if (warp == Y::LOAD_WARP && lane == 0) {
         dead_flag = 0;
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&full[s], KIND == CACHE_Q4 ? 4 : 1);
@@ -267,14 +288,64 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
             mbar_init(&s_read[t], 4);
-            mbar_init(&q_ready[t], 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if constexpr (KIND == CACHE_F16)
+            for (int x = 0; x < min(items, STAGES); x++) load(x);
     }
+    __syncwarp();
     if (warp == Y::MMA_WARP) {
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(Y::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // The queries, as f16 in the A operand's layout: row r of a tile, 16-byte chunk c of a 64-column block at r * 128 + ((c ^ (r & 7)) * 16).
+    // Every warp takes batches of eight rows, lanes across head_dim, and has all of its loads on their way at once (the softmax warps alone, with one
+    // batch ahead, took 9000 cycles for four latencies; a CTA of the 1792-row window prompt lives 45000).
+    {
+        constexpr int N = HD / 32, B = 8, BATCHES = QB / B, WARPS = Y::THREADS / 32, MINE = (BATCHES + WARPS - 1) / WARPS;
+        float x[MINE][B][N];
+#pragma unroll
+        for (int k = 0; k < MINE; k++) {
+            const int y0 = (warp + k * WARPS) * B;
+            if (y0 >= QB) break;
+            int i = min(row0 + y0, row_last) / a.group, g = min(row0 + y0, row_last) - i * a.group;
+#pragma unroll
+            for (int u = 0; u < B; u++) {
+                const float* src = a.q + i * a.q_ld + (int64_t)(kvh * a.group + g) * HD + lane * N;
+                if constexpr (N == 4) *reinterpret_cast<float4*>(x[k][u]) = *reinterpret_cast<const float4*>(src);
+                else *reinterpret_cast<float2*>(x[k][u]) = *reinterpret_cast<const float2*>(src);
+                if (row0 + y0 + u < row_last && ++g == a.group) { g = 0; i++; }   // (behind the last row: that row again)
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < MINE; k++) {
+            const int y0 = (warp + k * WARPS) * B;
+            if (y0 >= QB) break;
+            float c2 = 0.f;
+#pragma unroll
+            for (int u = 0; u < B; u++) {
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(x[k][u][e]));
+                // the exponent of the largest magnitude, 2^e <= top < 2^(e+1); an infinite one keeps its factor (the row is
+                // not finite and is computed again)
+                int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+                e = e > 127 ? 0 : max(e, -100);
+                const float up = row0 + y0 + u <= row_last ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
+                if (lane == u) c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+                __half2 h[N / 2];
+#pragma unroll
+                for (int v = 0; v < N / 2; v++) h[v] = __floats2half2_rn(x[k][u][2 * v] * up, x[k][u][2 * v + 1] * up);
+                const int c = lane * N / 8;
+                unsigned char* dst = q_s + y0 / QT * Y::Q_ROOM + (c >> 3) * (QT * 128) + (y0 % QT + u) * 128 + (((c & 7) ^ u) << 4) + (lane * N % 8) * 2;
+                if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
+                else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
+            }
+            if (lane < B) c2_s[y0 + lane] = c2;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads these through the async proxy
     }
     tc_before();
     __syncthreads();
@@ -284,20 +355,13 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     if (warp >= Y::LOAD_WARP) {
         // ------------------------------- K and V steps into the ring -------------------------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
-        const int items = 2 * (j1 - j0);
-        auto item_is_v = [&](int x) { return x > 0 && (x % 2 == 0 || x == items - 1); };
-        auto item_step = [&](int x) { return j0 + (x == items - 1 ? x / 2 : item_is_v(x) ? x / 2 - 1 : (x + 1) / 2); };
         if constexpr (KIND == CACHE_F16) {
             if (warp == Y::LOAD_WARP && lane == 0) {
-                int x = 0;
+                int x = min(items, STAGES);   // (the first are on their way)
                 for (; x < items; x++) {
-                    const int s = x % STAGES, j = item_step(x), t0 = st.at(j);
-                    const bool v = item_is_v(x);
-                    const CUtensorMap* map = j < st.n_first ? (v ? &tm_v_first : &tm_k_first) : (v ? &tm_v : &tm_k);
-                    if (x >= STAGES && !mbar_wait(&empty[s], (x / STAGES - 1) & 1, dead, err)) break;
-                    mbar_expect_tx(&full[s], Y::STAGE);
-#pragma unroll
-                    for (int b = 0; b < NB; b++) tma_load_3d(ring + s * Y::STAGE + b * (TK * 128), map, b * 64, t0, kvh, &full[s]);
+                    const int s = x % STAGES;
+                    if (!mbar_wait(&empty[s], (x / STAGES - 1) & 1, dead, err)) break;
+                    load(x);
                 }
                 for (int y = max(0, x - STAGES); y < x; y++) mbar_drain(&full[y % STAGES], (y / STAGES) & 1);  // no copy outlives the CTA
             }
@@ -387,8 +451,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         bool ok = true;
         if (warp < Y::MMA_WARP + TILES) {
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(QT >> 4) << 24);   // | N / 8 << 17
-            const uint64_t q_desc = desc_kmajor(smem_u32(q_s) + t * Y::Q_BYTES), k_desc = desc_kmajor(smem_u32(ring));
-            ok = warp_wait(&q_ready[t], 0, dead, err);
+            const uint64_t q_desc = desc_kmajor(smem_u32(q_s) + t * Y::Q_ROOM), k_desc = desc_kmajor(smem_u32(ring));
             for (int j = j0; j < j1 && ok; j++) {
                 const uint32_t x = j == j0 ? 0 : 2 * (j - j0) - 1, stage = x % STAGES;   // the step's place among the items
                 const Cols c = cols_at(j);
@@ -443,57 +506,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Y::SOFTMAX_REGS));
         const int tile = warp >> 2, r = threadIdx.x & (QT - 1);   // the thread's tile and row
         const int row = min(row0 + tile * QT + r, row_last);
-        // First the queries, as f16 in the A operand's layout: row r, 16-byte chunk c of a 64-column block at r * 128 +
-        // ((c ^ (r & 7)) * 16). A warp fetches its 32 rows in batches of eight, lanes across head_dim, one batch ahead. (Straight-line
-        // code for 32 rows is slower: every CTA would fetch it anew.)
-        float c2 = 0.f;                                           // scores are s * c2 in units of log2 e
-        {
-            constexpr int N = HD / 32, B = 8;
-            const int first = tile * QT + (warp & 3) * 32;
-            int i = min(row0 + first, row_last) / a.group, g = min(row0 + first, row_last) - i * a.group, fetched = row0 + first;
-            auto fetch = [&](float (&x)[B][N]) {
-#pragma unroll
-                for (int u = 0; u < B; u++) {
-                    const float* src = a.q + i * a.q_ld + (int64_t)(kvh * a.group + g) * HD + lane * N;
-                    if constexpr (N == 4) *reinterpret_cast<float4*>(x[u]) = *reinterpret_cast<const float4*>(src);
-                    else *reinterpret_cast<float2*>(x[u]) = *reinterpret_cast<const float2*>(src);
-                    if (fetched++ < row_last && ++g == a.group) { g = 0; i++; }   // (behind the last row: that row again)
-                }
-            };
-            float x[B][N], ahead[B][N];
-            fetch(ahead);
-#pragma unroll 1
-            for (int y0 = 0; y0 < 32; y0 += B) {
-#pragma unroll
-                for (int u = 0; u < B; u++)
-#pragma unroll
-                    for (int e = 0; e < N; e++) x[u][e] = ahead[u][e];
-                if (y0 + B < 32) fetch(ahead);
-#pragma unroll
-                for (int u = 0; u < B; u++) {
-                    const int y = y0 + u;
-                    float top = 0.f;
-#pragma unroll
-                    for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(x[u][e]));
-                    // the exponent of the largest magnitude, 2^e <= top < 2^(e+1); an infinite one keeps its factor (the row is
-                    // not finite and is computed again)
-                    int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
-                    e = e > 127 ? 0 : max(e, -100);
-                    const float up = row0 + first + y <= row_last ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
-                    if (lane == y) c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
-                    __half2 h[N / 2];
-#pragma unroll
-                    for (int v = 0; v < N / 2; v++) h[v] = __floats2half2_rn(x[u][2 * v] * up, x[u][2 * v + 1] * up);
-                    const int c = lane * N / 8, yy = (warp & 3) * 32 + y;
-                    unsigned char* dst = q_s + tile * Y::Q_BYTES + (c >> 3) * (QT * 128) + yy * 128 + (((c & 7) ^ u) << 4) + (lane * N % 8) * 2;
-                    if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
-                    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads these through the async proxy
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_ready[tile]);
-        }
+        const float c2 = c2_s[tile * QT + r];
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem + lanes + 2 * tile * TK, o_addr = tmem + lanes + O_COL + tile * HD;
         const int p = a.start + row / a.group, low = window_low(a, p);
@@ -618,8 +631,11 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         const bool live = row0 + tile * QT + r <= row_last;
         if (ok && __any_sync(0xffffffffu, live)) {
             tc_after();
-            const int64_t rec = ((int64_t)row / a.group * a.heads + kvh * a.group + row % a.group) * a.n_split + blockIdx.y;
-            unsigned char* turn = q_s + tile * Y::Q_BYTES + (warp & 3) * (32 * HD * 2);   // (the tile's scores are all computed: its queries' room is free)
+            const int ii = row / a.group, head = kvh * a.group + row % a.group;
+            const int64_t rec = ((int64_t)ii * a.heads + head) * a.n_split + blockIdx.y;
+            // A row leaves through shared memory, from where one copy takes it out whole: the tile's scores are all computed, so its queries' room is
+            // free. (Stored from registers by 16 lanes a row this was 5600 cycles of a CTA.)
+            unsigned char *turn = q_s + tile * Y::Q_ROOM + (warp & 3) * (32 * Y::OUT_ROW), *mine = turn + lane * Y::OUT_ROW;
             const bool empty_row = p + 1 - low + min(a.sinks, low) == 0;
             const float inv = empty_row ? 0.f : 1.0f / l;
             float check = fmaf(l, 0.f, a.n_split == 1 ? inv * 0.f : 0.f);   // a NaN once anything is not finite
@@ -634,53 +650,47 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e++) check = fmaf(x[e], 0.f, check);
-                if (live && a.n_split > 1) {
+                if (a.n_split > 1) {   // half a record at a time
+                    unsigned char* dst = mine + c % (HD / 2) * 4;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(a.rec_o + rec * HD + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                } else if (a.n_split == 1) {
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + e * 4) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                    if ((c + 32) % (HD / 2) == 0) {
+                        if (live) bulk_store(a.rec_o + rec * HD + c + 32 - HD / 2, mine, HD * 2);
+                        __syncwarp();
+                    }
+                } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         __half2 h[4];
 #pragma unroll
                         for (int u = 0; u < 4; u++) h[u] = empty_row ? __half2half2(__ushort_as_half(0)) : __floats2half2_rn(x[e + 2 * u] * inv, x[e + 2 * u + 1] * inv);
-                        *reinterpret_cast<uint4*>(turn + lane * (HD * 2) + ((((c + e) / 8) ^ (lane & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
+                        *reinterpret_cast<uint4*>(mine + (c + e) * 2) = *reinterpret_cast<uint4*>(h);
                     }
-                }
-                __syncwarp();
-            }
-            if (a.n_split == 1) {   // out of the warp's rows in shared memory, a row's bytes side by side
-                constexpr int LPR = HD / 8;   // lanes a row
-                int i = min(warp_row, row_last) / a.group, g = min(warp_row, row_last) - i * a.group + lane / LPR;
-#pragma unroll 4
-                for (int y = 0; y < 32; y += 32 / LPR) {
-                    while (g >= a.group) { g -= a.group; i++; }
-                    const int yy = y + lane / LPR, chunk = lane % LPR;
-                    if (warp_row + yy <= row_last)
-                        *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(a.out) + i * a.out_ld + (int64_t)(kvh * a.group + g) * HD + chunk * 8) =
-                            *reinterpret_cast<const uint4*>(turn + yy * (HD * 2) + ((chunk ^ (yy & 7)) << 4));
-                    g += 32 / LPR;
                 }
             }
             if (live && a.n_split > 1) a.rec_ml[rec] = make_float2(m - kShift, l);
             // rows next to infinite or NaN cache contents, again and one by one
             __syncwarp();
             uint32_t bad = __ballot_sync(0xffffffffu, live && check != 0.f && !empty_row);
+            if (bad && a.n_split > 1) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // (their records are there and may be replaced)
+            __syncwarp();
             while (bad) {
                 const int b = __ffs(bad) - 1;
                 bad &= bad - 1;
-                const int again = __shfl_sync(0xffffffffu, row, b);
                 float o[HD / 32], sm, sl;
-                slow_row<KIND, HD>(a, kvh, again, j0, j1, st, sm, sl, o);
-                const int i = again / a.group, head = kvh * a.group + again % a.group;
-                const int64_t rb = ((int64_t)i * a.heads + head) * a.n_split + blockIdx.y;
+                slow_row<KIND, HD>(a, kvh, __shfl_sync(0xffffffffu, row, b), j0, j1, st, sm, sl, o);
+                const int64_t rb = __shfl_sync(0xffffffffu, rec, b);
 #pragma unroll
                 for (int e = 0; e < HD / 32; e++) {
                     const int c = lane * (HD / 32) + e;
                     if (a.n_split > 1) a.rec_o[rb * HD + c] = o[e];
-                    else reinterpret_cast<__half*>(a.out)[i * a.out_ld + head * HD + c] = __float2half_rn(o[e] / sl);
+                    else *reinterpret_cast<__half*>(turn + b * Y::OUT_ROW + c * 2) = __float2half_rn(o[e] / sl);
                 }
                 if (a.n_split > 1 && lane == 0) a.rec_ml[rb] = make_float2(sm, sl);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the row's own lane copies it)
+                __syncwarp();
             }
+            if (live && a.n_split == 1) bulk_store(reinterpret_cast<__half*>(a.out) + ii * a.out_ld + (int64_t)head * HD, mine, HD * 2);
         }
     }
     tc_before();
