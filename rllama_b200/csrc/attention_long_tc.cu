@@ -31,7 +31,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "attention_long.h"
 
@@ -222,8 +221,8 @@ template <int KIND, int HD> struct Layout {
     static constexpr int THREADS = (LOAD_WARP + (KIND == CACHE_Q4 ? 8 : 2)) * 32;
     static constexpr size_t SMEM = TILES * Q_ROOM + STAGES * STAGE + 1024;
     // A thread is launched with LAUNCH_REGS registers (65536 over the threads of an SM, in eights); the MMA and loading warps give theirs to the
-    // softmax warps, whose sum with what is left is what was launched: 128 * 160 + 128 * 96 = 256 * 128 (f16), 256 * 144 + 384 * 64 = 640 * 96.
-    static constexpr int LAUNCH_REGS = KIND == CACHE_Q4 ? 96 : 128, SOFTMAX_REGS = KIND == CACHE_Q4 ? 144 : 160, OTHER_REGS = KIND == CACHE_Q4 ? 64 : 96;
+    // softmax warps, whose sum with what is left is what was launched: 128 * 152 + 128 * 104 = 256 * 128 (f16), 256 * 120 + 384 * 80 = 640 * 96.
+    static constexpr int LAUNCH_REGS = KIND == CACHE_Q4 ? 96 : 128, SOFTMAX_REGS = KIND == CACHE_Q4 ? 120 : 152, OTHER_REGS = KIND == CACHE_Q4 ? 80 : 104;
     static_assert(SOFTMAX_WARPS * SOFTMAX_REGS + (THREADS / 32 - SOFTMAX_WARPS) * OTHER_REGS <= THREADS / 32 * LAUNCH_REGS, "the shares fit in the launch's registers");
     static_assert((2 / TILES) * THREADS * LAUNCH_REGS <= 65536, "the CTAs of an SM fit in its registers");
 };
@@ -515,51 +514,38 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         bool ok = true;
         const int warp_row = row0 + tile * QT + (warp & 3) * 32;   // the warp's first and last position
         const int wa = a.start + min(warp_row, row_last) / a.group, wb = a.start + min(warp_row + 31, row_last) / a.group;
-        const int low_wa = window_low(a, wa), low_wb = window_low(a, wb);
+        const int low_wb = window_low(a, wb);
         const uint64_t c2_2 = pack2(c2, c2);
-        // One step; `whole`: every row of the warp sees all of it.
-        auto step = [&](auto whole, int j, Cols now) {
-            constexpr bool W = decltype(whole)::value;
+        // One step; `whole`: every row of the warp sees all of it. One piece of code for both (with one for each, the rows' first steps waited for
+        // instructions: 1792-row window prompt 73 us, so 68); what a row does not see, or nobody computed, weighs 2^-inf.
+        auto step = [&](bool whole, int j, Cols now) {
             const uint32_t p_addr = s_addr + TK + (steps & 1) * (TK / 2);
-            // columns of the step that the row sees: below `to`, and from `from` on or below `first`
-            const int t0 = W ? 0 : st.at(j);
-            const bool in_first = j < st.n_first;
-            const int to = (in_first ? st.s : p + 1) - t0, from = (in_first ? 0 : low) - t0, first = (in_first ? 0 : a.sinks) - t0;
-            // a block of 32 columns is -1: not computed, 0: seen by nobody in the warp, 2: all of it seen by everybody, 1: else
-            auto block = [&](int c) {
-                if (c < now.c0 || c >= now.c1) return -1;
-                if (in_first) return c + 32 <= to ? 2 : 1;
-                if (c >= wb + 1 - t0 || (c + 32 <= low_wa - t0 && c >= first)) return 0;
-                return c + 32 <= wa + 1 - t0 && (c >= low_wb - t0 || c + 32 <= first) ? 2 : 1;
-            };
             float x[TK];
-            int kind[TK / 32];
-#pragma unroll
-            for (int c = 0; c < TK; c += 32) {
-                kind[c / 32] = W ? 2 : block(c);
-                if (kind[c / 32] > 0) {
-                    tmem_ld32_issue(s_addr + c, x + c);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) x[c + e] = -INFINITY;
-                }
-            }
+            tmem_ld32_issue(s_addr, x);
+            tmem_ld32_issue(s_addr + 32, x + 32);
             tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < TK; c += 32) tmem_arrived(x + c);
+            tmem_arrived(x);
+            tmem_arrived(x + 32);
             tc_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_read[tile]);   // the next scores may come
+            if (!whole) {
+                // columns of the step that the row sees: below `to`, and from `from` on or below `first`
+                const int t0 = st.at(j);
+                const bool in_first = j < st.n_first;
+                const int to = (in_first ? st.s : p + 1) - t0, from = (in_first ? 0 : low) - t0, first = (in_first ? 0 : a.sinks) - t0;
+                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+#pragma unroll
+                for (int c = 0; c < TK; c += 32) {
+                    const uint32_t sees = c < now.c0 || c >= now.c1 ? 0u : below(to - c) & (~below(from - c) | below(first - c));
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        if (!(sees >> e & 1)) x[c + e] = -INFINITY;
+                }
+            }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains
 #pragma unroll
-            for (int c = 0; c < TK; c += 32) {
-                if (kind[c / 32] == 1) {
-#pragma unroll
-                    for (int e = c; e < c + 32; e++) x[e] = (e < to && (e >= from || e < first)) ? x[e] : -INFINITY;
-                }
-#pragma unroll
-                for (int e = c; e < c + 32; e++) tops[e & 3] = fmaxf(tops[e & 3], x[e]);
-            }
+            for (int e = 0; e < TK; e++) tops[e & 3] = fmaxf(tops[e & 3], x[e]);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * c2;
             const bool move = top > m + kLag;
             if (__any_sync(0xffffffffu, move)) {
@@ -586,22 +572,16 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             uint64_t sum[2] = {0, 0};   // two chains of two
 #pragma unroll
             for (int c = 0; c < TK; c += 32) {
-                if (kind[c / 32] < 0) continue;
                 uint32_t y[16];
-                if (kind[c / 32] == 0) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) y[e] = 0;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        float w0, w1;
-                        unpack2(fma2(pack2(x[c + 2 * e], x[c + 2 * e + 1]), c2_2, shift_2), w0, w1);
-                        w0 = ex2_approx(w0);
-                        w1 = ex2_approx(w1);
-                        sum[e & 1] = add2(sum[e & 1], pack2(w0, w1));
-                        const __half2 h = __floats2half2_rn(w0, w1);
-                        y[e] = *reinterpret_cast<const uint32_t*>(&h);
-                    }
+                for (int e = 0; e < 16; e++) {
+                    float w0, w1;
+                    unpack2(fma2(pack2(x[c + 2 * e], x[c + 2 * e + 1]), c2_2, shift_2), w0, w1);
+                    w0 = ex2_approx(w0);
+                    w1 = ex2_approx(w1);
+                    sum[e & 1] = add2(sum[e & 1], pack2(w0, w1));
+                    const __half2 h = __floats2half2_rn(w0, w1);
+                    y[e] = *reinterpret_cast<const uint32_t*>(&h);
                 }
                 tmem_st16(p_addr + c / 2, y);
             }
@@ -619,8 +599,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             ok = warp_wait(&s_full[tile], steps & 1, dead, err);
             if (!ok) break;
             tc_after();
-            if (whole) step(std::true_type{}, j, now);
-            else step(std::false_type{}, j, now);
+            step(whole, j, now);
             tc_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[2 * tile + (steps & 1)]);
