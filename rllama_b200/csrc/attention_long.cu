@@ -210,8 +210,8 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     } else {
         // The kernel for few rows reads the cache once for every eight of them, the one for many rows has tiles of 128 (256 in 4 bits) that cost
         // the same however many of their rows there are. Each says what it expects to take, from what was measured; e.g. 32
-        // heads, 8000 positions, us with few / tiles: f16 8 rows 31 / 31, 16 rows 50 / 32, 64 rows 163 / 39; 4 bits 8 rows 21 / 52, 24 rows 62 / 52, 64
-        // rows 104 / 53; 300 positions: f16 32 rows 10 / 15, 64 rows 17 / 15; 4 bits 64 rows 13 / 21, 128 rows 23 / 21.
+        // heads, 8000 positions, us with few / tiles: f16 8 rows 31 / 31, 16 rows 49 / 33, 64 rows 163 / 38; 4 bits 8 rows 21 / 43, 24 rows 62 / 44, 64
+        // rows 104 / 46; 300 positions: f16 32 rows 10 / 13, 64 rows 17 / 14; 4 bits 64 rows 13 / 17, 128 rows 23 / 19.
         const AttnSplit s = attn_long_few_splits(ctx, kind, a);
         const int t = attn_long_tc_splits(ctx, kind, a);
         few = attn_long_few_us(ctx, kind, a, s) <= attn_long_tc_us(ctx, kind, a, t);

@@ -747,13 +747,15 @@ int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     return (int)best;
 }
 
-// 14 us (20 with the unpacking of 4-bit rows), and the longer of the CTAs' steps, 1.2 us each, and the reading of the cache.
+// 7 us (10 with the unpacking of 4-bit rows), the longer of the CTAs' steps, 1.15 us each (4 bits 1.3, with one tile 1.0), and the reading of the cache, and
+// for records 2.5 us and what it takes to write and read them.
 double attn_long_tc_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, int splits) {
     const int tiles = kind == CACHE_Q4 ? 2 : 1;
     const int64_t rows = tiles * QT, ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + rows - 1) / rows), slots = (int64_t)ctx->sm_count * (2 / tiles);
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + rows / a.group, (int64_t)a.start + a.n), steps = (seen + TK - 1) / TK;
-    const double bytes = (double)seen * a.kv_heads * (kind == CACHE_Q4 ? a.hd + a.hd / 8 : a.hd * 4);
-    return (kind == CACHE_Q4 ? 20 : 14) + std::max(1.2 * (double)((ctas * splits + slots - 1) / slots) * (double)((steps + splits - 1) / splits), bytes / 6.5e6);
+    const double bytes = (double)seen * a.kv_heads * (kind == CACHE_Q4 ? a.hd + a.hd / 8 : a.hd * 4), step = kind == CACHE_F16 ? 1.15 : (int64_t)a.n * a.group > QT ? 1.3 : 1.0;
+    const double records = splits > 1 ? 2.5 + 2.0 * a.n * a.heads * splits * (a.hd * 4 + 8) / 5e6 : 0;
+    return (kind == CACHE_Q4 ? 10 : 7) + std::max(step * (double)((ctas * splits + slots - 1) / slots) * (double)((steps + splits - 1) / splits), bytes / 6.5e6) + records;
 }
 
 int launch_attn_long_tc(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
