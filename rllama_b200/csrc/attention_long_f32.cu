@@ -3,6 +3,7 @@
 // of a K/V head, as in attention_long_tc.cu) and walks the positions that some of them see 64 at a time; a thread computes 4 x 4 scores,
 // then 4 x HD / 16 columns of the result, from operands that lie in shared memory in rows padded by 16 bytes (8 and 12 vector loads for 64 and
 // 128 FMAs). The weights take the place of the K tile. Two CTAs share an SM: one's loads fall into the other's arithmetic.
+// 400 rows after 8000 positions, 40 heads: 1.97 ms, 34 TFLOP/s (of about 75 that the FMA pipes have).
 // A zero weight times an infinite or NaN value is a NaN here too; such rows are computed again, one warp to a row.
 #include <algorithm>
 

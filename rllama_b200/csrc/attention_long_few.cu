@@ -17,6 +17,10 @@
 // finite is computed again from what it sees alone. Scores, maxima, sums and O are f32; rounded to f16: the weights
 // (2^-11) and the result.
 //
+// Measured: 65536 4-bit positions, 32 heads, one token, 94 us, 3.2 TB/s: 446 instructions for 16 positions of a head (185 of them integer and
+// conversions) at 61 % of the issue rate; 384 positions 6.4 us, of which about 5 are the call. 16384 f16 positions and 4 first tokens, 64 heads on 8,
+// 20.5 us, 3.3 TB/s: the second kernel and the ring's first fill are half of it.
+//
 // Loads straight into registers (two tiles ahead: 141 us, one: 107, of 65536 positions, 32 heads, 4 bits) wait for one another: a warp
 // tells its outstanding loads apart by six counters only.
 #include <algorithm>

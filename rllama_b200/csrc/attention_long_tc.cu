@@ -2,21 +2,28 @@
 // computed. Query rows that share a K/V head form one list, row = i * group + g, so a tile of 128 rows is full even when a
 // few tokens attend with many heads.
 //
-// A CTA owns 256 rows (two tiles of 128) of a K/V head and walks the positions that some of them see in steps of 128:
+// A CTA owns one tile of 128 rows of a K/V head (f16; two CTAs share an SM) or two (4 bits) and walks the positions that some of them see in
+// steps of 64:
 //  * K and V steps pass through a ring of shared-memory stages, in the order in which they are used: K0 K1 V0 K2 V1 K3 ...
 //    An f16 cache's are fetched by TMA (128-byte swizzle, the tensor's extent ends at the last visible position: rows
-//    behind it read as zeros). A 4-bit cache's are unpacked by four warps; its values are f16 numbers, so the unpacked
+//    behind it read as zeros). A 4-bit cache's are unpacked by eight warps; its values are f16 numbers, so the unpacked
 //    operand carries no rounding.
-//  * one thread a tile issues its MMAs: S = Q K^T (both operands in shared memory), then O += P V with P in tensor memory as
+//  * two warps a tile issue its MMAs: one S = Q K^T (both operands in shared memory), one O += P V with P in tensor memory as
 //    the A operand. Tensor memory holds, per tile, O, one buffer of 64 scores and two of 64 weights: the scores are free
 //    again as soon as the softmax has them in registers, so the next ones are computed during the exponentials, and a
 //    weight buffer is only needed again two steps later. Neither side waits for a chain of the other's. (Weights written
 //    over their scores made a step's chain softmax, output product, next scores: with one buffer of 128 scores 5200
 //    cycles for 256 x 128 scores, with two of 64 still 4000.)
-//  * eight warps do the softmax, a thread a row: maximum of the step's 64 scores, weights 2^(s - m + 7) rounded to f16
+//  * four warps a tile do the softmax, a thread a row: maximum of the step's 64 scores, weights 2^(s - m + 7) rounded to f16
 //    (their sum is taken before the rounding), back to tensor memory. The running maximum m is only moved when a row's
 //    scores exceed it by 2^8 (then the row's O is scaled in place); weights therefore stay below 2^15, and the factor
 //    2^7 keeps weights down to 2^-21 of the largest normal f16 numbers. It cancels in O / l.
+//
+// Measured: 8192 rows, 32 heads on 8, window 2048 and 16 first tokens, 253 us, 955 TFLOP/s (305 us in a long run, at the clock that the power limit
+// leaves); 1792 rows, 64 heads, window 512 and 4 first tokens, 68 us, 380 TFLOP/s; 512 rows after 7680 positions in 4 bits, 40 heads, 134 us,
+// 620 TFLOP/s. The bound is latency: a step of the softmax is 64 exponentials (512 of its 1900 cycles, twice that for the two tiles of an SM) between
+// waits, tensor-memory reads and writes of 100 to 200 cycles each; tensor and exponential units are 45 to 50 % busy. What did not shorten it: part of
+// the exponentials by a polynomial, two threads a row, fetching the next scores before the weights are known to have arrived.
 //
 // Rounded to f16 besides the result: the queries, scaled by a power of two per row so that their largest element lies in
 // [2^8, 2^9) whatever the row's magnitude (an error of at most 2^-11 sum |q k| / sqrt(head_dim) in a score), and the
