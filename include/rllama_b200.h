@@ -200,6 +200,11 @@ int rlb_cache4_free(rlb_cache4* c);
 /* Writes n rows of rotated k and v, n x (kv_heads*head_dim), both f32 or both f16, to positions
  * start_pos .. start_pos+n-1.                                                                 */
 int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, int32_t start_pos);
+/* rlb_norm_rope_append into a 4-bit cache: q to q_out (may be q itself), k normalised and rotated
+ * and v as it is to positions start_pos .. start_pos+n-1, all rows f32; the same arguments.  */
+int rlb_cache4_norm_rope_append(rlb_cache4* c, rlb_tensor* q_out, const rlb_tensor* q, const rlb_tensor* k, const rlb_tensor* v,
+                                const rlb_tensor* q_gain, const rlb_tensor* k_gain, float eps, const rlb_tensor* rope, int32_t heads,
+                                int32_t start_pos);
 /* The values held at positions start_pos .. start_pos+n-1 as n x (kv_heads*head_dim) f16 or f32
  * rows; either of k_out and v_out may be null. Exact in both dtypes.                          */
 int rlb_cache4_read(rlb_cache4* c, rlb_tensor* k_out, rlb_tensor* v_out, int32_t start_pos);

@@ -21,7 +21,7 @@ EXPORTS = [
     "rlb_copy_inplace", "rlb_transpose_from", "rlb_hadamard_product_inplace", "rlb_silu_inplace",
     "rlb_matrix_mul_inplace_transposed", "rlb_attention_decode", "rlb_attention_decode_static", "rlb_attention_prefill",
     "rlb_rope_table", "rlb_norm_rope_append", "rlb_attention_window",
-    "rlb_cache4_create", "rlb_cache4_wrap", "rlb_cache4_free", "rlb_cache4_append", "rlb_cache4_read", "rlb_cache4_attention",
+    "rlb_cache4_create", "rlb_cache4_wrap", "rlb_cache4_free", "rlb_cache4_append", "rlb_cache4_norm_rope_append", "rlb_cache4_read", "rlb_cache4_attention",
     "rlb_model_create", "rlb_model_set_tensor", "rlb_model_finalize", "rlb_model_free",
     "rlb_tp_nccl_unique_id", "rlb_tp_nccl_init", "rlb_tp_peer_export", "rlb_tp_peer_import", "rlb_tp_peer_import_local", "rlb_tp_set_mode",
     "rlb_caches_create", "rlb_caches_true_clone", "rlb_caches_shift_left", "rlb_caches_free", "rlb_caches_read",
@@ -88,6 +88,7 @@ def lib():
         "rlb_norm_rope_append": [vp] * 8 + [ctypes.c_float, vp, i32, i32, i32, i32],
         "rlb_attention_window": [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32],
         "rlb_cache4_create": [vp, i32, i32, i32, P(vp)], "rlb_cache4_wrap": [vp, vp, vp, vp, vp, i32, i32, i32, P(vp)], "rlb_cache4_free": [vp],
+        "rlb_cache4_norm_rope_append": [vp] * 7 + [ctypes.c_float, vp, i32, i32],
         "rlb_cache4_append": [vp, vp, vp, i32], "rlb_cache4_read": [vp, vp, vp, i32], "rlb_cache4_attention": [vp, vp, vp, i32, i32, i32, i32],
         "rlb_model_create": [vp, P(ModelParams), P(vp)],
         "rlb_model_set_tensor": [vp, ci, i32, vp, i64, i64, i64, ci],

@@ -31,33 +31,90 @@ template <> __device__ __forceinline__ void load8<__half>(const __half* p, float
 }
 
 struct AppendArgs {
-    const void* src[2];  // K and V rows
-    int64_t ld[2];
+    const void* src[3];  // K and V rows, and with the rotation q rows
+    int64_t ld[3];
     uint8_t* codes[2];
     __half* scales[2];
     int kv_heads, max_seq, start, n;
+    // with the rotation (what it computes: rotate.cu)
+    float* q_out;
+    int64_t qo_ld;
+    const float* gain[3];      // of K and q heads; null: no norm
+    const float* table;        // a position's row: (cos, sin) of pair 0, 1, ...
+    int64_t table_ld;
+    float eps;
+    int heads;
 };
 
-// Both kernels: grid (4 kv_heads / 128, rows, K and V). A thread takes the same block of eight values of every group of a head's row, HD / 4
+// All kernels: grid (4 kv_heads / 128, rows, K and V; with the rotation also q, whose rows go through f32 to where the caller wants them). A thread takes the same block of eight values of every group of a head's row, HD / 4
 // values, which is a quarter of the row's codes side by side (cache4.h); four threads make a row. No thread divides by a runtime size. (1792 rows
 // of 64 heads of 128, f32, written and read back: one word a thread, found by 64-bit division: 51 + 49 us; this: 28 + 13 us, of 20 + 11 that the
-// bytes take; two rows a thread, or CTAs of 256: 4 to 10 us more.)
+// bytes take; two rows a thread, or CTAs of 256: 4 to 10 us more. With the rotation, 64 heads of q beside them: 51 us,
+// 4.9 TB/s, where the two ops one after the other take 57 + 28; a token's row is the call's 5 us.)
 constexpr int kThreads = 128;
 template <int G> struct Words;   // a quarter of a row's codes, and its scales
 template <> struct Words<4> { typedef uint4 T; typedef uint2 D; };
 template <> struct Words<2> { typedef uint2 T; typedef uint32_t D; };
 
-template <typename T, int HD>
+// Normalises (with a gain) and rotates a thread's values of a head's row, which are whole pairs.
+template <int G> __device__ __forceinline__ void norm_rope(float (&y)[G][8], const float* gain, float eps, const float* turn) {
+    if (gain) {
+        float part[G], ss = 0.f;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            part[g] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) part[g] = fmaf(y[g][e], y[g][e], part[g]);
+            ss += part[g];
+        }
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+        const float s = 1.0f / sqrtf(ss / (float)(G * kQ4Group) + eps);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            float w[8];
+            load8<float>(gain + g * kQ4Group, w);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[g][e] = y[g][e] * s * w[e];
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        float f[8];
+        load8<float>(turn + g * kQ4Group, f);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float x0 = y[g][e], x1 = y[g][e + 1];
+            y[g][e] = __fsub_rn(__fmul_rn(x0, f[e]), __fmul_rn(x1, f[e + 1]));
+            y[g][e + 1] = __fadd_rn(__fmul_rn(x0, f[e + 1]), __fmul_rn(x1, f[e]));
+        }
+    }
+}
+
+template <typename T, int HD, bool ROTATE>
 __global__ void __launch_bounds__(kThreads) append4_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int G = HD / kQ4Group;
     const int x = blockIdx.x * kThreads + threadIdx.x, which = blockIdx.z, block = x & 3;
-    const bool live = x < a.kv_heads * 4;   // (a row's four threads are all live or none is)
+    const bool live = x < (which == 2 ? a.heads : a.kv_heads) * 4;   // (a row's four threads are all live or none is)
     const int head = live ? x >> 2 : 0;
     const T* src = reinterpret_cast<const T*>(a.src[which]) + head * HD + block * 8;
     for (int i = blockIdx.y; i < a.n; i += gridDim.y) {
         float y[G][8];
 #pragma unroll
         for (int g = 0; g < G; g++) load8<T>(src + i * a.ld[which] + g * kQ4Group, y[g]);
+        if constexpr (ROTATE) {
+            if (which != 1) norm_rope<G>(y, a.gain[which] ? a.gain[which] + block * 8 : nullptr, a.eps, a.table + (a.start + i) * a.table_ld + block * 8);
+            if (which == 2) {
+                float* dst = a.q_out + i * a.qo_ld + head * HD + block * 8;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    if (!live) break;
+                    *reinterpret_cast<float4*>(dst + g * kQ4Group) = make_float4(y[g][0], y[g][1], y[g][2], y[g][3]);
+                    *reinterpret_cast<float4*>(dst + g * kQ4Group + 4) = make_float4(y[g][4], y[g][5], y[g][6], y[g][7]);
+                }
+                continue;
+            }
+        }
         uint32_t w[G];
         __half d[G];
 #pragma unroll
@@ -212,22 +269,60 @@ int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, i
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
     DeviceScope dev(ctx->device);
     RLB_CUDA(dev.err);
-    AppendArgs a;
+    AppendArgs a = {};
     a.src[0] = k->d; a.src[1] = v->d; a.ld[0] = k->cap; a.ld[1] = v->cap;
     for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
     a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos;
     a.n = (int)k->rows;
     const dim3 grid = rows_grid(k->rows, c->kv_heads);
     if (k->dtype == RLB_F16) {
-        if (c->hd == 128) append4_kernel<__half, 128><<<grid, kThreads, 0, ctx->stream>>>(a);
-        else append4_kernel<__half, 64><<<grid, kThreads, 0, ctx->stream>>>(a);
+        if (c->hd == 128) append4_kernel<__half, 128, false><<<grid, kThreads, 0, ctx->stream>>>(a);
+        else append4_kernel<__half, 64, false><<<grid, kThreads, 0, ctx->stream>>>(a);
     } else {
-        if (c->hd == 128) append4_kernel<float, 128><<<grid, kThreads, 0, ctx->stream>>>(a);
-        else append4_kernel<float, 64><<<grid, kThreads, 0, ctx->stream>>>(a);
+        if (c->hd == 128) append4_kernel<float, 128, false><<<grid, kThreads, 0, ctx->stream>>>(a);
+        else append4_kernel<float, 64, false><<<grid, kThreads, 0, ctx->stream>>>(a);
     }
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
     return RLB_OK;
+}
+
+int rlb_cache4_norm_rope_append(rlb_cache4* c, rlb_tensor* q_out, const rlb_tensor* q, const rlb_tensor* k, const rlb_tensor* v,
+                                const rlb_tensor* q_gain, const rlb_tensor* k_gain, float eps, const rlb_tensor* rope, int32_t heads, int32_t start_pos) {
+    const char* who = "rlb_cache4_norm_rope_append";
+    if (!c || !q_out || !q || !k || !v || !rope) return rlb_fail(RLB_ERR_INVALID, "%s: null pointer", who);
+    RLB_TRY(check_rows(who, c, k, q->rows, start_pos));
+    RLB_TRY(check_rows(who, c, v, q->rows, start_pos));
+    const int64_t n = q->rows, hd = c->hd;
+    if (q->ctx != c->ctx || q_out->ctx != c->ctx || rope->ctx != c->ctx) return rlb_fail(RLB_ERR_INVALID, "%s: the rows and the cache live on different contexts", who);
+    for (const rlb_tensor* g : {q_gain, k_gain})
+        if (g && (g->ctx != c->ctx || g->dtype != RLB_F32 || g->rows != 1 || g->cols != hd)) return rlb_fail(RLB_ERR_INVALID, "%s: a gain must be 1 x head_dim f32", who);
+    if (heads < 1 || heads > 65536) return rlb_fail(RLB_ERR_INVALID, "%s: bad heads %d", who, heads);
+    if (q->dtype != RLB_F32 || q->cols != heads * hd || q_out->dtype != RLB_F32 || q_out->rows != n || q_out->cols != q->cols)
+        return rlb_fail(RLB_ERR_INVALID, "%s: q and q_out must be n x heads*head_dim f32", who);
+    if (k->dtype != RLB_F32 || v->dtype != RLB_F32) return rlb_fail(RLB_ERR_INVALID, "%s: k and v must be f32", who);
+    if (rope->dtype != RLB_F32 || rope->cols != hd || rope->rows < start_pos + n)
+        return rlb_fail(RLB_ERR_INVALID, "%s: the rope table must be f32, head_dim wide and cover position %lld", who, (long long)(start_pos + n - 1));
+    if (!(eps >= 0.f)) return rlb_fail(RLB_ERR_INVALID, "%s: eps must not be negative", who);
+    if (n == 0) return RLB_OK;
+    rlb_ctx* ctx = c->ctx;
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);
+    RLB_CUDA(dev.err);
+    AppendArgs a = {};
+    a.src[0] = k->d; a.src[1] = v->d; a.src[2] = q->d; a.ld[0] = k->cap; a.ld[1] = v->cap; a.ld[2] = q->cap;
+    for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
+    a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos; a.n = (int)n;
+    a.q_out = (float*)q_out->d; a.qo_ld = q_out->cap;
+    a.gain[0] = k_gain ? (const float*)k_gain->d : nullptr; a.gain[2] = q_gain ? (const float*)q_gain->d : nullptr;
+    a.table = (const float*)rope->d; a.table_ld = rope->cap; a.eps = eps; a.heads = heads;
+    dim3 grid = rows_grid(n, std::max(c->kv_heads, (int)heads));
+    grid.z = 3;
+    if (hd == 128) append4_kernel<float, 128, true><<<grid, kThreads, 0, ctx->stream>>>(a);
+    else append4_kernel<float, 64, true><<<grid, kThreads, 0, ctx->stream>>>(a);
+    RLB_LAUNCH_CHECK();
+    count_launch(ctx);
+    return tensor_mark_ready(q_out);
 }
 
 int rlb_cache4_read(rlb_cache4* c, rlb_tensor* k_out, rlb_tensor* v_out, int32_t start_pos) {

@@ -189,6 +189,11 @@ class Cache4:
         """Rows of rotated k and v (both f32 or both f16) to positions start_pos, start_pos + 1, ..."""
         check(_ffi.lib().rlb_cache4_append(self._h, k._h, v._h, start_pos))
 
+    def norm_rope_append(self, q_out, q, k, v, rope, heads, start_pos, q_gain=None, k_gain=None, eps=1e-6):
+        """``CudaTensor.norm_rope_append`` into this cache: q_out <- the rows of q, k and v to positions start_pos, start_pos + 1, ..."""
+        check(_ffi.lib().rlb_cache4_norm_rope_append(self._h, q_out._h, q._h, k._h, v._h, q_gain._h if q_gain is not None else None,
+                                                     k_gain._h if k_gain is not None else None, eps, rope._h, heads, start_pos))
+
     def read(self, k_out, v_out, start_pos):
         """The values held, into f16 or f32 rows; either may be None."""
         check(_ffi.lib().rlb_cache4_read(self._h, k_out._h if k_out is not None else None, v_out._h if v_out is not None else None, start_pos))

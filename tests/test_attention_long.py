@@ -26,6 +26,7 @@ def test_null_handles_are_errors_not_crashes():
     assert lib.rlb_cache4_append(None, None, None, 0) == 1
     assert lib.rlb_cache4_read(None, None, None, 0) == 1
     assert lib.rlb_cache4_attention(None, None, None, 1, 0, 1, 0) == 1
+    assert lib.rlb_cache4_norm_rope_append(None, None, None, None, None, None, None, 0.0, None, 1, 0) == 1
     assert lib.rlb_cache4_free(None) == 0
 
 
@@ -238,6 +239,91 @@ def test_cache4_append_and_read(cl, n, kv, start, dtype, pad, hd):
     for p in parts:  # the other rows stay as they were
         rows = p.view(kv, max_seq, -1)
         assert (rows[:, :start] == 9).all() and (rows[:, start + n:] == 9).all()
+
+
+def empty_like_cache(cl, kv, max_seq, hd):
+    from rllama_b200 import Cache4
+    parts = empty_cache4(kv, max_seq, hd)
+    for p in parts:
+        p.fill_(9)
+    return parts, Cache4.wrap(cl, *parts, kv, max_seq, hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,heads,kv,start,norm,pad", [(1, 1, 1, 0, True, 0), (1, 40, 40, 383, False, 0), (5, 6, 2, 7, True, 4), (70, 3, 33, 500, True, 8),
+                                                       (130, 34, 1, 29999, False, 0)])
+def test_cache4_norm_rope_append(cl, n, heads, kv, start, norm, pad, hd):
+    g = gen(19)
+    max_seq, eps = start + n + 3, 1e-5
+    q, k, v = (normal(g, n, h * hd + pad, scale=2.0)[:, :h * hd] for h in (heads, kv, kv))
+    gains = [1 + normal(g, 1, hd, scale=0.2) for _ in range(2)] if norm else [None, None]
+    table, W = cl.rope_table(max_seq, hd), cl.wrap
+    wg = [W(x) if norm else None for x in gains]
+    parts, cache = empty_like_cache(cl, kv, max_seq, hd)
+    q_out = torch.empty(n, heads * hd, device=DEV)
+    cache.norm_rope_append(W(q_out), W(q), W(k), W(v), table, heads, start, *wg, eps)
+    # the two steps one after the other
+    kc, vc = (torch.empty(kv * max_seq, hd, device=DEV) for _ in range(2))
+    parts2, cache2 = empty_like_cache(cl, kv, max_seq, hd)
+    q2 = torch.empty_like(q_out)
+    W(q2).norm_rope_append(W(kc), W(vc), W(q), W(k), W(v), table, heads, kv, max_seq, start, *wg, eps)
+    rows = [c.view(kv, max_seq, hd)[:, start:start + n].transpose(0, 1).reshape(n, kv * hd) for c in (kc, vc)]
+    cache2.append(W(rows[0]), W(rows[1]), start)
+    assert torch.equal(parts[2], parts2[2]) and torch.equal(parts[3], parts2[3])
+    if not norm:   # (the norm's sums are taken in another order)
+        assert torch.equal(q_out, q2) and torch.equal(parts[0], parts2[0]) and torch.equal(parts[1], parts2[1])
+    pos = torch.arange(start, start + n, dtype=torch.float64, device=DEV)[:, None, None]
+    ang = pos * 10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float64, device=DEV) / hd)
+
+    def turned(x, gain):
+        x = x.double().reshape(n, -1, hd)
+        if gain is not None:
+            x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * gain.double()
+        a, b = x[..., 0::2], x[..., 1::2]
+        return torch.stack([a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos()], -1).reshape(n, -1, hd), (a.abs() + b.abs()).repeat_interleave(2, -1)
+
+    # f32 steps: the norm's sum (eight terms one after the other, four groups, four threads: 13 roundings, of which the root keeps half), division, sum with
+    # eps, root, reciprocal, two products: 13; cos and sin one each, product and sum: 4
+    f32 = 20 * 2.0 ** -24
+    y, size = turned(q, gains[0])
+    assert ((q_out.double().reshape(n, heads, hd) - y).abs() <= f32 * size).all()
+    ko = torch.empty(n, kv * hd, device=DEV)
+    cache.read(W(ko), None, start)
+    y, size = turned(k, gains[1])
+    y, size = y.reshape(n, -1, 32), size.reshape(n, -1, 32)
+    step = (y.abs() + f32 * size).amax(-1, keepdim=True) / 7   # as for the append alone, of the rotated row's f32
+    assert ((ko.double().reshape(n, -1, 32) - y).abs() <= step * (0.5 + 7 * 2.0 ** -8) + 7 * 2.0 ** -25 + f32 * size).all()
+    for p in parts:
+        held = p.view(kv, max_seq, -1)
+        assert (held[:, :start] == 9).all() and (held[:, start + n:] == 9).all()
+    wq = W(q)
+    cache.norm_rope_append(wq, wq, W(k), W(v), table, heads, start, *wg, eps)   # in place
+    assert torch.equal(q, q_out)
+
+
+@pytest.mark.gpu
+def test_cache4_norm_rope_append_refusals(cl):
+    from rllama_b200 import Cuda, RllamaError
+    W, f16 = cl.wrap, torch.float16
+    cache, table = empty_like_cache(cl, 2, 10, 64)[1], cl.rope_table(10, 64)
+
+    def t(r, c, dt=torch.float32, on=cl):
+        return on.wrap(torch.zeros(r, c, dtype=dt, device=DEV))
+
+    def call(q_out=None, q=None, k=None, v=None, tab=table, heads=4, start=3, qg=None, kg=None, eps=1e-6):
+        cache.norm_rope_append(q_out or t(2, 256), q or t(2, 256), k or t(2, 128), v or t(2, 128), tab, heads, start, qg, kg, eps)
+
+    call()
+    call(q_out=t(0, 256), q=t(0, 256), k=t(0, 128), v=t(0, 128), start=10)
+    other = Cuda(stream=torch.cuda.current_stream().cuda_stream)
+    for bad in (dict(start=9), dict(start=-1), dict(heads=3), dict(heads=0), dict(q=t(3, 256)), dict(q_out=t(2, 128)), dict(q_out=t(2, 256, f16)), dict(q=t(2, 256, f16)),
+                dict(k=t(2, 64)), dict(k=t(3, 128)), dict(k=t(2, 128, f16)), dict(v=t(2, 128, f16)), dict(v=t(2, 256)), dict(tab=cl.rope_table(4, 64)),
+                dict(tab=cl.rope_table(10, 128)), dict(qg=t(1, 128)), dict(kg=t(2, 64)), dict(kg=t(1, 64, f16)), dict(eps=-1.0), dict(eps=math.nan),
+                dict(q=t(2, 256, on=other)), dict(k=t(2, 128, on=other)), dict(qg=t(1, 64, on=other)), dict(tab=other.rope_table(10, 64))):
+        with pytest.raises(RllamaError) as e:
+            call(**bad)
+        assert e.value.status == 1
 
 
 @pytest.mark.gpu
