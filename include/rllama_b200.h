@@ -180,7 +180,9 @@ int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_tensor* vcac
  * window of max_seq_len or more is none. A row that sees nothing (window 0, no sinks) is zero;
  * what unseen cache rows hold does not matter.
  *   q    n x (heads*head_dim) f32, rotated
- *   out  n x (heads*head_dim) in the cache dtype, not q                                     */
+ *   out  n x (heads*head_dim) in the cache dtype, not q
+ * f32 caches: f32 throughout. f16 caches: scores, maxima and sums in f32; the softmax weights
+ * and, with many rows, the queries (scaled by a power of two a row) are rounded to f16 once.  */
 int rlb_attention_window(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor* kcache, const rlb_tensor* vcache, int32_t heads,
                          int32_t kv_heads, int32_t max_seq_len, int32_t start_pos, int32_t window, int32_t sinks);
 

@@ -503,10 +503,8 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                 if (leader) umma_commit(&empty[stage]);
             }
         }
-        if (!ok) {  // no product outlives the CTA (after a full run the softmax warps have waited for the last)
-            if (leader) umma_commit(&drained[warp - Y::MMA_WARP]);
-            mbar_drain(&drained[warp - Y::MMA_WARP], 0);
-        }
+        if (leader) umma_commit(&drained[warp - Y::MMA_WARP]);   // no product outlives the CTA, whoever gave up
+        mbar_drain(&drained[warp - Y::MMA_WARP], 0);
     } else {
         // ------------------------------- softmax: a thread owns a row ------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Y::SOFTMAX_REGS));

@@ -736,7 +736,7 @@ def test_a_captured_step_follows_its_inputs():
     g = gen(15)
     q, k, v = normal(g, 1, heads * hd), normal(g, 1, kv * hd), normal(g, 1, kv * hd)
     kc, vc = (normal(g, kv * max_seq, hd).half() for _ in range(2))
-    qr, out, out4 = torch.empty_like(q), torch.empty(1, heads * hd, dtype=torch.float16, device=DEV), torch.empty(1, heads * hd, dtype=torch.float16, device=DEV)
+    qr, q4, out, out4 = torch.empty_like(q), torch.empty_like(q), torch.empty(1, heads * hd, dtype=torch.float16, device=DEV), torch.empty(1, heads * hd, dtype=torch.float16, device=DEV)
     held = [torch.empty(1, kv * hd, device=DEV) for _ in range(2)]
     torch.cuda.synchronize()
     table, cache, W = on.rope_table(max_seq, hd), Cache4(on, kv, max_seq, hd), on.wrap
@@ -746,7 +746,8 @@ def test_a_captured_step_follows_its_inputs():
         W(out).attention_window(W(qr), W(kc), W(vc), heads, kv, max_seq, pos, 2500, 4)
         cache.append(W(k), W(v), pos)
         cache.read(W(held[0]), W(held[1]), pos)
-        cache.attention(W(out4), W(qr), heads, pos, 5)
+        cache.norm_rope_append(W(q4), W(q), W(k), W(v), table, heads, pos)
+        cache.attention(W(out4), W(q4), heads, pos, 5)
 
     step()
     side.synchronize()
@@ -759,11 +760,11 @@ def test_a_captured_step_follows_its_inputs():
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
-        got = [x.clone() for x in (qr, out, *held, out4)]
+        got = [x.clone() for x in (qr, q4, out, *held, out4)]
         with torch.cuda.stream(side):
             step()
         torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for a, b in zip(got, (qr, out, *held, out4)))
+        assert all(torch.equal(a, b) for a, b in zip(got, (qr, q4, out, *held, out4))) and torch.equal(qr, q4)
         assert torch.equal(held[0], values4(k.view(-1, hd)).view(1, -1)) and torch.equal(held[1], values4(v.view(-1, hd)).view(1, -1))
     del graph
     cache.free()
