@@ -18,7 +18,9 @@ namespace {
 
 // One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits). A row reads what it sees for
 // itself, so the bound is the caches' reading for one row and L2 for several (8 rows after 10000 positions, 32 heads: 306 us, 8.6 TB/s from L2);
-// 77 rows of 8 heads on 4, window 100, are 10.3 us, half of them the call.
+// 77 rows of 8 heads on 4, window 100, are 9.4 us, half of them the call. Four rows of a K/V head to a CTA, each position fetched once for them, are no
+// faster (that case 15.6, 16 rows after 4000 positions 186 against 117; only 64 heads on 8 gain, 208 to 194), nor are two or four positions of a warp at
+// a time: more registers, fewer warps.
 template <int HD>
 __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a) {
     constexpr int N = HD / 32;
@@ -156,8 +158,10 @@ int launch_rows(rlb_ctx* ctx, const AttnLongArgs& a) {
     return RLB_OK;
 }
 int rows_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
-    // eight CTAs an SM, and at least 64 positions to a split
+    // Eight CTAs an SM, and at least 64 positions to a split, but 128 to the only one: the second kernel costs as much. (77 rows of 8 heads, window
+    // 100: one split 9.4 us, two 11.4; 16 rows of 8 heads, window 200: two 10.4, four 8.6.)
     const int64_t rows = (int64_t)a.n * a.heads, most = std::min<int64_t>((int64_t)a.sinks + a.window, (int64_t)a.start + a.n);
+    if (most <= 128) return 1;
     const int64_t splits = std::min<int64_t>((8 * ctx->sm_count + rows - 1) / rows, (most + 63) / 64);
     return (int)std::max<int64_t>(1, std::min<int64_t>(splits, 256));
 }
