@@ -20,7 +20,7 @@
 //    2^7 keeps weights down to 2^-21 of the largest normal f16 numbers. It cancels in O / l.
 //
 // Measured: 8192 rows, 32 heads on 8, window 2048 and 16 first tokens, 253 us, 955 TFLOP/s (305 us in a long run, at the clock that the power limit
-// leaves); 1792 rows, 64 heads, window 512 and 4 first tokens, 68 us, 380 TFLOP/s; 512 rows after 7680 positions in 4 bits, 40 heads, 134 us,
+// leaves); 1792 rows, 64 heads, window 512 and 4 first tokens, 66 us, 395 TFLOP/s; 512 rows after 7680 positions in 4 bits, 40 heads, 134 us,
 // 620 TFLOP/s. The bound is latency: a step of the softmax is 64 exponentials (512 of its 1900 cycles, twice that for the two tiles of an SM) between
 // waits, tensor-memory reads and writes of 100 to 200 cycles each; tensor and exponential units are 45 to 50 % busy. What did not shorten it: part of
 // the exponentials by a polynomial, two threads a row, fetching the next scores before the weights are known to have arrived.
@@ -237,7 +237,7 @@ template <int KIND, int HD> struct Layout {
 template <int KIND, int HD>
 __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD>::TILES)
     attn_long_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                        const __grid_constant__ CUtensorMap tm_k_first, const __grid_constant__ CUtensorMap tm_v_first, const __grid_constant__ AttnLongArgs a, int* err) {
+                        const __grid_constant__ CUtensorMap tm_k_first, const __grid_constant__ CUtensorMap tm_v_first, const __grid_constant__ AttnLongArgs a, int ahead, int* err) {
     typedef Layout<KIND, HD> Y;
     constexpr int NB = Y::NB, STAGES = Y::STAGES, TILES = Y::TILES, QB = Y::ROWS;
     constexpr uint32_t O_COL = TILES * 2 * TK;   // [tile]: S [TK], P [buffer][TK / 2]; then [tile]: O [HD]
@@ -370,6 +370,15 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                     load(x);
                 }
                 for (int y = max(0, x - STAGES); y < x; y++) mbar_drain(&full[y % STAGES], (y / STAGES) & 1);  // no copy outlives the CTA
+            } else if (warp > Y::LOAD_WARP && a.n_split == 1 && blockIdx.x + ahead < gridDim.x) {
+                // The queries of the CTA that will have this one's place, into L2: the CTAs of a round start together, and memory is idle in
+                // between (1792-row window prompt 68 us without, 66 with).
+                const int next = blockIdx.x + ahead, kv_next = next % a.kv_heads, first = ((n_rows + QB - 1) / QB - 1 - next / a.kv_heads) * QB;
+                for (int y = lane; y < QB && first + y < n_rows; y += 32) {
+                    const int row = first + y;
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.q + row / a.group * a.q_ld + (int64_t)(kv_next * a.group + row % a.group) * HD), "n"(HD * 4)
+                                 : "memory");
+                }
             }
         } else {
             // Two groups of four warps take every other item. A thread unpacks a quarter of a row: the same block of eight
@@ -729,7 +738,7 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
         attr_mark(set, ctx->device);
     }
     const int blocks = (a.n * a.group + Y::ROWS - 1) / Y::ROWS;
-    kern<<<dim3((unsigned)(blocks * a.kv_heads), a.n_split), Y::THREADS, Y::SMEM, ctx->stream>>>(mk, mv, mkf, mvf, a, ctx->d_err);
+    kern<<<dim3((unsigned)(blocks * a.kv_heads), a.n_split), Y::THREADS, Y::SMEM, ctx->stream>>>(mk, mv, mkf, mvf, a, ctx->sm_count * (2 / Y::TILES), ctx->d_err);
     RLB_LAUNCH_CHECK();
     count_launch(ctx);
     return RLB_OK;
