@@ -7,8 +7,9 @@
 //
 // All of it is f32; a cache row is rounded once, to the cache's dtype.
 //
-// Every value is read and written once, so memory is the bound: 1792 rows of 64 heads and 64 K/V heads of 128 into f16 caches take 57 us, 5.1 TB/s,
-// where one row a thread took 63 (two or eight: as long as four, or longer; streaming loads and stores too). A token's row is the call's 6 us.
+// Every value is read and written once, so memory is the bound: 1792 rows of 64 heads and 64 K/V heads of 128 into f16 caches, with the norm, take 49 us,
+// 5.9 TB/s (one row a thread at a time 63; two or eight no faster than four; streaming loads and stores neither). Instructions count beside it: with a
+// reduction over the warp, a square root and a division for every row it was 57. A token's row is the call's 5 us.
 #include "internal.h"
 
 #include <algorithm>
@@ -46,7 +47,7 @@ template <typename CT, int N> __device__ __forceinline__ void store_cache(CT* p,
 
 // grid (slots / 8, tokens): a warp per slot (the q heads, the k heads, the v heads) and U tokens, whose loads are all in flight. A lane
 // holds HD / 32 neighbouring values, i.e. whole pairs, and the norm's sum is one reduction over the warp.
-constexpr int U = 4;
+constexpr int U = 4;   // (the norm's sums are dealt to the lanes four rows at a time)
 
 template <typename CT, int HD>
 __global__ void __launch_bounds__(256) norm_rope_append_kernel(const __grid_constant__ RotateArgs a) {
@@ -61,41 +62,60 @@ __global__ void __launch_bounds__(256) norm_rope_append_kernel(const __grid_cons
     const float* gain = kind == 0 ? a.q_gain : kind == 1 ? a.k_gain : nullptr;
     float g[N];
     if (gain) *reinterpret_cast<V*>(g) = *reinterpret_cast<const V*>(gain + c);
+    CT* cache = reinterpret_cast<CT*>(kind == 2 ? a.vcache : a.kcache) + ((int64_t)head * a.max_seq + a.start) * HD + c;
+    const int lane = threadIdx.x & 31;
     for (int i0 = blockIdx.y * U; i0 < a.n; i0 += gridDim.y * U) {
+        const int last = a.n - 1 - i0;   // of the U rows
+        const float *p = src + i0 * ld, *t = a.table + (a.start + i0) * a.table_ld + c;
         float x[U][N], f[U][N];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int i = min(i0 + u, a.n - 1);
-            *reinterpret_cast<V*>(x[u]) = *reinterpret_cast<const V*>(src + i * ld);
-            if (kind != 2) *reinterpret_cast<V*>(f[u]) = *reinterpret_cast<const V*>(a.table + (a.start + i) * a.table_ld + c);
+            const int y = min(u, last);
+            *reinterpret_cast<V*>(x[u]) = *reinterpret_cast<const V*>(p + y * ld);
+            if (kind != 2) *reinterpret_cast<V*>(f[u]) = *reinterpret_cast<const V*>(t + y * a.table_ld);
         }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = i0 + u;
-            if (i >= a.n) break;
-            const int64_t row = ((int64_t)head * a.max_seq + a.start + i) * HD + c;
-            if (kind == 2) {
-                store_cache<CT, N>(reinterpret_cast<CT*>(a.vcache) + row, x[u]);
-                continue;
-            }
+        if (kind != 2) {
             if (gain) {
-                float ss = 0.f;
+                // The rows' sums of squares, four at a time: lanes hand on half of the rows that they hold until they hold one, eight lanes a row.
+                float ss[U];
 #pragma unroll
-                for (int e = 0; e < N; e++) ss = fmaf(x[u][e], x[u][e], ss);
+                for (int u = 0; u < U; u++) {
+                    ss[u] = 0.f;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float s = 1.0f / sqrtf(ss / (float)HD + a.eps);
+                    for (int e = 0; e < N; e++) ss[u] = fmaf(x[u][e], x[u][e], ss[u]);
+                }
+                const bool up = lane & 16, odd = lane & 8;
+                float s0 = (up ? ss[2] : ss[0]) + __shfl_xor_sync(0xffffffffu, up ? ss[0] : ss[2], 16);
+                float s1 = (up ? ss[3] : ss[1]) + __shfl_xor_sync(0xffffffffu, up ? ss[1] : ss[3], 16);
+                s0 = (odd ? s1 : s0) + __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 8);
 #pragma unroll
-                for (int e = 0; e < N; e++) x[u][e] = x[u][e] * s * g[e];
+                for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+                const float s = rsqrtf(s0 / (float)HD + a.eps);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const float su = __shfl_sync(0xffffffffu, s, 8 * u);
+#pragma unroll
+                    for (int e = 0; e < N; e++) x[u][e] = x[u][e] * su * g[e];
+                }
             }
-            float y[N];
 #pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                y[e] = __fsub_rn(__fmul_rn(x[u][e], f[u][e]), __fmul_rn(x[u][e + 1], f[u][e + 1]));
-                y[e + 1] = __fadd_rn(__fmul_rn(x[u][e], f[u][e + 1]), __fmul_rn(x[u][e + 1], f[u][e]));
-            }
-            if (kind == 0) *reinterpret_cast<V*>(a.q_out + i * a.qo_ld + head * HD + c) = *reinterpret_cast<const V*>(y);
-            else store_cache<CT, N>(reinterpret_cast<CT*>(a.kcache) + row, y);
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const float x0 = x[u][e], x1 = x[u][e + 1];
+                    x[u][e] = __fsub_rn(__fmul_rn(x0, f[u][e]), __fmul_rn(x1, f[u][e + 1]));
+                    x[u][e + 1] = __fadd_rn(__fmul_rn(x0, f[u][e + 1]), __fmul_rn(x1, f[u][e]));
+                }
+        }
+        if (kind == 0) {
+            float* dst = a.q_out + i0 * a.qo_ld + head * HD + c;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (u <= last) *reinterpret_cast<V*>(dst + u * a.qo_ld) = *reinterpret_cast<const V*>(x[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (u <= last) store_cache<CT, N>(cache + (int64_t)i0 * HD + u * HD, x[u]);
         }
     }
 }
