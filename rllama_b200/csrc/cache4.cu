@@ -46,17 +46,20 @@ struct AppendArgs {
     int heads;
 };
 
-// All kernels: grid (4 kv_heads / 128, rows, K and V; with the rotation also q, whose rows go through f32 to where the caller wants them). A thread takes the same block of eight values of every group of a head's row, HD / 4
-// values, which is a quarter of the row's codes side by side (cache4.h); four threads make a row. No thread divides by a runtime size. (1792 rows
-// of 64 heads of 128, f32, written and read back: one word a thread, found by 64-bit division: 51 + 49 us; this: 28 + 13 us, of 20 + 11 that the
-// bytes take; two rows a thread, or CTAs of 256: 4 to 10 us more. With the rotation, 64 heads of q beside them: 51 us,
-// 4.9 TB/s, where the two ops one after the other take 57 + 28; a token's row is the call's 5 us.)
+// All kernels: a grid over heads, rows, and K and V (with the rotation also q, whose rows go through f32 to where the caller wants them). A thread
+// takes the same block of eight values of every group of a head's row when it reads, which is a quarter of the row's codes side by side
+// (cache4.h), and of half of the groups when it writes; four or eight threads make a row. No thread divides by a runtime size. (1792 rows of 64
+// heads of 128, f32, written and read back: one word a thread, found by 64-bit division: 51 + 49 us; this: 27 + 13 us, of 20 + 11 that the bytes
+// take. A quarter row a thread in the append too: 28, as it leaves room for half of the warps; two rows a thread, or CTAs of 256: up to 10 us
+// more.) With the rotation, 64 heads of q beside them: 48.6 us, 5.2 TB/s (a quarter row a thread: 51.1), where the two ops one after the other take
+// 50 + 27; a token's row is the call's 4 us.
 constexpr int kThreads = 128;
-template <int G> struct Words;   // a quarter of a row's codes, and its scales
+template <int G> struct Words;   // a thread's words of a row, and their scales
 template <> struct Words<4> { typedef uint4 T; typedef uint2 D; };
+template <> struct Words<1> { typedef uint32_t T; typedef unsigned short D; };
 template <> struct Words<2> { typedef uint2 T; typedef uint32_t D; };
 
-// Normalises (with a gain) and rotates a thread's values of a head's row, which are whole pairs.
+// Normalises (with a gain) and rotates a thread's values of a head's row, which are whole pairs; eight neighbouring threads have the row.
 template <int G> __device__ __forceinline__ void norm_rope(float (&y)[G][8], const float* gain, float eps, const float* turn) {
     if (gain) {
         float part[G], ss = 0.f;
@@ -69,7 +72,8 @@ template <int G> __device__ __forceinline__ void norm_rope(float (&y)[G][8], con
         }
         ss += __shfl_xor_sync(0xffffffffu, ss, 1);
         ss += __shfl_xor_sync(0xffffffffu, ss, 2);
-        const float s = 1.0f / sqrtf(ss / (float)(G * kQ4Group) + eps);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 4);
+        const float s = 1.0f / sqrtf(ss / (float)(2 * G * kQ4Group) + eps);
 #pragma unroll
         for (int g = 0; g < G; g++) {
             float w[8];
@@ -93,19 +97,19 @@ template <int G> __device__ __forceinline__ void norm_rope(float (&y)[G][8], con
 
 template <typename T, int HD, bool ROTATE>
 __global__ void __launch_bounds__(kThreads) append4_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int G = HD / kQ4Group;
-    const int x = blockIdx.x * kThreads + threadIdx.x, which = blockIdx.z, block = x & 3;
-    const bool live = x < (which == 2 ? a.heads : a.kv_heads) * 4;   // (a row's four threads are all live or none is)
-    const int head = live ? x >> 2 : 0;
-    const T* src = reinterpret_cast<const T*>(a.src[which]) + head * HD + block * 8;
+    constexpr int ALL = HD / kQ4Group, G = ALL / 2;   // groups of a row, of a thread
+    const int x = blockIdx.x * kThreads + threadIdx.x, which = blockIdx.z, block = x & 3, half = x >> 2 & 1;
+    const bool live = x < (which == 2 ? a.heads : a.kv_heads) * 8;   // (a row's four threads are all live or none is)
+    const int head = live ? x >> 3 : 0;
+    const T* src = reinterpret_cast<const T*>(a.src[which]) + head * HD + half * (HD / 2) + block * 8;
     for (int i = blockIdx.y; i < a.n; i += gridDim.y) {
         float y[G][8];
 #pragma unroll
         for (int g = 0; g < G; g++) load8<T>(src + i * a.ld[which] + g * kQ4Group, y[g]);
         if constexpr (ROTATE) {
-            if (which != 1) norm_rope<G>(y, a.gain[which] ? a.gain[which] + block * 8 : nullptr, a.eps, a.table + (a.start + i) * a.table_ld + block * 8);
+            if (which != 1) norm_rope<G>(y, a.gain[which] ? a.gain[which] + half * (HD / 2) + block * 8 : nullptr, a.eps, a.table + (a.start + i) * a.table_ld + half * (HD / 2) + block * 8);
             if (which == 2) {
-                float* dst = a.q_out + i * a.qo_ld + head * HD + block * 8;
+                float* dst = a.q_out + i * a.qo_ld + head * HD + half * (HD / 2) + block * 8;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     if (!live) break;
@@ -129,8 +133,8 @@ __global__ void __launch_bounds__(kThreads) append4_kernel(const __grid_constant
         }
         if (!live) continue;
         const int64_t row = (int64_t)head * a.max_seq + a.start + i;
-        *reinterpret_cast<typename Words<G>::T*>(a.codes[which] + row * (HD / 2) + block * (HD / 8)) = *reinterpret_cast<const typename Words<G>::T*>(w);
-        if (block == 0) *reinterpret_cast<typename Words<G>::D*>(a.scales[which] + row * G) = *reinterpret_cast<const typename Words<G>::D*>(d);
+        *reinterpret_cast<typename Words<G>::T*>(a.codes[which] + row * (HD / 2) + block * (HD / 8) + half * (HD / 16)) = *reinterpret_cast<const typename Words<G>::T*>(w);
+        if (block == 0) *reinterpret_cast<typename Words<G>::D*>(a.scales[which] + row * ALL + half * G) = *reinterpret_cast<const typename Words<G>::D*>(d);
     }
 }
 
@@ -274,7 +278,7 @@ int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, i
     for (int w = 0; w < 2; w++) { a.codes[w] = c->codes[w]; a.scales[w] = c->scales[w]; }
     a.kv_heads = c->kv_heads; a.max_seq = c->max_seq; a.start = start_pos;
     a.n = (int)k->rows;
-    const dim3 grid = rows_grid(k->rows, c->kv_heads);
+    const dim3 grid = rows_grid(k->rows, 2 * c->kv_heads);
     if (k->dtype == RLB_F16) {
         if (c->hd == 128) append4_kernel<__half, 128, false><<<grid, kThreads, 0, ctx->stream>>>(a);
         else append4_kernel<__half, 64, false><<<grid, kThreads, 0, ctx->stream>>>(a);
@@ -316,7 +320,7 @@ int rlb_cache4_norm_rope_append(rlb_cache4* c, rlb_tensor* q_out, const rlb_tens
     a.q_out = (float*)q_out->d; a.qo_ld = q_out->cap;
     a.gain[0] = k_gain ? (const float*)k_gain->d : nullptr; a.gain[2] = q_gain ? (const float*)q_gain->d : nullptr;
     a.table = (const float*)rope->d; a.table_ld = rope->cap; a.eps = eps; a.heads = heads;
-    dim3 grid = rows_grid(n, std::max(c->kv_heads, (int)heads));
+    dim3 grid = rows_grid(n, 2 * std::max(c->kv_heads, (int)heads));
     grid.z = 3;
     if (hd == 128) append4_kernel<float, 128, true><<<grid, kThreads, 0, ctx->stream>>>(a);
     else append4_kernel<float, 64, true><<<grid, kThreads, 0, ctx->stream>>>(a);

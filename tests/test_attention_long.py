@@ -283,7 +283,7 @@ def test_cache4_norm_rope_append(cl, n, heads, kv, start, norm, pad, hd):
         a, b = x[..., 0::2], x[..., 1::2]
         return torch.stack([a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos()], -1).reshape(n, -1, hd), (a.abs() + b.abs()).repeat_interleave(2, -1)
 
-    # f32 steps: the norm's sum (eight terms one after the other, four groups, four threads: 13 roundings, of which the root keeps half), division, sum with
+    # f32 steps: the norm's sum (eight terms one after the other, up to four groups, eight threads: at most 14 roundings, of which the root keeps half), division, sum with
     # eps, root, reciprocal, two products: 13; cos and sin one each, product and sum: 4
     f32 = 20 * 2.0 ** -24
     y, size = turned(q, gains[0])
