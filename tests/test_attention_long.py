@@ -804,6 +804,43 @@ def test_two_threads_on_one_context(cl):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 300])
+def test_two_streams_at_once(n):
+    """Contexts on two streams, whose kernels share the SMs (and their tensor memory): each has the results that it has alone."""
+    from rllama_b200 import Cache4, Cuda
+    heads, kv, hd, max_seq = 8, 4, 128, 6000
+    start = max_seq - n
+    g = gen(20)
+    q = normal(g, n, heads * hd)
+    kc, vc = (normal(g, kv * max_seq, hd).half() for _ in range(2))
+    rows = [normal(g, max_seq, kv * hd) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ons = [Cuda(stream=s.cuda_stream) for s in streams]
+    outs = [[torch.empty(n, heads * hd, dtype=torch.float16, device=DEV) for _ in range(12)] for _ in range(2)]
+    torch.cuda.synchronize()
+    cache = Cache4(ons[1], kv, max_seq, hd)
+    cache.append(*(ons[1].wrap(x) for x in rows), 0)
+    calls = [lambda o: ons[0].wrap(o).attention_window(ons[0].wrap(q), ons[0].wrap(kc), ons[0].wrap(vc), heads, kv, max_seq, start, 4000, 4),
+             lambda o: cache.attention(ons[1].wrap(o), ons[1].wrap(q), heads, start)]
+    alone = []
+    for call in calls:
+        o = torch.empty(n, heads * hd, dtype=torch.float16, device=DEV)
+        torch.cuda.synchronize()
+        call(o)
+        torch.cuda.synchronize()
+        alone.append(o)
+    for i in range(12):
+        for k in range(2):
+            calls[k](outs[k][i])
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert torch.isfinite(alone[k]).all() and all(torch.equal(o, alone[k]) for o in outs[k])
+    cache.free()
+    for on in ons:
+        on.close()
+
+
+@pytest.mark.gpu
 def test_ops_with_scratch_of_the_context_refuse_capture():
     from rllama_b200 import Cuda, RllamaError
     side = torch.cuda.Stream()
