@@ -65,8 +65,9 @@ int rlb_ctx_create(int verbose, int nth_device, rlb_ctx** out);
 /* A context whose work goes to the caller's stream (a cudaStream_t of that device; NULL is the
  * legacy default stream), for hosts that mix the tier-1 ops with their own GPU work: the calls
  * follow what the caller queued before and come before what is queued after. The stream must
- * outlive the context and the caller's current device is left as it was. The ops say which of them
- * may be captured into a CUDA graph. Models need a context of their own stream (RLB_ERR_STATE).  */
+ * outlive the context and the caller's current device is left as it was. The per-thread default
+ * stream, which is another one in every host thread, is refused. The ops say which of them may be
+ * captured into a CUDA graph. Models need a context of their own stream (RLB_ERR_STATE).          */
 int rlb_ctx_create_on_stream(int verbose, int nth_device, void* cuda_stream, rlb_ctx** out);
 int rlb_ctx_destroy(rlb_ctx* ctx);
 /* OpenCL::flush (src/tensor_opencl_support.rs:130-132): waits for all queued work.    */

@@ -149,11 +149,13 @@ int rlb_ctx_create_on_stream(int verbose, int nth_device, void* cuda_stream, rlb
     if (!out) return rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create_on_stream: null out pointer");
     *out = nullptr;
     cudaStream_t s = (cudaStream_t)cuda_stream;
+    // That handle is another stream in every host thread, while the calls of a context share scratch because they follow one another on one stream.
+    if (s == cudaStreamPerThread) return rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create_on_stream: the per-thread default stream is not one stream");
     int before = -1;
     cudaGetDevice(&before);  // the caller's device stays current: it is the caller's stream that is used
     int status = ctx_new(verbose, nth_device, true, s, out);
-    // (the legacy and the per-thread default stream belong to whatever device is current: nothing to compare)
-    if (status == RLB_OK && s != nullptr && s != cudaStreamLegacy && s != cudaStreamPerThread) {
+    // (the legacy default stream belongs to whatever device is current: nothing to compare)
+    if (status == RLB_OK && s != nullptr && s != cudaStreamLegacy) {
         int dev = -1;
         cudaError_t e = cudaStreamGetDevice(s, &dev);
         if (e != cudaSuccess) status = rlb_fail(RLB_ERR_INVALID, "rlb_ctx_create_on_stream: not a stream: %s", cudaGetErrorString(e));

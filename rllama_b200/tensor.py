@@ -20,8 +20,8 @@ def capacity_cols(cols, dtype):
 
 class Cuda:
     """Counterpart of ``OpenCL`` (``OpenCL::new(verbose, nth_device)``). ``stream``: a CUDA stream handle (an integer, e.g.
-    ``torch.cuda.current_stream().cuda_stream``; 0 is the legacy default stream) that the ops are queued on, in order with the
-    caller's own work there; the stream must outlive the context. Without it the context has a stream of its own."""
+    ``torch.cuda.current_stream().cuda_stream``; 0 is the legacy default stream, the per-thread one is refused) that the ops are queued
+    on, in order with the caller's own work there; the stream must outlive the context. Without it the context has a stream of its own."""
 
     def __init__(self, verbose=False, nth_device=0, stream=None):
         self._h = ctypes.c_void_p()
