@@ -230,6 +230,7 @@ int rlb_tensor_upload(rlb_ctx* ctx, const void* host, int64_t rows, int64_t cols
     if (!host) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_upload: null host pointer");
     RLB_TRY(tensor_new(ctx, rows, cols, capacity_cols, dtype, out));
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);  // (a default stream is that of the current device)
     rlb_tensor* t = *out;
     cudaError_t e = cudaMemcpyAsync(t->d, host, t->bytes(), cudaMemcpyHostToDevice, ctx->stream);
     if (e == cudaSuccess) e = cudaEventRecord(t->ready, ctx->stream);
@@ -244,6 +245,7 @@ int rlb_tensor_upload(rlb_ctx* ctx, const void* host, int64_t rows, int64_t cols
 int rlb_tensor_zeros(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t capacity_cols, rlb_dtype dtype, rlb_tensor** out) {
     RLB_TRY(tensor_new(ctx, rows, cols, capacity_cols, dtype, out));
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
+    DeviceScope dev(ctx->device);  // (a default stream is that of the current device)
     rlb_tensor* t = *out;
     cudaError_t e = cudaMemsetAsync(t->d, 0, t->bytes(), ctx->stream);
     if (e == cudaSuccess) e = cudaEventRecord(t->ready, ctx->stream);
@@ -279,6 +281,8 @@ int rlb_tensor_wrap(rlb_ctx* ctx, void* device, int64_t rows, int64_t cols, int6
 
 int rlb_tensor_wait(rlb_tensor* t) {
     if (!t) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wait: null tensor");
+    DeviceScope dev(t->device);
+    RLB_CUDA(dev.err);
     if (t->ready && !t->ctx->borrowed_stream) RLB_CUDA(cudaEventSynchronize(t->ready));
     else RLB_CUDA(cudaStreamSynchronize(t->ctx->stream));  // (a graph that was replayed there has recorded no event)
     return ctx_check_error_word(t->ctx);

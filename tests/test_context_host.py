@@ -116,3 +116,21 @@ def test_the_per_thread_stream_is_refused(lib):
     for stream in (None, LEGACY, lib.fake_stream(0)):
         lib.rlb_ctx_destroy(context(lib, 0, stream))
     assert lib.rlb_ctx_create_on_stream(0, 1, ctypes.c_void_p(lib.fake_stream(0)), ctypes.byref(h)) == 1 and not h.value   # another device's
+
+
+@pytest.mark.parametrize("stream", [None, LEGACY])
+def test_the_default_stream_is_that_of_the_context_s_device(lib, stream):
+    """A context on device 1's default stream while device 0 is current: everything is queued on, and waited for, device 1."""
+    lib.fake_reset(0)
+    ctx, t, host, ev = context(lib, 1, stream), ctypes.c_void_p(), (ctypes.c_float * 32)(*range(32)), ctypes.c_void_p()
+    for make in (lambda: lib.rlb_tensor_zeros(ctx, 4, 8, 8, 0, ctypes.byref(t)), lambda: lib.rlb_tensor_upload(ctx, host, 4, 8, 8, 0, ctypes.byref(t))):
+        lib.fake_reset(0)
+        assert make() == 0, lib.rlb_last_error()
+        assert lib.rlb_tensor_wait(t) == 0 and lib.rlb_ctx_flush(ctx) == 0
+        assert lib.rlb_silu_inplace(t) == 0 and lib.rlb_copy_inplace(t, t) == 0
+        assert lib.rlb_tensor_download(t, host, ctypes.byref(ev)) == 0 and lib.rlb_event_wait(ev) == 0
+        log = [line.split() for line in lib.fake_log().decode().splitlines() if line != "event wait"]
+        assert len(log) >= 8 and all(line[1] == "1" for line in log), log
+        assert lib.fake_device() == 0
+        assert lib.rlb_tensor_free(t) == 0
+    assert lib.rlb_ctx_destroy(ctx) == 0 and lib.fake_device() == 0
