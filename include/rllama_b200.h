@@ -156,7 +156,8 @@ int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q, const rlb_
  * head_dim is 64 or 128; caches have up to 2^30 positions (RLB_ERR_LIMIT). Rows may be padded
  * (capacity_cols), caches may not. A call with no rows does nothing. What a call writes overlaps
  * none of its other arguments, unless said otherwise. On a context of the caller's stream these
- * ops may be captured into a CUDA graph (rlb_cache4_create and rlb_rope_table excepted): a graph
+ * ops may be captured into a CUDA graph (meanwhile RLB_ERR_STATE refuses what allocates or waits:
+ * rlb_cache4_create, rlb_rope_table, rlb_tensor_upload, zeros, wait, download, rlb_ctx_flush): a graph
  * then owns the scratch of its calls, so graphs may be replayed in any order and next to one
  * another. The shapes, pointers and positions are fixed at the time of capture. The context
  * outlives the graphs captured on it.

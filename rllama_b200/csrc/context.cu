@@ -58,6 +58,13 @@ int check_device_memory(const rlb_ctx* ctx, const void* p, const char* who) {
     return RLB_OK;
 }
 
+// Calls that allocate or wait, which would break the caller's capture, and ops whose scratch belongs to the context: a captured copy of these would
+// go on using scratch that the context may have replaced since, or that another graph uses at the same time.
+static int refuse_capture(const rlb_ctx* ctx, const char* op, const char* why = "its scratch belongs to the context") {
+    if (ctx_capturing(ctx)) return rlb_fail(RLB_ERR_STATE, "%s cannot be captured into a graph: %s", op, why);
+    return RLB_OK;
+}
+
 int OpWorkspace::get(rlb_ctx* c, size_t bytes) {
     ctx = c;
     if (ctx_capturing(c)) {
@@ -187,6 +194,7 @@ int rlb_ctx_flush(rlb_ctx* ctx) {
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
     DeviceScope dev(ctx->device);
     RLB_CUDA(dev.err);
+    RLB_TRY(refuse_capture(ctx, "rlb_ctx_flush", "it waits"));
     RLB_CUDA(cudaStreamSynchronize(ctx->stream));
     return ctx_check_error_word(ctx);
 }
@@ -206,9 +214,10 @@ static int tensor_new(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t cap, rlb
     // 128-bit vector access needs 16-byte aligned rows
     if ((cap * (int64_t)dtype_size(dtype)) % 16 != 0)
         return rlb_fail(RLB_ERR_INVALID, "tensor: capacity_cols %lld does not give 16-byte aligned rows", (long long)cap);
+    DeviceScope dev(ctx->device);
+    RLB_TRY(refuse_capture(ctx, "making a tensor", "it allocates"));
     rlb_tensor* t = new rlb_tensor();
     t->ctx = ctx; t->device = ctx->device; t->rows = rows; t->cols = cols; t->cap = cap; t->dtype = dtype;
-    DeviceScope dev(ctx->device);
     size_t bytes = t->bytes();
     cudaError_t e = cudaMalloc(&t->d, bytes ? bytes : 16);
     if (e != cudaSuccess) {
@@ -283,6 +292,7 @@ int rlb_tensor_wait(rlb_tensor* t) {
     if (!t) return rlb_fail(RLB_ERR_INVALID, "rlb_tensor_wait: null tensor");
     DeviceScope dev(t->device);
     RLB_CUDA(dev.err);
+    RLB_TRY(refuse_capture(t->ctx, "rlb_tensor_wait", "it waits"));
     if (t->ready && !t->ctx->borrowed_stream) RLB_CUDA(cudaEventSynchronize(t->ready));
     else RLB_CUDA(cudaStreamSynchronize(t->ctx->stream));  // (a graph that was replayed there has recorded no event)
     return ctx_check_error_word(t->ctx);
@@ -294,6 +304,7 @@ int rlb_tensor_download(rlb_tensor* t, void* host, rlb_event** out_event) {
     std::lock_guard<std::recursive_mutex> g(ctx->mu);
     DeviceScope dev(ctx->device);
     RLB_CUDA(dev.err);
+    RLB_TRY(refuse_capture(ctx, "rlb_tensor_download", "its event is one to wait for"));
     rlb_event* ev = new rlb_event();
     ev->ctx = ctx;
     cudaError_t e = cudaEventCreateWithFlags(&ev->ev, cudaEventDisableTiming);
@@ -337,13 +348,6 @@ int rlb_tensor_free(rlb_tensor* t) {
     }
     if (t->d) cudaFree(t->d);
     delete t;
-    return RLB_OK;
-}
-
-// Ops whose scratch belongs to the context: a captured copy of them would go on using scratch that the context may have
-// replaced since, or that another graph uses at the same time.
-static int refuse_capture(const rlb_ctx* ctx, const char* op) {
-    if (ctx_capturing(ctx)) return rlb_fail(RLB_ERR_STATE, "%s cannot be captured into a graph: its scratch belongs to the context", op);
     return RLB_OK;
 }
 

@@ -141,6 +141,8 @@ extern "C" int rlb_rope_table(rlb_ctx* ctx, int32_t max_seq_len, int32_t head_di
     *out = nullptr;
     if (max_seq_len < 1 || head_dim < 4 || head_dim % 4 != 0)
         return rlb_fail(RLB_ERR_INVALID, "rlb_rope_table: bad max_seq_len %d or head_dim %d (a multiple of 4)", max_seq_len, head_dim);
+    DeviceScope dev(ctx->device);
+    if (ctx_capturing(ctx)) return rlb_fail(RLB_ERR_STATE, "rlb_rope_table allocates: it cannot be captured into a graph");
     // compute_freqs_cis (src/transformer.rs:858-885): f64 angles, narrowed to f32 where they are applied
     float* tab = new (std::nothrow) float[(size_t)max_seq_len * head_dim];
     if (!tab) return rlb_fail(RLB_ERR_OOM, "rlb_rope_table: out of host memory");
@@ -152,7 +154,6 @@ extern "C" int rlb_rope_table(rlb_ctx* ctx, int32_t max_seq_len, int32_t head_di
             tab[(size_t)pos * head_dim + 2 * i + 1] = (float)sin(ang);
         }
     }
-    DeviceScope dev(ctx->device);
     int s = dev.err == cudaSuccess ? RLB_OK : rlb_fail(RLB_ERR_CUDA, "rlb_rope_table: %s", cudaGetErrorString(dev.err));
     if (s == RLB_OK) s = rlb_tensor_upload(ctx, tab, max_seq_len, head_dim, head_dim, RLB_F32, out);
     if (s == RLB_OK) s = rlb_tensor_wait(*out);

@@ -1,0 +1,49 @@
+"""What a caller may do with a context while its stream is captured into a CUDA graph: calls that cannot be part of a graph say so and leave the
+capture as it is, and handles may be dropped."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def on():
+    from rllama_b200 import Cuda
+    side = torch.cuda.Stream()
+    cl = Cuda(stream=side.cuda_stream)
+    yield cl, side
+    cl.close()
+
+
+def captured(on, during):
+    """x + 1 as a graph, with `during` called in between; x after three replays."""
+    cl, side = on
+    x = torch.zeros(4, 8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        x.add_(1)
+        during(cl.wrap(x))
+        x.add_(1)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    return x
+
+
+@pytest.mark.parametrize("what", ["zeros", "upload", "rope_table", "flush", "wait", "download", "cache4"])
+def test_calls_that_cannot_be_captured_leave_the_capture_alone(on, what):
+    from rllama_b200 import Cache4, RllamaError
+    cl = on[0]
+    calls = {"zeros": lambda x: cl.zeros(4, 8, 0), "upload": lambda x: cl.upload(np.zeros((4, 8), np.float32)), "rope_table": lambda x: cl.rope_table(8, 64),
+             "flush": lambda x: cl.flush(), "wait": lambda x: x.wait_until_ready(), "download": lambda x: x.to_numpy(), "cache4": lambda x: Cache4(cl, 1, 8, 64)}
+
+    def during(x):
+        with pytest.raises(RllamaError) as e:
+            calls[what](x)
+        assert e.value.status == 5
+
+    assert (captured(on, during) == 6).all()
+    if what != "flush":
+        calls[what](cl.wrap(torch.zeros(4, 8, device="cuda")))   # outside a capture all is well

@@ -134,3 +134,18 @@ def test_the_default_stream_is_that_of_the_context_s_device(lib, stream):
         assert lib.fake_device() == 0
         assert lib.rlb_tensor_free(t) == 0
     assert lib.rlb_ctx_destroy(ctx) == 0 and lib.fake_device() == 0
+
+
+def test_calls_that_cannot_be_captured_are_refused_before_they_reach_the_runtime(lib):
+    """Allocations and waits would break the capture of the caller's stream and report something else."""
+    lib.fake_reset(0)
+    ctx, t, u, host, ev = context(lib, 0, lib.fake_stream(0)), ctypes.c_void_p(), ctypes.c_void_p(), (ctypes.c_float * 32)(), ctypes.c_void_p()
+    assert lib.rlb_tensor_zeros(ctx, 4, 8, 8, 0, ctypes.byref(t)) == 0
+    lib.fake_reset(0)
+    lib.fake_capture(1)
+    for call in (lambda: lib.rlb_tensor_zeros(ctx, 4, 8, 8, 0, ctypes.byref(u)), lambda: lib.rlb_tensor_upload(ctx, host, 4, 8, 8, 0, ctypes.byref(u)),
+                 lambda: lib.rlb_tensor_wait(t), lambda: lib.rlb_ctx_flush(ctx), lambda: lib.rlb_tensor_download(t, host, ctypes.byref(ev))):
+        assert call() == 5 and lib.fake_log() == b"" and not u.value and not ev.value
+    assert lib.rlb_silu_inplace(t) == 0   # (an op that may be captured)
+    lib.fake_capture(0)
+    assert lib.rlb_tensor_wait(t) == 0 and lib.rlb_tensor_free(t) == 0 and lib.rlb_ctx_destroy(ctx) == 0
