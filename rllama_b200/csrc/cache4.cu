@@ -257,6 +257,7 @@ int rlb_cache4_free(rlb_cache4* c) {
     if (!c) return RLB_OK;
     if (c->owned) {
         DeviceScope dev(c->device);
+        OutsideCapture free_now;
         cudaFree(c->owned);  // waits for the device
     }
     delete c;

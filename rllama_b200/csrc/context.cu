@@ -342,6 +342,7 @@ int rlb_tensor_free(rlb_tensor* t) {
         return RLB_OK;
     }
     DeviceScope dev(t->device);  // (the context may be gone by now)
+    OutsideCapture free_now;
     if (t->ready) {
         cudaEventSynchronize(t->ready);  // the reference also waits for the initial write before dropping
         cudaEventDestroy(t->ready);

@@ -93,6 +93,13 @@ struct DeviceScope {
     ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
 };
 
+// Handles may be dropped while the thread captures some stream: a free is no part of the graph and may not end the capture.
+struct OutsideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Device scratch of one call. Eagerly it is the context's op_scratch (one stream, so calls follow one another); while the
 // stream is captured it is allocated and freed by nodes of the graph itself, so that graphs share no scratch with one
 // another or with eager calls and stay valid whatever the context does later.

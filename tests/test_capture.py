@@ -47,3 +47,22 @@ def test_calls_that_cannot_be_captured_leave_the_capture_alone(on, what):
     assert (captured(on, during) == 6).all()
     if what != "flush":
         calls[what](cl.wrap(torch.zeros(4, 8, device="cuda")))   # outside a capture all is well
+
+
+def test_handles_may_be_dropped_during_a_capture(on):
+    """As by a garbage collector: freeing them must not break the capture, and their memory comes back."""
+    from rllama_b200 import Cache4
+    cl = on[0]
+    before = torch.cuda.mem_get_info()[0]
+    room = 1 << 26
+    drop = [cl.zeros(16, room, 0), cl.rope_table(64, 64), Cache4(cl, 64, 1 << 16, 128), cl.wrap(torch.zeros(4, 8, device="cuda"))]
+    cl.flush()
+    held = torch.cuda.mem_get_info()[0]
+    assert before - held > 1 << 30
+
+    def during(x):
+        while drop:
+            drop.pop().free()
+
+    assert (captured(on, during) == 6).all()
+    assert torch.cuda.mem_get_info()[0] - held > 1 << 30
