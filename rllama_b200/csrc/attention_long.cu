@@ -160,6 +160,7 @@ int launch_rows(rlb_ctx* ctx, const AttnLongArgs& a) {
 int rows_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
     // Eight CTAs an SM, and at least 64 positions to a split, but 128 to the only one: the second kernel costs as much. (77 rows of 8 heads, window
     // 100: one split 9.4 us, two 11.4; 16 rows of 8 heads, window 200: two 10.4, four 8.6.)
+    if (ctx->attn_long_splits) return ctx->attn_long_splits;
     const int64_t rows = (int64_t)a.n * a.heads, most = std::min<int64_t>((int64_t)a.sinks + a.window, (int64_t)a.start + a.n);
     if (most <= 128) return 1;
     const int64_t splits = std::min<int64_t>((8 * ctx->sm_count + rows - 1) / rows, (most + 63) / 64);
@@ -210,7 +211,7 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
         const int t = attn_long_f32_splits(ctx, a), r = rows_splits(ctx, a);
         const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks, (int64_t)a.start + a.n);
         const double row_us = 5 + 0.12e-3 * (double)a.n * a.heads * (double)seen * (a.hd == 128 ? 1 : 0.7);
-        tiles = attn_long_f32_us(ctx, a, t) < row_us;
+        tiles = ctx->attn_long ? ctx->attn_long == 2 : attn_long_f32_us(ctx, a, t) < row_us;
         split.n = tiles ? t : r;
         split.records = split.n > 1;
     } else {
@@ -220,7 +221,7 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
         // rows 104 / 46; 300 positions: f16 32 rows 10 / 13, 64 rows 17 / 14; 4 bits 64 rows 13 / 17, 128 rows 23 / 19.
         const AttnSplit s = attn_long_few_splits(ctx, kind, a);
         const int t = attn_long_tc_splits(ctx, kind, a);
-        few = attn_long_few_us(ctx, kind, a, s) <= attn_long_tc_us(ctx, kind, a, t);
+        few = ctx->attn_long ? ctx->attn_long == 1 : attn_long_few_us(ctx, kind, a, s) <= attn_long_tc_us(ctx, kind, a, t);
         tiles = !few;
         split = few ? s : AttnSplit{t, t > 1};
     }

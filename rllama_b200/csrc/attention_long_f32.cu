@@ -211,6 +211,7 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
 }  // namespace
 
 int attn_long_f32_splits(rlb_ctx* ctx, const AttnLongArgs& a) {
+    if (ctx->attn_long_splits) return ctx->attn_long_splits;
     // rounds over the SMs times the steps of a split and about two more for its set-up and record
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + QT - 1) / QT), slots = (int64_t)ctx->sm_count * 2;
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + QT / a.group, (int64_t)a.start + a.n), steps = (seen + TK - 1) / TK;

@@ -570,6 +570,7 @@ static int64_t positions_seen(const AttnLongArgs& a, int rows) {
 }
 
 AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+    if (const int n = ctx->attn_long_splits) return {n, n > 1 && (ctx->attn_long_records || n > kMaxCluster)};
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
     const int64_t seen = positions_seen(a, kRows);
     // as many as fill the SMs, but at least a tile of 16 positions for every warp

@@ -749,6 +749,7 @@ int launch(rlb_ctx* ctx, const AttnLongArgs& a) {
 // Splits of the positions: CTAs run in rounds over the SMs, and a CTA costs its share of the steps and about eight more (set-up,
 // queries, masks, record or result). A split has at least eight steps.
 int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
+    if (ctx->attn_long_splits) return ctx->attn_long_splits;
     const int tiles = kind == CACHE_Q4 ? 2 : 1;
     const int64_t rows = tiles * QT, ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + rows - 1) / rows), slots = (int64_t)ctx->sm_count * (2 / tiles);
     const int64_t seen = std::min<int64_t>((int64_t)a.window + a.sinks + rows / a.group, (int64_t)a.start + a.n);

@@ -4,7 +4,9 @@
 // :999-1025, :2127-2206).
 #include "internal.h"
 
+#include <algorithm>
 #include <cstdarg>
+#include <cstdlib>
 #include <cstring>
 #include <new>
 
@@ -134,6 +136,11 @@ static int ctx_new(int verbose, int nth_device, bool borrow, cudaStream_t stream
     ctx->verbose = verbose != 0;
     ctx->borrowed_stream = borrow;
     ctx->stream = stream;
+    if (const char* e = getenv("RLB_ATTN_LONG")) ctx->attn_long = strcmp(e, "few") == 0 ? 1 : strcmp(e, "tiles") == 0 ? 2 : 0;
+    if (const char* e = getenv("RLB_ATTN_LONG_SPLITS")) {
+        ctx->attn_long_splits = std::min(std::max(atoi(e), 0), 64);
+        ctx->attn_long_records = strchr(e, 'r') != nullptr;
+    }
     cudaError_t se = borrow ? cudaSuccess : cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
     if (se == cudaSuccess) se = cudaHostAlloc((void**)&ctx->h_err, 64, cudaHostAllocMapped);
     if (se == cudaSuccess) {

@@ -57,6 +57,10 @@ struct rlb_ctx {
     // (each may start while its predecessor drains; every one of them waits for the predecessor before it
     // touches anything but weights)
     bool pdl_chain = false;
+    // Long-context attention, for tests and measurements (RLB_ATTN_LONG, RLB_ATTN_LONG_SPLITS when the context is made): the kernel
+    // (0: the one expected to be faster, 1: for few rows, 2: tiles), the number of splits (0: chosen) and whether records join them where a cluster could.
+    int attn_long = 0, attn_long_splits = 0;
+    bool attn_long_records = false;
 };
 int ctx_check_error_word(rlb_ctx* ctx);  // after a synchronisation: RLB_ERR_CUDA if a kernel raised the word
 

@@ -1,0 +1,144 @@
+"""Every kernel of the long-context attention, with its positions whole and split: which one a call gets goes by its expected time, and the
+shapes of small tests would leave some of them out. The contexts here name the kernel; the cases and their bounds are those of
+test_attention_long.py."""
+import contextlib
+import os
+
+import pytest
+
+import test_attention_long as T
+
+torch = T.torch
+pytestmark = pytest.mark.gpu
+
+# kind of cache, kernel, splits (r: joined through records, in the kernel for few rows; without it by a cluster)
+KERNELS = [("f32", "few", "1"), ("f32", "few", "3"), ("f32", "tiles", "1"), ("f32", "tiles", "3")] + [
+    (kind, *which) for kind in ("f16", "q4") for which in (("few", "1"), ("few", "3"), ("few", "3r"), ("tiles", "1"), ("tiles", "3"))]
+
+
+@contextlib.contextmanager
+def context(kernel, splits):
+    """A context on the current stream whose attention runs in the named kernel."""
+    from rllama_b200 import Cuda
+    names = {"RLB_ATTN_LONG": kernel, "RLB_ATTN_LONG_SPLITS": splits}
+    before = {name: os.environ.get(name) for name in names}
+    os.environ.update(names)
+    try:
+        cl = Cuda(stream=torch.cuda.current_stream().cuda_stream)
+    finally:
+        for name, value in before.items():
+            os.environ.pop(name) if value is None else os.environ.__setitem__(name, value)
+    yield cl
+    torch.cuda.synchronize()
+    cl.close()
+
+
+@pytest.fixture(params=KERNELS, ids="-".join)
+def on(request):
+    kind, kernel, splits = request.param
+    with context(kernel, splits) as cl:
+        yield kind, cl
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "q4"])
+def test_the_context_chooses(kind):
+    """One launch, or two where records are joined; and the two kernels differ in their last bits."""
+    q, k, v = T.normal(T.gen(0), 40, 8 * 128), T.normal(T.gen(1), 2, 500, 128), T.normal(T.gen(2), 2, 500, 128)
+    results = {}
+    for which in [(kernel, splits) for x, kernel, splits in KERNELS if x == kind]:
+        with context(*which) as cl:
+            before = cl.kernel_launches()
+            results[which] = T.attend(cl, q, k, v, 8, 2, 128, 460, 1000, 0, kind, 500)[0]
+            cluster = which == ("few", "3") and kind != "f32"
+            assert cl.kernel_launches() - before == (kind == "q4") + (1 if which[1] == "1" or cluster else 2)
+    assert not torch.equal(results["few", "1"], results["tiles", "1"])
+
+
+def test_shapes(on):
+    for shape in T.SHAPES:
+        T.check_attention(on[1], *shape, on[0])
+
+
+def test_long_contexts(on):
+    for shape in T.LONG:
+        T.check_attention(on[1], *shape, on[0])
+
+
+@pytest.mark.parametrize("window", [0, 1, 31, 32, 33, 64, 65, 127, 128, 129])
+def test_window_and_tile_edges(on, window):
+    T.test_attention_window_and_tile_edges(on[1], on[0], window)
+
+
+def test_random_shapes(on):
+    import random
+    for seed in range(20):
+        r = random.Random(100 + seed)
+        kv = r.choice([1, 2, 3, 5, 8])
+        heads, n = kv * r.choice([1, 1, 2, 3, 7, 8, 16]), r.choice([1, 1, 2, 7, 20, 55, 100, 190, 333])
+        start = int(2 ** r.uniform(0, 11.5)) - 1
+        T.check_attention(on[1], heads, kv, r.choice([64, 128]), n, start, r.choice([10 ** 9, r.randrange(1, start + n + 1), r.randrange(1, start + n + 1)]),
+                          r.choice([0, 0, 1, 4, 50, 10 ** 9]), on[0], seed=seed, max_seq=start + n + r.randrange(3))
+
+
+def test_strided_rows(on):
+    T.test_attention_strided_rows(on[1], on[0])
+
+
+@pytest.mark.parametrize("n", [1, 3, 150, 300])
+def test_rows_that_see_nothing_are_zero(on, n):
+    T.test_attention_rows_that_see_nothing_are_zero(on[1], on[0], n)
+
+
+@pytest.mark.parametrize("n,start,window,sinks", [(1, 900, 100, 4), (5, 900, 100, 4), (200, 700, 64, 3), (300, 0, 40, 0)])
+def test_unseen_rows_may_hold_anything(on, n, start, window, sinks):
+    T.test_attention_unseen_rows_may_hold_anything(on[1], on[0], n, start, window, sinks)
+
+
+@pytest.mark.parametrize("on", [x for x in KERNELS if x[0] != "q4"], ids="-".join, indirect=True)
+@pytest.mark.parametrize("n", [4, 40, 200])
+def test_a_bad_row_reaches_only_the_rows_that_see_it(on, n):
+    T.test_attention_a_bad_row_reaches_only_the_rows_that_see_it(on[1], on[0], n)
+
+
+@pytest.mark.parametrize("on", [x for x in KERNELS if x[0] == "q4"], ids="-".join, indirect=True)
+@pytest.mark.parametrize("n", [4, 40, 200, 300])
+def test_a_bad_group_of_a_4_bit_row_reaches_only_the_rows_that_see_it(on, n):
+    from rllama_b200 import Cache4
+    cl = on[1]
+    heads, kv, hd, start, window, sinks = 2, 1, 64, 50, 13, 2
+    total, at = start + n, start + n // 2
+    g = T.gen(6)
+    q, k, v = T.normal(g, n, heads * hd), T.normal(g, total, hd), T.normal(g, total, hd)
+    want, spread, top = T.attention64(q, *(T.values4(x).view(1, total, hd) for x in (k, v)), heads, kv, hd, start, window, sinks)
+    tol = T.tolerance(want, spread, top, torch.float16, hd, window + sinks)
+    sees = T.visible(start, n, window, sinks, total)[:, at]
+    for which in (0, 1):
+        parts = T.empty_cache4(kv, total, hd)
+        cache, out = Cache4.wrap(cl, *parts, kv, total, hd), torch.empty(n, heads * hd, dtype=torch.float16, device=T.DEV)
+        cache.append(cl.wrap(k), cl.wrap(v), 0)
+        parts[1 + 2 * which][at, 1] = float("nan")
+        cache.attention(cl.wrap(out), cl.wrap(q), heads, start, window, sinks)
+        bad = out.view(n, heads, 2, 32)[sees].isnan()
+        assert bad[:, :, 1].all() and (which == 1 or bad.all())
+        assert ((out[~sees].double() - want[~sees]).abs() <= tol[~sees]).all()
+        if which == 1:   # the other half of the result is that of the other values
+            good = torch.zeros(n, heads, hd, dtype=torch.bool, device=T.DEV)
+            good[..., :32] = True
+            good = good.view(n, -1)
+            assert ((out.double() - want).abs() <= tol)[good].all()
+
+
+@pytest.mark.parametrize("n", [1, 6, 140, 300])
+def test_flat_and_sharp(on, n):
+    for q_scale in (1e-6, 30.0):
+        T.test_attention_flat_and_sharp(on[1], on[0], n, q_scale)
+
+
+@pytest.mark.parametrize("n", [1, 140, 300])
+def test_magnitudes(on, n):
+    T.test_attention_magnitudes(on[1], on[0], n)
+
+
+@pytest.mark.parametrize("n", [5, 150])
+def test_a_bad_query_reaches_only_its_row(on, n):
+    T.test_attention_a_bad_query_reaches_only_its_row(on[1], on[0], n)
