@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
         const int row = row0 + min(r, rows - 1), p = a.start + row / a.group, low = window_low(a, p);
         float k0[KIND == CACHE_Q4 ? HD / kQ4Group : 1][2] = {};   // -8 times a group's sum of the row's high and low halves, times 2^-24
         float c2;
+        bool late = false;   // 4 bits: 2^24 is a factor of its own
         {
             const float* src = a.q + (int64_t)(row / a.group) * a.q_ld + (int64_t)(kvh * a.group + row % a.group) * HD + 8 * c;
             float x[KS][4], top = 0.f;
@@ -304,7 +305,9 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
                         k0[g][h] += __shfl_xor_sync(0xffffffffu, k0[g][h], 2);
                         k0[g][h] *= -8.f / 16777216.f;
                     }
-                c2 *= 16777216.f;
+                // (with queries from 2^112 on the factor of all would not be finite, although their scores are; then it is applied in two)
+                late = __any_sync(0xffffffffu, c2 > 0x1p103f);
+                if (!late) c2 *= 16777216.f;
             }
         }
         // the thread's places in a stage
@@ -367,6 +370,10 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] *= c2;
+            if (KIND == CACHE_Q4 && late) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] *= 16777216.f;
+            }
             // (a block of one position sees all of its share)
             bool whole = v + 16 <= v1 && (v >= run.s || v + 16 <= run.s);
             if (pa != pb) { const int t0 = run.at(v); whole = whole && t0 + 15 <= pa && (t0 >= window_low(a, pb) || t0 + 15 < a.sinks); }

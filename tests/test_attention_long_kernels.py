@@ -142,3 +142,34 @@ def test_magnitudes(on, n):
 @pytest.mark.parametrize("n", [5, 150])
 def test_a_bad_query_reaches_only_its_row(on, n):
     T.test_attention_a_bad_query_reaches_only_its_row(on[1], on[0], n)
+
+
+def check_best_row(cl, kind, n, size):
+    """One-hot queries whose scores lie further apart than f32 can weigh: the result is the value of the largest score, or the mean of equal ones.
+    (c of them: each weight may be rounded to f16 after it was added to their sum, 2^-11; the sum of c, the division and a product are c + 8 half steps
+    of f32; the result is rounded to its type.)"""
+    heads, kv, hd, start, window, total = 2, 1, 64, 200 - n, 90, 200
+    g = T.gen(17)
+    key = torch.arange(total, device=T.DEV)[torch.randperm(total, generator=g, device=T.DEV)]
+    k, v = torch.zeros(kv, total, hd, device=T.DEV), T.normal(g, kv, total, hd)
+    k[0, :, 0] = torch.where(key < 128, 1 + key / 128, 2 + (key - 128) / 64)
+    q = torch.zeros(n, heads, hd, device=T.DEV)
+    q[:, 0, 0], q[:, 1, 0] = size, -size
+    out, k, v = T.attend(cl, q.view(n, -1), k, v, heads, kv, hd, start, window, 3, kind, total + 10)
+    sees = T.visible(start, n, window, 3, total)
+    half, weight = torch.finfo(out.dtype).eps / 2, 0.0 if kind == "f32" else 2.0 ** -11
+    for h, sign in ((0, 1), (1, -1)):
+        s = (sign * k[0, :, 0].double()).expand(n, total).masked_fill(~sees, -float("inf"))
+        best = (s == s.amax(1, keepdim=True)).double()
+        count = best.sum(1, keepdim=True)
+        want, spread = (best @ x / count for x in (v[0].double(), v[0].double().abs()))
+        off = (out.view(n, heads, hd)[:, h].double() - want).abs()
+        assert (off <= half * want.abs() * (1 + weight) + (weight + (count + 8) * 2.0 ** -24) * spread + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("on", [x for x in KERNELS if x[1] == "few"], ids="-".join, indirect=True)
+@pytest.mark.parametrize("n", [1, 5, 150])
+@pytest.mark.parametrize("size", [1e30, 1e33, 1e34, 1e36, 1e37])
+def test_queries_next_to_the_largest_f32(on, n, size):
+    """Scores that f32 can still hold are computed without a step that it cannot."""
+    check_best_row(on[1], on[0], n, size)
