@@ -523,7 +523,9 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem + lanes + 2 * tile * TK, o_addr = tmem + lanes + O_COL + tile * HD;
         const int p = a.start + row / a.group, low = window_low(a, p);
-        float m = -FLT_MAX, l = 0.f;
+        // The row's weights are 2^(s c2 + shift), shift = kShift - m (FLT_MAX: nothing seen yet). It is the rounded shift that counts everywhere, in a
+        // move's factor and in a record too: with scores beyond 2^23 it is not kShift - m any more.
+        float shift = FLT_MAX, l = 0.f;
         uint32_t steps = 0;
         bool ok = true;
         const int warp_row = row0 + tile * QT + (warp & 3) * 32;   // the warp's first and last position
@@ -561,10 +563,10 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
 #pragma unroll
             for (int e = 0; e < TK; e++) tops[e & 3] = fmaxf(tops[e & 3], x[e]);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * c2;
-            const bool move = top > m + kLag;
+            const bool move = top + shift > kShift + kLag;
             if (__any_sync(0xffffffffu, move)) {
-                const float m_new = move ? top : m, scale = ex2_approx(m - m_new);
-                m = m_new;
+                const float shift_new = move ? kShift - top : shift, scale = ex2_approx(shift_new - shift);
+                shift = shift_new;
                 l *= scale;
                 if (steps > 0) {
                     ok = warp_wait(&pv_done[2 * tile + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, dead, err);   // O is at rest
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                     tmem_st_wait();
                 }
             }
-            const uint64_t shift_2 = pack2(kShift - m, kShift - m);
+            const uint64_t shift_2 = pack2(shift, shift);
             if (steps >= 2) ok = warp_wait(&pv_done[2 * tile + (steps & 1)], ((steps - 2) >> 1) & 1, dead, err) && ok;   // the weights two steps ago are used
             uint64_t sum[2] = {0, 0};   // two chains of two
 #pragma unroll
@@ -661,10 +663,12 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                     }
                 }
             }
-            if (live && a.n_split > 1) a.rec_ml[rec] = make_float2(m - kShift, l);
-            // rows next to infinite or NaN cache contents, again and one by one
+            if (live && a.n_split > 1) a.rec_ml[rec] = make_float2(-shift, l);
+            // Rows next to infinite or NaN cache contents, again and one by one. So are those whose largest weight, 2^kShift when it was taken, has come out
+            // as less than half of that or too large for f16: top is rounded before it is subtracted, the scores are not, and for scores beyond 2^23 the
+            // difference is no longer small against 1.
             __syncwarp();
-            uint32_t bad = __ballot_sync(0xffffffffu, live && check != 0.f && !empty_row);
+            uint32_t bad = __ballot_sync(0xffffffffu, live && !empty_row && (check != 0.f || (shift < FLT_MAX && !(l >= 64.f))));
             if (bad && a.n_split > 1) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // (their records are there and may be replaced)
             __syncwarp();
             while (bad) {

@@ -173,3 +173,36 @@ def check_best_row(cl, kind, n, size):
 def test_queries_next_to_the_largest_f32(on, n, size):
     """Scores that f32 can still hold are computed without a step that it cannot."""
     check_best_row(on[1], on[0], n, size)
+
+
+@pytest.mark.parametrize("n", [1, 5, 150])
+@pytest.mark.parametrize("size", [1e6, 1e7, 1e8, 1e9, 3e9, 1e10, 1e11, 1e20, 1e30, 1e36])
+def test_huge_queries_find_the_best_row(on, n, size):
+    """Scores whose rounding in f32 is larger than the steps of an exponential: the largest one still weighs something."""
+    check_best_row(on[1], on[0], n, size)
+
+
+@pytest.mark.parametrize("n", [1, 40, 150])
+def test_large_scores_of_full_queries(on, n):
+    """The same with queries that are not one-hot, at magnitudes where scores pass 2^23 units: every row is a mean of values, never zero or NaN, and
+    where the largest score leads by more than all roundings together it is that row's value."""
+    kind, cl = on
+    heads, kv, hd, start = 2, 1, 128, 300
+    total = start + n
+    for seed, size in enumerate((1e5, 1e7, 1e8, 1e9, 1e11)):
+        g = T.gen(30 + seed)
+        q, k, v = T.normal(g, n, heads * hd, scale=size), T.normal(g, kv, total, hd), T.normal(g, kv, total, hd)
+        out, k, v = T.attend(cl, q, k, v, heads, kv, hd, start, 200, 3, kind, total + 3)
+        sees = T.visible(start, n, 200, 3, total)
+        assert torch.isfinite(out).all() and (out.view(n, heads, hd) != 0).any(-1).all()
+        for h in range(heads):
+            qq = q[:, h * hd:(h + 1) * hd].double()
+            s = (qq @ k[0].double().T / hd ** 0.5).masked_fill(~sees, -float("inf"))
+            size_of = torch.where(sees, qq.abs() @ k[0].double().abs().T / hd ** 0.5, 0.0).amax(-1)
+            two = s.topk(2, -1)
+            # scores off by 2^-11 (f16 queries) and (hd + 8) 2^-24 of their terms each; a lead of 20 beyond that leaves 1e-8 of the weight to the others
+            sure = two.values[:, 0] - two.values[:, 1] > 2 * (2.0 ** -11 + (hd + 8) * 2.0 ** -24) * size_of + 20
+            want = v[0].double()[two.indices[:, 0]]
+            off = (out.view(n, heads, hd)[:, h].double() - want).abs()
+            tol = torch.finfo(out.dtype).eps / 2 * want.abs() + (2.0 ** -11 * (kind != "f32") + 16 * 2.0 ** -24 + 1e-6) * (want.abs() + 10) + 2.0 ** -25
+            assert sure.any() and (off <= tol)[sure].all()
