@@ -231,6 +231,7 @@ template <int KIND, int HD> struct Layout {
     // softmax warps, whose sum with what is left is what was launched: 128 * 152 + 128 * 104 = 256 * 128 (f16), 256 * 120 + 384 * 80 = 640 * 96.
     static constexpr int LAUNCH_REGS = KIND == CACHE_Q4 ? 96 : 128, SOFTMAX_REGS = KIND == CACHE_Q4 ? 120 : 152, OTHER_REGS = KIND == CACHE_Q4 ? 80 : 104;
     static_assert(SOFTMAX_WARPS * SOFTMAX_REGS + (THREADS / 32 - SOFTMAX_WARPS) * OTHER_REGS <= THREADS / 32 * LAUNCH_REGS, "the shares fit in the launch's registers");
+    static_assert(MMA_WARP % 4 == 0 && THREADS % 128 == 0, "whole warpgroups give registers away, and whole ones take them");
     static_assert((2 / TILES) * THREADS * LAUNCH_REGS <= 65536, "the CTAs of an SM fit in its registers");
 };
 
@@ -358,9 +359,11 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     tc_after();
     const uint32_t tmem = tmem_slot;
 
+    // (one instruction for all warps of a warpgroup, whatever their roles)
+    if (warp >= Y::MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Y::SOFTMAX_REGS));
     if (warp >= Y::LOAD_WARP) {
         // ------------------------------- K and V steps into the ring -------------------------------------------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
         if constexpr (KIND == CACHE_F16) {
             if (warp == Y::LOAD_WARP && lane == 0) {
                 int x = min(items, STAGES);   // (the first are on their way)
@@ -450,7 +453,6 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         }
     } else if (warp >= Y::MMA_WARP) {
         // ------------------------------- MMA issuers -----------------------------------------------------------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
         // A warp for a tile's scores and one for its output products: a wait, a commit or the issue of eight MMAs costs 100 to 300 cycles each, and
         // one warp with all of a step's was busy for 1800 cycles, about as long as the softmax (512-row 4-bit chunk 153 us, with two warps 149; 8192-row prompt 278 and
         // 274).
@@ -516,7 +518,6 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         mbar_drain(&drained[warp - Y::MMA_WARP], 0);
     } else {
         // ------------------------------- softmax: a thread owns a row ------------------------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Y::SOFTMAX_REGS));
         const int tile = warp >> 2, r = threadIdx.x & (QT - 1);   // the thread's tile and row
         const int row = min(row0 + tile * QT + r, row_last);
         const float c2 = c2_s[tile * QT + r];
