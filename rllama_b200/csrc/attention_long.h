@@ -93,6 +93,15 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
     for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(bar, parity); i++) {}
 }
+// |x| into a running maximum; a NaN stays.
+__device__ __forceinline__ void max_abs_nan(float& top, float x) { asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x))); }
+// Whether a row of sum l, unnormalised results up to o_top in magnitude and maximum m has to be computed again from what it sees alone: a NaN that the
+// sum does not have may come from a position that the row does not see, times weight zero. Anything else that is not finite comes from what it sees, and is
+// the result, unless the scores are so large (beyond 2^20) that a weight may have left the range of f16 or f32. (|m| = FLT_MAX: no score counted yet.)
+__device__ __forceinline__ bool row_is_suspect(float l, float o_top, float m) {
+    if (fabsf(m) > 0x1p20f && fabsf(m) < FLT_MAX) return !(l <= FLT_MAX && o_top <= FLT_MAX);
+    return l == l && o_top != o_top;
+}
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -4,7 +4,7 @@
 // then 4 x HD / 16 columns of the result, from operands that lie in shared memory in rows padded by 16 bytes (8 and 12 vector loads for 64 and
 // 128 FMAs). The weights take the place of the K tile. Two CTAs share an SM: one's loads fall into the other's arithmetic.
 // 400 rows after 8000 positions, 40 heads: 1.97 ms, 34 TFLOP/s (of about 75 that the FMA pipes have).
-// A zero weight times an infinite or NaN value is a NaN here too; such rows are computed again, one warp to a row.
+// A zero weight times an infinite or NaN value is a NaN here too; rows with a NaN that their sum does not have are computed again, one warp to a row.
 #include <algorithm>
 
 #include "attention_long.h"
@@ -149,19 +149,20 @@ __global__ void __launch_bounds__(kThreads, 2) attn_long_f32_kernel(const __grid
         const float inv = a.n_split > 1 ? 1.f : sees ? 1.0f / sum : 0.f;
         const int64_t rec = ((int64_t)ii * a.heads + head) * a.n_split + blockIdx.y;
         float* dst = a.n_split > 1 ? a.rec_o + rec * HD : reinterpret_cast<float*>(a.out) + ii * a.out_ld + head * HD;
-        float check = fmaf(sum, 0.f, inv * 0.f);   // a NaN once anything is not finite
+        float o_top = 0.f;
 #pragma unroll
         for (int g = 0; g < NC; g++) {
             float4 x;
             x.x = o[i][g][0] * inv; x.y = o[i][g][1] * inv; x.z = o[i][g][2] * inv; x.w = o[i][g][3] * inv;
-            check = fmaf(x.x, 0.f, fmaf(x.y, 0.f, fmaf(x.z, 0.f, fmaf(x.w, 0.f, check))));
+#pragma unroll
+            for (int e = 0; e < 4; e++) max_abs_nan(o_top, o[i][g][e]);
             *reinterpret_cast<float4*>(dst + g * 64 + tx * 4) = a.n_split > 1 || sees ? x : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         if (a.n_split > 1 && tx == 0) a.rec_ml[rec] = make_float2(m[i], sum);
-        if (sees && check != 0.f) atomicOr(&bad[y >> 5], 1u << (y & 31));
+        if (sees && row_is_suspect(sum, o_top, 0.f)) atomicOr(&bad[y >> 5], 1u << (y & 31));
     }
     __syncthreads();
-    // rows next to infinite or NaN cache contents, again from what they see alone, a warp to a row
+    // rows next to infinite or NaN cache contents that they do not see, again from what they see alone, a warp to a row
     constexpr int N = HD / 32;
     const int lane = tid & 31, warp = tid >> 5;
     for (int y = warp; y < QT; y += kThreads / 32) {

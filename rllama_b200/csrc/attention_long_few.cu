@@ -13,8 +13,8 @@
 //    values, its columns the positions; pairs of positions are interleaved with one byte permutation a register.
 // The positions of a tile are dealt to the 2 x 8 columns of S so that a thread's four scores belong to positions c, 4 + c, 8 + c, 12 + c: the
 // rows of V that the four threads of a column read side by side are then neighbours in shared memory.
-// The running maximum m moves only when a score exceeds it by 2^8, as in attention_long_tc.cu, and a row whose result is not
-// finite is computed again from what it sees alone. Scores, maxima, sums and O are f32; rounded to f16: the weights
+// The running maximum m moves only when a score exceeds it by 2^8, as in attention_long_tc.cu, and a row whose result is a NaN
+// although its sum is not is computed again from what it sees alone. Scores, maxima, sums and O are f32; rounded to f16: the weights
 // (2^-11) and the result.
 //
 // Measured: 65536 4-bit positions, 32 heads, one token, 94 us, 3.2 TB/s: 446 instructions for 16 positions of a head (185 of them integer and
@@ -385,7 +385,8 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
                 }
             }
             float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            if (__any_sync(0xffffffffu, top > m + kLag)) {
+            // (no weight reaches 2^16, where f16 ends, whatever the rounding of m + kLag and kShift - m)
+            if (__any_sync(0xffffffffu, top >= m + kLag)) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float m_new = fmaxf(m, top), scale = ex2_approx(m - m_new);
@@ -458,15 +459,16 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
     const bool live = joins && jr < rows;
     if (live) join(kWarps, jr);
     M -= kShift;
-    float check = L * 0.f;   // a NaN once anything is not finite
+    float check = 0.f;   // a NaN once one of them is
 #pragma unroll
-    for (int e = 0; e < PER; e++) check = fmaf(O[e], 0.f, check);
+    for (int e = 0; e < PER; e++) check += fabsf(O[e]);
     const int jrow = row0 + min(jr, rows - 1), ji = jrow / a.group, jh = kvh * a.group + jrow % a.group;
     const bool sees = visible_run(a, a.start + ji, a.start + ji).len > 0;
-    // (a row that sees something has a sum above zero somewhere, but perhaps not in this share)
-    if (live && (check != 0.f || (a.n_split == 1 && sees && L == 0.f))) atomicOr(&bad, 1u << jr);
+    // A NaN that the sum has too comes from a score that the row sees, and an infinity from a value that it sees: those are the result. Any other may come
+    // from a position that it does not see, times weight zero. (A row that sees something has a sum above zero somewhere, but perhaps not in this share.)
+    if (live && ((check != check && L == L) || (a.n_split == 1 && sees && L == 0.f))) atomicOr(&bad, 1u << jr);
     __syncthreads();
-    for (uint32_t todo = bad; todo; todo &= todo - 1) {   // uniform: rows next to infinite or NaN cache contents, one by one
+    for (uint32_t todo = bad; todo; todo &= todo - 1) {   // uniform: rows next to infinite or NaN cache contents that they do not see, one by one
         const int y = __ffs(todo) - 1, again = row0 + y, i = again / a.group, head = kvh * a.group + again % a.group, pp = a.start + i;
         constexpr int N = HD / 32;
         const float k2 = rsqrtf((float)HD) * 1.4426950408889634f;

@@ -29,8 +29,8 @@
 // [2^8, 2^9) whatever the row's magnitude (an error of at most 2^-11 sum |q k| / sqrt(head_dim) in a score), and the
 // weights (2^-11 each). Scores, maxima, sums and O are f32.
 //
-// A zero weight times an infinite or NaN value is a NaN in an MMA, so a row whose result is not finite is computed again,
-// one warp to a row, from the positions that it sees alone. Only rows next to such cache contents pay for it.
+// A zero weight times an infinite or NaN value is a NaN in an MMA, so a row whose result is a NaN although its sum is not is computed
+// again, one warp to a row, from the positions that it sees alone. Only rows next to such cache contents pay for it.
 //
 // Every wait is bounded; when one runs out the kernel raises the context's error word, no later wait of the CTA blocks, and
 // the tensor memory is released before the CTA returns.
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             unsigned char *turn = q_s + tile * Y::Q_ROOM + (warp & 3) * (32 * Y::OUT_ROW), *mine = turn + lane * Y::OUT_ROW;
             const bool empty_row = p + 1 - low + min(a.sinks, low) == 0;
             const float inv = empty_row ? 0.f : 1.0f / l;
-            float check = fmaf(l, 0.f, a.n_split == 1 ? inv * 0.f : 0.f);   // a NaN once anything is not finite
+            float o_top = 0.f;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 float x[32];
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                     for (int e = 0; e < 32; e++) x[e] = 0.f;
                 }
 #pragma unroll
-                for (int e = 0; e < 32; e++) check = fmaf(x[e], 0.f, check);
+                for (int e = 0; e < 32; e++) max_abs_nan(o_top, x[e]);
                 if (a.n_split > 1) {   // half a record at a time
                     unsigned char* dst = mine + c % (HD / 2) * 4;
 #pragma unroll
@@ -665,11 +665,11 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                 }
             }
             if (live && a.n_split > 1) a.rec_ml[rec] = make_float2(-shift, l);
-            // Rows next to infinite or NaN cache contents, again and one by one. So are those whose largest weight, 2^kShift when it was taken, has come out
+            // Rows next to infinite or NaN cache contents that they do not see, again and one by one. So are those whose largest weight, 2^kShift when it was taken, has come out
             // as less than half of that or too large for f16: top is rounded before it is subtracted, the scores are not, and for scores beyond 2^23 the
             // difference is no longer small against 1.
             __syncwarp();
-            uint32_t bad = __ballot_sync(0xffffffffu, live && !empty_row && (check != 0.f || (shift < FLT_MAX && !(l >= 64.f))));
+            uint32_t bad = __ballot_sync(0xffffffffu, live && !empty_row && (row_is_suspect(l, o_top, shift) || (shift < FLT_MAX && l < 64.f)));
             if (bad && a.n_split > 1) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // (their records are there and may be replaced)
             __syncwarp();
             while (bad) {

@@ -206,3 +206,51 @@ def test_large_scores_of_full_queries(on, n):
             off = (out.view(n, heads, hd)[:, h].double() - want).abs()
             tol = torch.finfo(out.dtype).eps / 2 * want.abs() + (2.0 ** -11 * (kind != "f32") + 16 * 2.0 ** -24 + 1e-6) * (want.abs() + 10) + 2.0 ** -25
             assert sure.any() and (off <= tol)[sure].all()
+
+
+def milliseconds(call):
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    times = []
+    for _ in range(4):
+        start.record()
+        call()
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    return min(times[1:])
+
+
+@pytest.mark.parametrize("kind,kernel", [("f32", "tiles"), ("f16", "few"), ("f16", "tiles"), ("q4", "few"), ("q4", "tiles")])
+def test_rows_that_see_a_bad_position_cost_no_more(kind, kernel):
+    """A row's result is not a number because of what it sees: nothing is to be gained from another pass over its positions. (Such passes made 128 rows
+    after 4000 positions a hundred times slower.)"""
+    from rllama_b200 import Cache4
+    heads, hd, n, start = 8, 128, 128, 4000
+    total, dt = start + n, torch.float32 if kind == "f32" else torch.float16
+    g = T.gen(21)
+    q, k, v = T.normal(g, n, heads * hd), T.normal(g, total, heads * hd), T.normal(g, total, heads * hd)
+    out = torch.empty(n, heads * hd, dtype=dt, device=T.DEV)
+    with context(kernel, "1") as cl:
+        if kind == "q4":
+            parts = T.empty_cache4(heads, total, hd)
+            cache = Cache4.wrap(cl, *parts, heads, total, hd)
+            cache.append(cl.wrap(k), cl.wrap(v), 0)
+            places = [parts[1].view(heads, total, -1)[:, 100, 2]]       # K's scales; a V group cannot hold an infinity
+            call = lambda: cache.attention(cl.wrap(out), cl.wrap(q), heads, start)
+        else:
+            kc, vc = (x.view(total, heads, hd).transpose(0, 1).reshape(heads * total, hd).to(dt) for x in (k, v))
+            places = [x.view(heads, total, hd)[:, 100, 3] for x in (kc, vc)]
+            call = lambda: cl.wrap(out).attention_window(cl.wrap(q), cl.wrap(kc), cl.wrap(vc), heads, heads, total, start, total)
+        clean = milliseconds(call)
+        for which, place in enumerate(places):
+            before = place.clone()
+            place.fill_(float("inf") if which else float("nan"))
+            bad = milliseconds(call)
+            o = out.view(n, heads, hd)
+            assert bool((o[..., 3] == float("inf")).all()) if which else o.isnan().all()
+            assert which == 0 or torch.isfinite(o[..., 4:]).all()
+            assert bad < 4 * clean + 0.05, (clean, bad)
+            place.copy_(before)
+        q[:, 5] = float("nan")   # head 0 of every row
+        bad = milliseconds(call)
+        assert out.view(n, heads, hd)[:, 0].isnan().all() and torch.isfinite(out.view(n, heads, hd)[:, 1:]).all() and bad < 4 * clean + 0.05, (clean, bad)
