@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) attn_long_merge_kernel(const __grid_const
             for (int e = 0; e < N; e += 2) *reinterpret_cast<float2*>(out + lane * N + e) = make_float2(o[e], o[e + 1]);
         } else {
 #pragma unroll
-            for (int e = 0; e < N; e += 2) *reinterpret_cast<__half2*>(out + lane * N + e) = __floats2half2_rn(o[e], o[e + 1]);
+            for (int e = 0; e < N; e += 2) *reinterpret_cast<__half2*>(out + lane * N + e) = mean_f16(o[e], o[e + 1]);
         }
         return;
     }

@@ -54,7 +54,15 @@ template <int KIND, int HD> __device__ __forceinline__ void load_row(const void*
 }
 
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+// A mean of f16 values as f16. Weights that were rounded up may put a mean of values next to the largest f16 beyond it (up to 65504 (1 + 2^-11)), and only
+// an infinity that the row sees may make one.
+constexpr float kMaxF16 = 65504.f, kInfF16 = 65520.f;   // (from there on a rounded f16 is infinite)
+__device__ __forceinline__ float within_f16(float v) { return fabsf(v) <= FLT_MAX ? fminf(fmaxf(v, -kMaxF16), kMaxF16) : v; }
+__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(within_f16(v)); }
+__device__ __forceinline__ __half2 mean_f16(float x, float y) {
+    if (fmaxf(fabsf(x), fabsf(y)) >= kInfF16) { x = within_f16(x); y = within_f16(y); }
+    return __floats2half2_rn(x, y);
+}
 
 constexpr uint32_t kWaitLimit = 1u << 22;
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

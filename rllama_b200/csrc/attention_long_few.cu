@@ -539,7 +539,11 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
     const float inv = sees ? 1.0f / L : 0.f;
     __half* dst = reinterpret_cast<__half*>(a.out) + ji * a.out_ld + (int64_t)jh * HD + jc;
 #pragma unroll
-    for (int e = 0; e < PER; e += 2) *reinterpret_cast<__half2*>(dst + e) = sees ? __floats2half2_rn(O[e] * inv, O[e + 1] * inv) : __half2half2(__ushort_as_half(0));
+    for (int e = 0; e < PER; e += 2) {
+        const float x = O[e] * inv, y = O[e + 1] * inv;
+        // (4-bit values end at 65408: no rounding puts their mean beyond f16)
+        *reinterpret_cast<__half2*>(dst + e) = !sees ? __half2half2(__ushort_as_half(0)) : KIND == CACHE_F16 ? mean_f16(x, y) : __floats2half2_rn(x, y);
+    }
 }
 
 template <int KIND, int HD>

@@ -667,9 +667,10 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             if (live && a.n_split > 1) a.rec_ml[rec] = make_float2(-shift, l);
             // Rows next to infinite or NaN cache contents that they do not see, again and one by one. So are those whose largest weight, 2^kShift when it was taken, has come out
             // as less than half of that or too large for f16: top is rounded before it is subtracted, the scores are not, and for scores beyond 2^23 the
-            // difference is no longer small against 1.
+            // difference is no longer small against 1. And rows that rounded weights have put beyond f16's largest value (see mean_f16).
+            const bool beyond = a.n_split == 1 && o_top * inv >= kInfF16 && o_top <= FLT_MAX;
             __syncwarp();
-            uint32_t bad = __ballot_sync(0xffffffffu, live && !empty_row && (row_is_suspect(l, o_top, shift) || (shift < FLT_MAX && l < 64.f)));
+            uint32_t bad = __ballot_sync(0xffffffffu, live && !empty_row && (row_is_suspect(l, o_top, shift) || (shift < FLT_MAX && l < 64.f) || beyond));
             if (bad && a.n_split > 1) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // (their records are there and may be replaced)
             __syncwarp();
             while (bad) {

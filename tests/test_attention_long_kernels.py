@@ -254,3 +254,19 @@ def test_rows_that_see_a_bad_position_cost_no_more(kind, kernel):
         q[:, 5] = float("nan")   # head 0 of every row
         bad = milliseconds(call)
         assert out.view(n, heads, hd)[:, 0].isnan().all() and torch.isfinite(out.view(n, heads, hd)[:, 1:]).all() and bad < 4 * clean + 0.05, (clean, bad)
+
+
+@pytest.mark.parametrize("on", [x for x in KERNELS if x[0] != "f32"], ids="-".join, indirect=True)
+@pytest.mark.parametrize("n", [1, 9, 300])
+def test_values_next_to_the_largest_f16(on, n):
+    """A mean of values is never beyond the largest of them: weights that were rounded up do not make an infinity of 65504 (4 bits: 65408)."""
+    kind, cl = on
+    heads, kv, hd, start = 8, 2, 128, 500
+    total = start + n
+    for seed in range(4):
+        g = T.gen(40 + seed)
+        q, k = T.normal(g, n, heads * hd, scale=1.0 + seed), T.normal(g, kv, total, hd)
+        v = (65504.0 * torch.where(torch.arange(hd, device=T.DEV) % 3 == 0, -1.0, 1.0)).expand(kv, total, hd)
+        out, k, v = T.attend(cl, q, k, v, heads, kv, hd, start, 300, 2, kind, total + 3)
+        want = v[0, 0].repeat(heads).double()
+        assert ((out.double() - want).abs() <= 2 * 2.0 ** -11 * want.abs()).all() and (out.double().abs() <= 65504).all()
