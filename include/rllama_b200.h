@@ -205,7 +205,8 @@ int rlb_cache4_free(rlb_cache4* c);
  * start_pos .. start_pos+n-1.                                                                 */
 int rlb_cache4_append(rlb_cache4* c, const rlb_tensor* k, const rlb_tensor* v, int32_t start_pos);
 /* rlb_norm_rope_append into a 4-bit cache: q to q_out (may be q itself), k normalised and rotated
- * and v as it is to positions start_pos .. start_pos+n-1, all rows f32; the same arguments.  */
+ * and v as it is to positions start_pos .. start_pos+n-1, all rows f32; the same arguments and
+ * the same bits as that op into an f32 cache and an append of its rows.                       */
 int rlb_cache4_norm_rope_append(rlb_cache4* c, rlb_tensor* q_out, const rlb_tensor* q, const rlb_tensor* k, const rlb_tensor* v,
                                 const rlb_tensor* q_gain, const rlb_tensor* k_gain, float eps, const rlb_tensor* rope, int32_t heads,
                                 int32_t start_pos);

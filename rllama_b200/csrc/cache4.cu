@@ -62,13 +62,20 @@ template <> struct Words<2> { typedef uint2 T; typedef uint32_t D; };
 // Normalises (with a gain) and rotates a thread's values of a head's row, which are whole pairs; eight neighbouring threads have the row.
 template <int G> __device__ __forceinline__ void norm_rope(float (&y)[G][8], const float* gain, float eps, const float* turn) {
     if (gain) {
-        float part[G], ss = 0.f;
+        // (the additions in the order of rotate.cu: runs of 2 G values, their neighbours in the group of eight, the other group, the row's other threads)
+        constexpr int RUN = 2 * G, RUNS = 8 / RUN;
+        float ss = 0.f;
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            part[g] = 0.f;
+            float part[RUNS];
 #pragma unroll
-            for (int e = 0; e < 8; e++) part[g] = fmaf(y[g][e], y[g][e], part[g]);
-            ss += part[g];
+            for (int r = 0; r < RUNS; r++) {
+                part[r] = 0.f;
+#pragma unroll
+                for (int e = 0; e < RUN; e++) part[r] = fmaf(y[g][r * RUN + e], y[g][r * RUN + e], part[r]);
+            }
+            const float sum = RUNS == 2 ? part[0] + part[1] : (part[0] + part[1]) + (part[RUNS - 2] + part[RUNS - 1]);
+            ss = g == 0 ? sum : ss + sum;
         }
         ss += __shfl_xor_sync(0xffffffffu, ss, 1);
         ss += __shfl_xor_sync(0xffffffffu, ss, 2);

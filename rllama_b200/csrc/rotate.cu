@@ -76,7 +76,9 @@ __global__ void __launch_bounds__(256) norm_rope_append_kernel(const __grid_cons
         }
         if (kind != 2) {
             if (gain) {
-                // The rows' sums of squares, four at a time: lanes hand on half of the rows that they hold until they hold one, eight lanes a row.
+                // The rows' sums of squares, four at a time: lanes hand on half of the rows that they hold until they hold one, eight lanes a row. The order of the
+                // additions (values 4 apart, with head_dim 128 then 32, or else 2 and 4; then 8, 16 and the row's halves) is that of cache4.cu, whose
+                // rotation has the same bits.
                 float ss[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
@@ -84,16 +86,18 @@ __global__ void __launch_bounds__(256) norm_rope_append_kernel(const __grid_cons
 #pragma unroll
                     for (int e = 0; e < N; e++) ss[u] = fmaf(x[u][e], x[u][e], ss[u]);
                 }
-                const bool up = lane & 16, odd = lane & 8;
-                float s0 = (up ? ss[2] : ss[0]) + __shfl_xor_sync(0xffffffffu, up ? ss[0] : ss[2], 16);
-                float s1 = (up ? ss[3] : ss[1]) + __shfl_xor_sync(0xffffffffu, up ? ss[1] : ss[3], 16);
-                s0 = (odd ? s1 : s0) + __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 8);
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-                const float s = rsqrtf(s0 / (float)HD + a.eps);
+                constexpr int SECOND = N == 4 ? 8 : 2;
+                const bool up = lane & 1, odd = lane & SECOND;
+                float s0 = (up ? ss[2] : ss[0]) + __shfl_xor_sync(0xffffffffu, up ? ss[0] : ss[2], 1);
+                float s1 = (up ? ss[3] : ss[1]) + __shfl_xor_sync(0xffffffffu, up ? ss[1] : ss[3], 1);
+                s0 = (odd ? s1 : s0) + __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, SECOND);
+                s0 += __shfl_xor_sync(0xffffffffu, s0, N == 4 ? 2 : 4);
+                s0 += __shfl_xor_sync(0xffffffffu, s0, N == 4 ? 4 : 8);
+                s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
+                const float s = 1.0f / sqrtf(s0 / (float)HD + a.eps);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const float su = __shfl_sync(0xffffffffu, s, 8 * u);
+                    const float su = __shfl_sync(0xffffffffu, s, (u >> 1) + (u & 1) * SECOND);
 #pragma unroll
                     for (int e = 0; e < N; e++) x[u][e] = x[u][e] * su * g[e];
                 }
