@@ -106,7 +106,9 @@ template <typename T, int HD, bool ROTATE>
 __global__ void __launch_bounds__(kThreads) append4_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int ALL = HD / kQ4Group, G = ALL / 2;   // groups of a row, of a thread
     const int x = blockIdx.x * kThreads + threadIdx.x, which = blockIdx.z, block = x & 3, half = x >> 2 & 1;
-    const bool live = x < (which == 2 ? a.heads : a.kv_heads) * 8;   // (a row's four threads are all live or none is)
+    const int threads = (which == 2 ? a.heads : a.kv_heads) * 8;
+    if (ROTATE && blockIdx.x * kThreads >= threads) return;   // (the grid is as wide as the most heads need: 64 heads on 8 49 us with these CTAs, 31 without)
+    const bool live = x < threads;   // (a row's eight threads are all live or none is)
     const int head = live ? x >> 3 : 0;
     const T* src = reinterpret_cast<const T*>(a.src[which]) + head * HD + half * (HD / 2) + block * 8;
     for (int i = blockIdx.y; i < a.n; i += gridDim.y) {

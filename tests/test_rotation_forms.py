@@ -32,3 +32,29 @@ def test_both_rotations_agree_bit_for_bit(n, heads, kv, start, pad, hd):
         W(a).norm_rope_append(W(half[0]), W(half[1]), W(q), W(k), W(v), table, heads, kv, max_seq, start, *map(W, gains), 1e-5)
         assert torch.equal(half[m], c.half())
     cl.flush()
+
+
+@pytest.mark.gpu
+def test_shared_heads_cost_what_their_bytes_do():
+    """64 query heads on 8 K/V heads move 0.53 of the bytes of 64 on 64 (the K/V planes of the grid once worked on as many heads as q's)."""
+    from rllama_b200 import Cuda
+    cl = Cuda(stream=torch.cuda.current_stream().cuda_stream)
+    n, heads, hd, max_seq, W = 1792, 64, 128, 2048, cl.wrap
+    table, gain, us = cl.rope_table(max_seq, hd), torch.ones(1, hd, device=T.DEV), {}
+    for kv in (64, 8):
+        sets = []
+        for _ in range(4):   # more than the L2 cache holds
+            q, k, v = (torch.ones(n, h * hd, device=T.DEV) for h in (heads, kv, kv))
+            sets.append([W(x) for x in (torch.empty_like(q), q, k, v)] + [T.empty_like_cache(cl, kv, max_seq, hd)[1]])
+        best = []
+        for _ in range(6):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            for i in range(20):
+                q_out, q, k, v, cache = sets[i % 4]
+                cache.norm_rope_append(q_out, q, k, v, table, heads, 0, W(gain), W(gain))
+            end.record()
+            torch.cuda.synchronize()
+            best.append(start.elapsed_time(end))
+        us[kv] = min(best[1:]) * 50
+    assert us[8] < 0.72 * us[64], us
