@@ -18,6 +18,25 @@ def capacity_cols(cols, dtype):
     return (int(cols) + m - 1) // m * m
 
 
+_MOST = 2 ** 31 - 1
+
+
+def _i32(args):
+    """The library takes 32-bit numbers, and ctypes would cut off the rest. ``args``: the bits of all of them, or-ed (of numbers that fit the sign is all
+    that lies beyond 31 bits, and a negative one among others is refused by the library)."""
+    if args >> 31 not in (0, -1):
+        raise OverflowError("an argument does not fit in 32 bits")
+
+
+def _given(tensor):
+    """The handle of an optional argument."""
+    if tensor is None:
+        return None
+    if not tensor._h:
+        raise ValueError("the tensor has been freed")
+    return tensor._h
+
+
 class Cuda:
     """Counterpart of ``OpenCL`` (``OpenCL::new(verbose, nth_device)``). ``stream``: a CUDA stream handle (an integer, e.g.
     ``torch.cuda.current_stream().cuda_stream``; 0 is the legacy default stream, the per-thread one is refused) that the ops are queued
@@ -85,6 +104,7 @@ class Cuda:
 
     def rope_table(self, max_seq_len, head_dim):
         """The rotation's (cos, sin) pairs, one row a position (``compute_freqs_cis``)."""
+        _i32(int(max_seq_len) | int(head_dim))
         t = CudaTensor(self, max_seq_len, head_dim, head_dim, F32)
         check(_ffi.lib().rlb_rope_table(self._h, int(max_seq_len), int(head_dim), ctypes.byref(t._h)))
         return t
@@ -140,12 +160,15 @@ class CudaTensor:
     def norm_rope_append(self, kcache, vcache, q, k, v, rope, heads, kv_heads, max_seq_len, start_pos, q_gain=None, k_gain=None, eps=1e-6):
         """self <- the rows of q, their heads normalised (with a gain) and rotated; k likewise and v as it is go to positions
         start_pos, start_pos + 1, ... of the caches."""
-        check(_ffi.lib().rlb_norm_rope_append(self._h, kcache._h, vcache._h, q._h, k._h, v._h, q_gain._h if q_gain is not None else None,
-                                              k_gain._h if k_gain is not None else None, eps, rope._h, heads, kv_heads, max_seq_len, start_pos))
+        _i32(heads | kv_heads | max_seq_len | start_pos)
+        check(_ffi.lib().rlb_norm_rope_append(self._h, kcache._h, vcache._h, q._h, k._h, v._h, _given(q_gain), _given(k_gain), eps, rope._h,
+                                              heads, kv_heads, max_seq_len, start_pos))
 
     def attention_window(self, q, kcache, vcache, heads, kv_heads, max_seq_len, start_pos, window, sinks=0):
         """self <- attention of the rows of q (row i at position p = start_pos + i) over the positions t <= p with
         t > p - window or t < sinks; heads / kv_heads query heads share a K/V head."""
+        window, sinks = min(window, _MOST), min(sinks, _MOST)
+        _i32(heads | kv_heads | max_seq_len | start_pos | window | sinks)
         check(_ffi.lib().rlb_attention_window(self._h, q._h, kcache._h, vcache._h, heads, kv_heads, max_seq_len, start_pos, window, sinks))
 
     def free(self):
@@ -169,6 +192,7 @@ class Cache4:
     def __init__(self, cl, kv_heads, max_seq_len, head_dim, _arrays=None):
         self.cl, self.kv_heads, self.max_seq_len, self.head_dim = cl, int(kv_heads), int(max_seq_len), int(head_dim)
         self._h = ctypes.c_void_p()
+        _i32(self.kv_heads | self.max_seq_len | self.head_dim)
         self._keep = _arrays
         if _arrays is None:
             check(_ffi.lib().rlb_cache4_create(cl._h, self.kv_heads, self.max_seq_len, self.head_dim, ctypes.byref(self._h)))
@@ -187,20 +211,24 @@ class Cache4:
 
     def append(self, k, v, start_pos):
         """Rows of rotated k and v (both f32 or both f16) to positions start_pos, start_pos + 1, ..."""
+        _i32(start_pos)
         check(_ffi.lib().rlb_cache4_append(self._h, k._h, v._h, start_pos))
 
     def norm_rope_append(self, q_out, q, k, v, rope, heads, start_pos, q_gain=None, k_gain=None, eps=1e-6):
         """``CudaTensor.norm_rope_append`` into this cache: q_out <- the rows of q, k and v to positions start_pos, start_pos + 1, ..."""
-        check(_ffi.lib().rlb_cache4_norm_rope_append(self._h, q_out._h, q._h, k._h, v._h, q_gain._h if q_gain is not None else None,
-                                                     k_gain._h if k_gain is not None else None, eps, rope._h, heads, start_pos))
+        _i32(heads | start_pos)
+        check(_ffi.lib().rlb_cache4_norm_rope_append(self._h, q_out._h, q._h, k._h, v._h, _given(q_gain), _given(k_gain), eps, rope._h, heads, start_pos))
 
     def read(self, k_out, v_out, start_pos):
         """The values held, into f16 or f32 rows; either may be None."""
-        check(_ffi.lib().rlb_cache4_read(self._h, k_out._h if k_out is not None else None, v_out._h if v_out is not None else None, start_pos))
+        _i32(start_pos)
+        check(_ffi.lib().rlb_cache4_read(self._h, _given(k_out), _given(v_out), start_pos))
 
     def attention(self, out, q, heads, start_pos, window=None, sinks=0):
         """out (f16) <- ``attention_window`` of the rows of q over the values held; no window by default."""
-        check(_ffi.lib().rlb_cache4_attention(self._h, out._h, q._h, heads, start_pos, self.max_seq_len if window is None else window, sinks))
+        window, sinks = _MOST if window is None else min(window, _MOST), min(sinks, _MOST)
+        _i32(heads | start_pos | window | sinks)
+        check(_ffi.lib().rlb_cache4_attention(self._h, out._h, q._h, heads, start_pos, window, sinks))
 
     def free(self):
         if self._h:
