@@ -153,7 +153,8 @@ int rlb_attention_decode_static(rlb_tensor* out, const rlb_tensor* q, const rlb_
  * Tier 1, long contexts: what lies between the q/k/v projection and wo, for caches in f16, f32
  * or 4 bits, a sliding window with first tokens that stay visible, and K/V heads shared by
  * heads / kv_heads query heads each (query head h reads K/V head h / (heads / kv_heads)).
- * head_dim is 64 or 128; caches have up to 2^30 positions (RLB_ERR_LIMIT). Rows may be padded
+ * head_dim is 64 or 128; caches have up to 2^30 positions and rows fewer than 2^31 columns
+ * (RLB_ERR_LIMIT); 4-bit caches have up to 65536 heads. Rows may be padded
  * (capacity_cols), caches may not. A call with no rows does nothing. What a call writes overlaps
  * none of its other arguments, unless said otherwise. On a context of the caller's stream these
  * ops may be captured into a CUDA graph (meanwhile RLB_ERR_STATE refuses what allocates or waits:

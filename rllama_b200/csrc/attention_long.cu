@@ -177,6 +177,7 @@ int check(const char* who, const rlb_tensor* out, const rlb_tensor* q, rlb_dtype
     if (max_seq > kMaxPositions) return rlb_fail(RLB_ERR_LIMIT, "%s: max_seq_len %d is more than %d", who, max_seq, kMaxPositions);
     if (window < 0 || sinks < 0) return rlb_fail(RLB_ERR_INVALID, "%s: window %d and sinks %d must not be negative", who, window, sinks);
     if (q->dtype != RLB_F32 || q->cols != heads * hd) return rlb_fail(RLB_ERR_INVALID, "%s: q must be n x heads*head_dim f32", who);
+    if (q->cols > kMaxColumns) return rlb_fail(RLB_ERR_LIMIT, "%s: rows of %lld columns are more than %lld", who, (long long)q->cols, (long long)kMaxColumns);
     if (out->dtype != out_dtype || out->rows != q->rows || out->cols != q->cols)
         return rlb_fail(RLB_ERR_INVALID, "%s: out must be n x heads*head_dim in %s", who, out_dtype == RLB_F16 ? "f16" : "f32");
     if (out->d == q->d && q->rows > 0) return rlb_fail(RLB_ERR_INVALID, "%s: out and q are one tensor", who);

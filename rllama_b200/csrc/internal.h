@@ -239,6 +239,7 @@ struct rlb_cache4 {
     void* owned = nullptr;                    // the allocation behind the four arrays, when the library made it
 };
 
+constexpr int64_t kMaxColumns = 0x7fffffff;   // of a row of heads: a head's first column is an int
 constexpr int kMaxPositions = 1 << 30;   // of a long-context cache: positions and the ends of tiles behind them are ints
 struct AttnLongArgs {
     const float* q = nullptr;                 // n rows of heads * hd f32, row stride q_ld

@@ -187,6 +187,8 @@ extern "C" int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_t
         return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: q and q_out must be n x heads*head_dim f32");
     if (k->dtype != RLB_F32 || k->rows != n || k->cols != kv_heads * hd || v->dtype != RLB_F32 || v->rows != n || v->cols != k->cols)
         return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: k and v must be n x kv_heads*head_dim f32");
+    if (std::max(q->cols, k->cols) > kMaxColumns)
+        return rlb_fail(RLB_ERR_LIMIT, "norm_rope_append: rows of %lld columns are more than %lld", (long long)std::max(q->cols, k->cols), (long long)kMaxColumns);
     if (rope->dtype != RLB_F32 || rope->cols != hd || rope->rows < start_pos + n)
         return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: the rope table must be f32, head_dim wide and cover position %lld", (long long)(start_pos + n - 1));
     if (!(eps >= 0.f)) return rlb_fail(RLB_ERR_INVALID, "norm_rope_append: eps must not be negative");

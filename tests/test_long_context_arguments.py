@@ -65,3 +65,25 @@ def test_results_with_a_window_or_first_tokens_beyond_32_bits(kind):
     for x in [b for b in BEYOND if b > 0]:
         T.check_attention(cl, 4, 2, 64, 3, 200, x, 0, kind)
         T.check_attention(cl, 4, 2, 64, 3, 200, 5, x, kind)
+
+
+@pytest.mark.gpu
+def test_rows_wider_than_31_bits_are_refused():
+    """Columns are counted in 32 bits inside the kernels. (Without rows no memory is needed: the widths are checked first.)"""
+    import test_attention_long as T
+    torch, cl = T.torch, Cuda(stream=T.torch.cuda.current_stream().cuda_stream)
+    W, heads = cl.wrap, 2 ** 25
+    for h, status in ((heads, 7), (heads - 1, 0)):
+        wide = [W(torch.empty(0, h * 64, dtype=dt, device=T.DEV)) for dt in (torch.float32, torch.float32, torch.float16)]
+        row = [W(torch.zeros(1, 64, device=T.DEV)) for _ in range(2)]
+        half = [W(torch.zeros(1, 64, dtype=torch.float16, device=T.DEV)) for _ in range(2)]
+        none, table = W(torch.empty(0, 64, device=T.DEV)), cl.rope_table(1, 64)
+        for call in (lambda: wide[0].attention_window(wide[1], *row, h, 1, 1, 0, 1), lambda: wide[2].attention_window(wide[0], *half, h, 1, 1, 0, 1),
+                     lambda: wide[0].norm_rope_append(*row, wide[1], none, none, table, h, 1, 1, 0),
+                     lambda: Cache4(cl, 1, 1, 64).attention(wide[2], wide[0], h, 0)):
+            if status:
+                with pytest.raises(RllamaError) as e:
+                    call()
+                assert e.value.status == status
+            else:
+                call()
