@@ -32,29 +32,11 @@ __global__ void __launch_bounds__(256) attn_long_row_kernel(const AttnLongArgs a
     const int chunk = (run.len + a.n_split - 1) / a.n_split;
     const int v0 = min(run.len, (int)blockIdx.y * chunk), v1 = min(run.len, v0 + chunk);
     const int64_t base = (int64_t)(head / a.group) * a.max_seq;
-    const float c2 = rsqrtf((float)HD) * 1.4426950408889634f;
-    float q[N], o[N] = {}, m = -FLT_MAX, l = 0.f;
+    PlainRow<CACHE_F32, HD> one(a, i, head, lane);
+    for (int v = v0 + warp; v < v1; v += 8) one.see(a, base + run.at(v), lane);
+    if (lane == 0) { w_m[warp] = one.m; w_l[warp] = one.l; }
 #pragma unroll
-    for (int e = 0; e < N; e++) q[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * c2;
-    for (int v = v0 + warp; v < v1; v += 8) {
-        const int64_t row = base + run.at(v);
-        float k[N], x[N];
-        load_row<CACHE_F32, HD>(a.k, a.k_scale, row, lane, k);
-        load_row<CACHE_F32, HD>(a.v, a.v_scale, row, lane, x);
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; e++) s = fmaf(q[e], k[e], s);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float m_new = fmaxf(m, s), w = exp2f(s - m_new), scale = exp2f(m - m_new);
-        l = l * scale + w;
-#pragma unroll
-        for (int e = 0; e < N; e++) o[e] = fmaf(o[e], scale, w * x[e]);
-        m = m_new;
-    }
-    if (lane == 0) { w_m[warp] = m; w_l[warp] = l; }
-#pragma unroll
-    for (int e = 0; e < N; e++) w_o[warp][lane * N + e] = o[e];
+    for (int e = 0; e < N; e++) w_o[warp][lane * N + e] = one.o[e];
     __syncthreads();
     if (threadIdx.x >= HD) return;
     float M = -FLT_MAX, L = 0.f, O = 0.f;

@@ -53,6 +53,31 @@ template <int KIND, int HD> __device__ __forceinline__ void load_row(const void*
     }
 }
 
+// The plain form of a row, by one warp: lanes over head_dim, one position after the other. Maximum m, sum l, unnormalised result o.
+template <int KIND, int HD> struct PlainRow {
+    static constexpr int N = HD / 32;
+    float q[N], o[N] = {}, m = -FLT_MAX, l = 0.f;
+    __device__ __forceinline__ PlainRow(const AttnLongArgs& a, int i, int head, int lane) {
+        const float c2 = rsqrtf((float)HD) * 1.4426950408889634f;
+#pragma unroll
+        for (int e = 0; e < N; e++) q[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * c2;
+    }
+    __device__ __forceinline__ void see(const AttnLongArgs& a, int64_t row, int lane) {   // the position at that row of the cache
+        float k[N], x[N], s = 0.f;
+        load_row<KIND, HD>(a.k, a.k_scale, row, lane, k);
+        load_row<KIND, HD>(a.v, a.v_scale, row, lane, x);
+#pragma unroll
+        for (int e = 0; e < N; e++) s = fmaf(q[e], k[e], s);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        const float m_new = fmaxf(m, s), w = exp2f(s - m_new), scale = exp2f(m - m_new);
+        l = l * scale + w;
+#pragma unroll
+        for (int e = 0; e < N; e++) o[e] = fmaf(o[e], scale, w * x[e]);
+        m = m_new;
+    }
+};
+
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 // A mean of f16 values as f16. Weights that were rounded up may put a mean of values next to the largest f16 beyond it (up to 65504 (1 + 2^-11)), and only
 // an infinity that the row sees may make one.

@@ -168,30 +168,16 @@ __global__ void __launch_bounds__(kThreads, 2) attn_long_f32_kernel(const __grid
     for (int y = warp; y < QT; y += kThreads / 32) {
         if (!((bad[y >> 5] >> (y & 31)) & 1)) continue;
         const int row = row0 + y, ii = row / a.group, head = kvh * a.group + row % a.group, pp = a.start + ii;
-        float qq[N], oo[N] = {}, mm = -FLT_MAX, ll = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; e++) qq[e] = a.q[ii * a.q_ld + head * HD + lane * N + e] * c2;
+        PlainRow<CACHE_F32, HD> one(a, ii, head, lane);
         for (int w = v0; w < v1; w++) {
             const int t = run.at(w);
-            if (!visible(a, pp, t)) continue;
-            float kk[N], x[N], s = 0.f;
-            load_row<CACHE_F32, HD>(a.k, nullptr, (int64_t)kvh * a.max_seq + t, lane, kk);
-            load_row<CACHE_F32, HD>(a.v, nullptr, (int64_t)kvh * a.max_seq + t, lane, x);
-#pragma unroll
-            for (int e = 0; e < N; e++) s = fmaf(qq[e], kk[e], s);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            const float m_new = fmaxf(mm, s), wt = exp2f(s - m_new), scale = exp2f(mm - m_new);
-            ll = ll * scale + wt;
-#pragma unroll
-            for (int e = 0; e < N; e++) oo[e] = fmaf(oo[e], scale, wt * x[e]);
-            mm = m_new;
+            if (visible(a, pp, t)) one.see(a, (int64_t)kvh * a.max_seq + t, lane);
         }
         const int64_t rec = ((int64_t)ii * a.heads + head) * a.n_split + blockIdx.y;
         float* dst = a.n_split > 1 ? a.rec_o + rec * HD : reinterpret_cast<float*>(a.out) + ii * a.out_ld + head * HD;
 #pragma unroll
-        for (int e = 0; e < N; e++) dst[lane * N + e] = a.n_split > 1 ? oo[e] : oo[e] / ll;
-        if (a.n_split > 1 && lane == 0) a.rec_ml[rec] = make_float2(mm, ll);
+        for (int e = 0; e < N; e++) dst[lane * N + e] = a.n_split > 1 ? one.o[e] : one.o[e] / one.l;
+        if (a.n_split > 1 && lane == 0) a.rec_ml[rec] = make_float2(one.m, one.l);
     }
 }
 

@@ -471,31 +471,16 @@ __global__ void __launch_bounds__(Ring<KIND, HD, CLUSTER>::THREADS, KIND == CACH
     for (uint32_t todo = bad; todo; todo &= todo - 1) {   // uniform: rows next to infinite or NaN cache contents that they do not see, one by one
         const int y = __ffs(todo) - 1, again = row0 + y, i = again / a.group, head = kvh * a.group + again % a.group, pp = a.start + i;
         constexpr int N = HD / 32;
-        const float k2 = rsqrtf((float)HD) * 1.4426950408889634f;
-        float qq[N], oo[N] = {}, mm = -FLT_MAX, ll = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; e++) qq[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * k2;
+        PlainRow<KIND, HD> one(a, i, head, lane);
         for (int w = v0 + warp; joins && w < v1; w += kWarps) {
             const int t = run.at(w);
-            if (!visible(a, pp, t)) continue;
-            float k[N], x[N], s = 0.f;
-            load_row<KIND, HD>(a.k, a.k_scale, base + t, lane, k);
-            load_row<KIND, HD>(a.v, a.v_scale, base + t, lane, x);
-#pragma unroll
-            for (int e = 0; e < N; e++) s = fmaf(qq[e], k[e], s);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            const float m_new = fmaxf(mm, s), wt = exp2f(s - m_new), scale = exp2f(mm - m_new);
-            ll = ll * scale + wt;
-#pragma unroll
-            for (int e = 0; e < N; e++) oo[e] = fmaf(oo[e], scale, wt * x[e]);
-            mm = m_new;
+            if (visible(a, pp, t)) one.see(a, base + t, lane);
         }
         __syncthreads();
         if (joins) {
-            if (lane == 0) { m_s[warp][0] = mm; l_s[warp][0] = ll; }
+            if (lane == 0) { m_s[warp][0] = one.m; l_s[warp][0] = one.l; }
 #pragma unroll
-            for (int e = 0; e < N; e++) o_s[warp][0][lane * N + e] = oo[e];
+            for (int e = 0; e < N; e++) o_s[warp][0][lane * N + e] = one.o[e];
         }
         __syncthreads();
         if (jr == y) join(kWarps, 0);

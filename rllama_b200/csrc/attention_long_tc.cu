@@ -179,35 +179,20 @@ __device__ __forceinline__ Cols step_cols(const AttnLongArgs& a, const Steps& st
     return c;
 }
 
-// The plain form of one row over steps [j0, j1), by one warp: what the row sees and nothing else.
+// One row over steps [j0, j1), by one warp: what the row sees and nothing else.
 template <int KIND, int HD>
 __device__ __noinline__ void slow_row(const AttnLongArgs& a, int kvh, int row, int j0, int j1, const Steps& st, float& m_out, float& l_out, float (&o)[HD / 32]) {
-    constexpr int N = HD / 32;
-    const int lane = threadIdx.x & 31, i = row / a.group, head = kvh * a.group + row % a.group, p = a.start + i;
-    const float c2 = rsqrtf((float)HD) * 1.4426950408889634f;
-    float q[N], m = -FLT_MAX, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < N; e++) { q[e] = a.q[i * a.q_ld + head * HD + lane * N + e] * c2; o[e] = 0.f; }
+    const int lane = threadIdx.x & 31, i = row / a.group, p = a.start + i;
+    PlainRow<KIND, HD> one(a, i, kvh * a.group + row % a.group, lane);
     for (int j = j0; j < j1; j++)
         for (int x = 0; x < TK; x++) {
             const int t = st.at(j) + x;
-            if (!(j < st.n_first ? t < st.s : visible(a, p, t))) continue;
-            float k[N], v[N], s = 0.f;
-            const int64_t r = (int64_t)kvh * a.max_seq + t;
-            load_row<KIND, HD>(a.k, a.k_scale, r, lane, k);
-            load_row<KIND, HD>(a.v, a.v_scale, r, lane, v);
-#pragma unroll
-            for (int e = 0; e < N; e++) s = fmaf(q[e], k[e], s);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            const float m_new = fmaxf(m, s), w = exp2f(s - m_new), scale = exp2f(m - m_new);
-            l = l * scale + w;
-#pragma unroll
-            for (int e = 0; e < N; e++) o[e] = fmaf(o[e], scale, w * v[e]);
-            m = m_new;
+            if (j < st.n_first ? t < st.s : visible(a, p, t)) one.see(a, (int64_t)kvh * a.max_seq + t, lane);
         }
-    m_out = m;
-    l_out = l;
+    m_out = one.m;
+    l_out = one.l;
+#pragma unroll
+    for (int e = 0; e < HD / 32; e++) o[e] = one.o[e];
 }
 
 template <int KIND, int HD> struct Layout {
@@ -412,7 +397,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                     }
                 }
             };
-            // (row rr + 32 u keeps rr's place in the swizzle pattern, so the four passes store at constant offsets)
+            // (row rr + 32 u keeps rr's place in the swizzle pattern, so all passes store at constant offsets)
             uint32_t off[G];
 #pragma unroll
             for (int g = 0; g < G; g++) {
