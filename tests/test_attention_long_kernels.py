@@ -270,3 +270,29 @@ def test_values_next_to_the_largest_f16(on, n):
         out, k, v = T.attend(cl, q, k, v, heads, kv, hd, start, 300, 2, kind, total + 3)
         want = v[0, 0].repeat(heads).double()
         assert ((out.double() - want).abs() <= 2 * 2.0 ** -11 * want.abs()).all() and (out.double().abs() <= 65504).all()
+
+
+@pytest.mark.parametrize("on", [x for x in KERNELS if x[1] == "few" or x[0] == "f32"], ids="-".join, indirect=True)
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_queries_keep_their_low_halves(on, n):
+    """Two kinds of keys whose scores differ by what f16 queries would lose: the kernel for few rows, which holds 22 bits of them, tells them apart (and so
+    does f32). The tile kernel rounds queries to f16 and is not asked."""
+    kind, cl = on
+    heads, kv, hd, start = 4, 2, 128, 300
+    total = start + n
+    q = torch.full((n, heads, hd), 8.0, device=T.DEV)
+    q[..., hd // 2:] *= 1 + 0.98 * 2.0 ** -11                       # rounds down to 8 in f16
+    k = torch.zeros(kv, total, hd, device=T.DEV)
+    k[:, ::2, :hd // 2] = k[:, 1::2, hd // 2:] = 1.4140625
+    v = torch.ones(kv, total, hd, device=T.DEV)
+    v[:, 1::2] = -1.0
+    q = q.view(n, -1)
+    out, k, v = T.attend(cl, q, k, v, heads, kv, hd, start, 200, 3, kind, total + 3)
+    want, spread, top = T.attention64(q, k, v, heads, kv, hd, start, 200, 3)
+    # queries 2^-22; products summed by additions that may cut off, a whole step each, with 4 bits of codes up to 15 where the values are 7; weights as
+    # everywhere (2^-11 in f16, sums of 203)
+    e = (2.0 ** -22 + 2 * (hd + 8) * 2.0 ** -24) * top * (15 / 7 if kind == "q4" else 1) + (211 + 8) * 2.0 ** -24 + (0 if kind == "f32" else 2.0 ** -11)
+    tol = 1.1 * 2 * e * spread + torch.finfo(out.dtype).eps / 2 * want.abs() + 2.0 ** -25
+    assert ((out.double() - want).abs() <= tol).all()
+    short = T.attention64(q.half().float(), k, v, heads, kv, hd, start, 200, 3)[0]
+    assert ((short - want).abs() > 2 * tol).all()   # (what a lost low half looks like)
