@@ -217,6 +217,7 @@ int rlb_cache4_create(rlb_ctx* ctx, int32_t kv_heads, int32_t max_seq_len, int32
     DeviceScope dev(ctx->device);
     RLB_CUDA(dev.err);
     if (ctx_capturing(ctx)) return rlb_fail(RLB_ERR_STATE, "rlb_cache4_create allocates: it cannot be captured into a graph");
+    OutsideCapture now;
     const size_t rows = (size_t)kv_heads * max_seq_len;
     const size_t codes = (rows * (head_dim / 2) + 255) & ~(size_t)255, scales = (rows * (head_dim / kQ4Group) * 2 + 255) & ~(size_t)255;
     rlb_cache4* c = new (std::nothrow) rlb_cache4();
@@ -266,7 +267,7 @@ int rlb_cache4_free(rlb_cache4* c) {
     if (!c) return RLB_OK;
     if (c->owned) {
         DeviceScope dev(c->device);
-        OutsideCapture free_now;
+        OutsideCapture now;
         cudaFree(c->owned);  // waits for the device
     }
     delete c;

@@ -67,6 +67,19 @@ static int refuse_capture(const rlb_ctx* ctx, const char* op, const char* why = 
     return RLB_OK;
 }
 
+static int grow_op_scratch(rlb_ctx* c, size_t bytes) {
+    if (bytes <= c->op_scratch_bytes) return RLB_OK;
+    OutsideCapture now;
+    RLB_CUDA(cudaStreamSynchronize(c->stream));
+    if (c->op_scratch) cudaFree(c->op_scratch);
+    c->op_scratch = nullptr;
+    c->op_scratch_bytes = 0;
+    cudaError_t e = cudaMalloc(&c->op_scratch, bytes);
+    if (e != cudaSuccess) { c->op_scratch = nullptr; return rlb_fail(RLB_ERR_OOM, "scratch (%zu bytes): %s", bytes, cudaGetErrorString(e)); }
+    c->op_scratch_bytes = bytes;
+    return RLB_OK;
+}
+
 int OpWorkspace::get(rlb_ctx* c, size_t bytes) {
     ctx = c;
     if (ctx_capturing(c)) {
@@ -75,15 +88,7 @@ int OpWorkspace::get(rlb_ctx* c, size_t bytes) {
         in_graph = true;
         return RLB_OK;
     }
-    if (bytes > c->op_scratch_bytes) {
-        RLB_CUDA(cudaStreamSynchronize(c->stream));
-        if (c->op_scratch) cudaFree(c->op_scratch);
-        c->op_scratch = nullptr;
-        c->op_scratch_bytes = 0;
-        cudaError_t e = cudaMalloc(&c->op_scratch, bytes);
-        if (e != cudaSuccess) { c->op_scratch = nullptr; return rlb_fail(RLB_ERR_OOM, "scratch (%zu bytes): %s", bytes, cudaGetErrorString(e)); }
-        c->op_scratch_bytes = bytes;
-    }
+    RLB_TRY(grow_op_scratch(c, bytes));
     p = c->op_scratch;
     return RLB_OK;
 }
@@ -130,6 +135,7 @@ static int ctx_new(int verbose, int nth_device, bool borrow, cudaStream_t stream
                         nth_device, prop.name, prop.major, prop.minor);
     if (verbose) printf("---\nSelected CUDA device: %s\n", prop.name);
     RLB_CUDA(cudaSetDevice(nth_device));
+    OutsideCapture now;
     rlb_ctx* ctx = new rlb_ctx();
     ctx->device = nth_device;
     ctx->sm_count = prop.multiProcessorCount;
@@ -187,7 +193,8 @@ int rlb_ctx_create_on_stream(int verbose, int nth_device, void* cuda_stream, rlb
 int rlb_ctx_destroy(rlb_ctx* ctx) {
     if (!ctx) return RLB_OK;
     DeviceScope dev(ctx->device);
-    cudaStreamSynchronize(ctx->stream);
+    OutsideCapture now;
+    if (!ctx_capturing(ctx)) cudaStreamSynchronize(ctx->stream);
     if (ctx->op_scratch) cudaFree(ctx->op_scratch);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
     if (ctx->h_err) cudaFreeHost(ctx->h_err);
@@ -202,6 +209,7 @@ int rlb_ctx_flush(rlb_ctx* ctx) {
     DeviceScope dev(ctx->device);
     RLB_CUDA(dev.err);
     RLB_TRY(refuse_capture(ctx, "rlb_ctx_flush", "it waits"));
+    OutsideCapture now;
     RLB_CUDA(cudaStreamSynchronize(ctx->stream));
     return ctx_check_error_word(ctx);
 }
@@ -223,6 +231,7 @@ static int tensor_new(rlb_ctx* ctx, int64_t rows, int64_t cols, int64_t cap, rlb
         return rlb_fail(RLB_ERR_INVALID, "tensor: capacity_cols %lld does not give 16-byte aligned rows", (long long)cap);
     DeviceScope dev(ctx->device);
     RLB_TRY(refuse_capture(ctx, "making a tensor", "it allocates"));
+    OutsideCapture now;
     rlb_tensor* t = new rlb_tensor();
     t->ctx = ctx; t->device = ctx->device; t->rows = rows; t->cols = cols; t->cap = cap; t->dtype = dtype;
     size_t bytes = t->bytes();
@@ -300,6 +309,7 @@ int rlb_tensor_wait(rlb_tensor* t) {
     DeviceScope dev(t->device);
     RLB_CUDA(dev.err);
     RLB_TRY(refuse_capture(t->ctx, "rlb_tensor_wait", "it waits"));
+    OutsideCapture now;
     if (t->ready && !t->ctx->borrowed_stream) RLB_CUDA(cudaEventSynchronize(t->ready));
     else RLB_CUDA(cudaStreamSynchronize(t->ctx->stream));  // (a graph that was replayed there has recorded no event)
     return ctx_check_error_word(t->ctx);
@@ -334,6 +344,7 @@ int rlb_tensor_download(rlb_tensor* t, void* host, rlb_event** out_event) {
 
 int rlb_event_wait(rlb_event* ev) {
     if (!ev) return rlb_fail(RLB_ERR_INVALID, "rlb_event_wait: null event");
+    OutsideCapture now;
     cudaError_t e = cudaEventSynchronize(ev->ev);
     rlb_ctx* ctx = ev->ctx;
     cudaEventDestroy(ev->ev);
@@ -349,7 +360,7 @@ int rlb_tensor_free(rlb_tensor* t) {
         return RLB_OK;
     }
     DeviceScope dev(t->device);  // (the context may be gone by now)
-    OutsideCapture free_now;
+    OutsideCapture now;
     if (t->ready) {
         cudaEventSynchronize(t->ready);  // the reference also waits for the initial write before dropping
         cudaEventDestroy(t->ready);
@@ -471,15 +482,7 @@ extern "C" int rlb_attention_decode(rlb_tensor* out, const rlb_tensor* q, const 
     // scratch: [pos : 256 B][counters : heads, padded to 256 B][records]
     const size_t cnt_bytes = ((size_t)heads * sizeof(unsigned int) + 255) & ~(size_t)255;
     const size_t need = 256 + cnt_bytes + attn_decode_scratch_floats(heads, hd, n_split) * sizeof(float);
-    if (need > ctx->op_scratch_bytes) {
-        RLB_CUDA(cudaStreamSynchronize(ctx->stream));
-        if (ctx->op_scratch) cudaFree(ctx->op_scratch);
-        ctx->op_scratch = nullptr;
-        ctx->op_scratch_bytes = 0;
-        cudaError_t e = cudaMalloc(&ctx->op_scratch, need);
-        if (e != cudaSuccess) return rlb_fail(RLB_ERR_OOM, "attention scratch (%zu bytes): %s", need, cudaGetErrorString(e));
-        ctx->op_scratch_bytes = need;
-    }
+    RLB_TRY(grow_op_scratch(ctx, need));
     char* base = (char*)ctx->op_scratch;
     RLB_CUDA(cudaMemsetAsync(base, 0, 256 + cnt_bytes, ctx->stream));
     AttnDecodeArgs a;

@@ -505,6 +505,7 @@ int make_map(CUtensorMap* map, const void* ptr, int rows, int K, int64_t ld, int
 // Grows the context's GEMM scratch (split activations + partial tiles) to at least `need` bytes.
 int reserve_scratch(rlb_ctx* ctx, size_t need) {
     if (need <= ctx->gemm_scratch_bytes) return RLB_OK;
+    OutsideCapture now;
     RLB_CUDA(cudaStreamSynchronize(ctx->stream));
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
     ctx->gemm_scratch = nullptr;

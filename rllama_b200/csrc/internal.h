@@ -97,7 +97,8 @@ struct DeviceScope {
     ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
 };
 
-// Handles may be dropped while the thread captures some stream: a free is no part of the graph and may not end the capture.
+// Allocations, frees and waits while this or another thread captures some other stream (or handles are dropped during the capture of this one): they are no part
+// of the graph, and in the runtime's default mode they would end the capture.
 struct OutsideCapture {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }

@@ -66,3 +66,31 @@ def test_handles_may_be_dropped_during_a_capture(on):
 
     assert (captured(on, during) == 6).all()
     assert torch.cuda.mem_get_info()[0] - held > 1 << 30
+
+
+def test_another_context_works_during_a_capture(on, monkeypatch):
+    """A context on another stream may be made, allocate, run and go while this one's stream is captured (as by a second thread)."""
+    from rllama_b200 import Cache4, Cuda
+    monkeypatch.setenv("RLB_ATTN_LONG_SPLITS", "3r")   # scratch for records
+    side = torch.cuda.Stream()
+    q, kc = torch.ones(1, 256, device="cuda"), torch.ones(2 * 300, 128, dtype=torch.float16, device="cuda")
+    outs = [torch.zeros(1, 256, dtype=torch.float16, device="cuda") for _ in range(3)]
+    torch.cuda.synchronize()
+
+    def during(x):
+        other = Cuda(stream=side.cuda_stream)
+        W = other.wrap
+        W(outs[0]).attention_window(W(q), W(kc), W(kc), 2, 2, 300, 299, 300)
+        table, cache, zeros = other.rope_table(300, 128), Cache4(other, 2, 300, 128), other.zeros(300, 256, 0)
+        cache.append(zeros, zeros, 0)
+        cache.attention(W(outs[1]), W(q), 2, 299)
+        W(outs[2]).attention_decode(W(q), W(kc), W(kc), 2, 300, 299, 40)
+        assert (W(outs[0]).to_numpy() == 1).all()
+        other.flush()
+        for t in (table, cache, zeros):
+            t.free()
+        other.close()
+
+    outs[1].fill_(1)
+    assert (captured(on, during) == 6).all()
+    assert (outs[0] == 1).all() and (outs[1] == 0).all() and (outs[2] == 1).all()
