@@ -18,7 +18,7 @@ namespace {
 
 // One query row over an f32 cache: a CTA of eight warps, a warp per position, lanes over head_dim; grid (rows, splits). A row reads what it sees for
 // itself, so the bound is the caches' reading for one row and L2 for several (8 rows after 10000 positions, 32 heads: 306 us, 8.6 TB/s from L2);
-// 77 rows of 8 heads on 4, window 100, are 9.4 us, half of them the call. Four rows of a K/V head to a CTA, each position fetched once for them, are no
+// 77 rows of 8 heads on 4, window 100, are 8.8 us, half of them the call. Four rows of a K/V head to a CTA, each position fetched once for them, are no
 // faster (that case 15.6, 16 rows after 4000 positions 186 against 117; only 64 heads on 8 gain, 208 to 194), nor are two or four positions of a warp at
 // a time: more registers, fewer warps.
 template <int HD>
@@ -201,7 +201,10 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
         // The kernel for few rows reads the cache once for every eight of them, the one for many rows has tiles of 128 (256 in 4 bits) that cost
         // the same however many of their rows there are. Each says what it expects to take, from what was measured; e.g. 32
         // heads, 8000 positions, us with few / tiles: f16 8 rows 31 / 31, 16 rows 49 / 33, 64 rows 163 / 38; 4 bits 8 rows 21 / 43, 24 rows 62 / 44, 64
-        // rows 104 / 46; 300 positions: f16 32 rows 10 / 13, 64 rows 17 / 14; 4 bits 64 rows 13 / 17, 128 rows 23 / 19.
+        // rows 104 / 46; 300 positions: f16 32 rows 10 / 13, 64 rows 17 / 14; 4 bits 64 rows 13 / 17, 128 rows 23 / 19. Not covered: prompts with windows
+        // of up to 16 positions (4 bits, narrow heads: up to 64). A round of CTAs of the kernel for few rows costs about 4 us (4 bits 5.5) however little it
+        // reads, which its estimate leaves out: 1792 rows of 64 heads, window 4, take 378 us where tiles take 45 (4 bits 265 and 68). With wider windows the
+        // choice was right in all of the shapes measured but one: 512 rows of 8 heads of 64, window 256, 15.9 and 12.1.
         const AttnSplit s = attn_long_few_splits(ctx, kind, a);
         const int t = attn_long_tc_splits(ctx, kind, a);
         few = ctx->attn_long ? ctx->attn_long == 1 : attn_long_few_us(ctx, kind, a, s) <= attn_long_tc_us(ctx, kind, a, t);

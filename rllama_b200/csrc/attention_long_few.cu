@@ -18,7 +18,7 @@
 // (2^-11) and the result.
 //
 // Measured: 65536 4-bit positions, 32 heads, one token, 94 us, 3.2 TB/s: 446 instructions for 16 positions of a head (185 of them integer and
-// conversions) at 61 % of the issue rate; 384 positions 6.4 us, of which about 5 are the call. 16384 f16 positions and 4 first tokens, 64 heads on 8,
+// conversions), 61 % of the issue slots; 384 positions 6.4 us a call, 5.1 in a graph. 16384 f16 positions and 4 first tokens, 64 heads on 8,
 // 20.5 us, 3.3 TB/s: the second kernel and the ring's first fill are half of it.
 //
 // Loads straight into registers (two tiles ahead: 141 us, one: 107, of 65536 positions, 32 heads, 4 bits) wait for one another: a warp
@@ -584,7 +584,8 @@ AttnSplit attn_long_few_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs&
 }
 
 // 6 us, 2 more for a second kernel, and the rounds of CTAs over the SMs, a CTA reading 44 KB a us (f16: an SM's share of the memory's rate) or,
-// with 4 bits and two CTAs an SM, 9.8 KB (what their arithmetic allows).
+// with 4 bits and two CTAs an SM, 9.8 KB (what their arithmetic allows). A round's own cost, whatever it reads, is not counted:
+// attention_long.cu says where that matters.
 double attn_long_few_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, AttnSplit s) {
     const int64_t ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + kRows - 1) / kRows), slots = (int64_t)ctx->sm_count * (kind == CACHE_Q4 ? 2 : 1);
     const double row = kind == CACHE_Q4 ? a.hd + a.hd / 8 : a.hd * 4, rate = kind == CACHE_Q4 ? 9.8e3 : 44e3;

@@ -19,9 +19,9 @@
 //    scores exceed it by 2^8 (then the row's O is scaled in place); weights therefore stay below 2^15, and the factor
 //    2^7 keeps weights down to 2^-21 of the largest normal f16 numbers. It cancels in O / l.
 //
-// Measured: 8192 rows, 32 heads on 8, window 2048 and 16 first tokens, 253 us, 955 TFLOP/s (305 us in a long run, at the clock that the power limit
-// leaves); 1792 rows, 64 heads, window 512 and 4 first tokens, 66 us, 395 TFLOP/s; 512 rows after 7680 positions in 4 bits, 40 heads, 134 us,
-// 620 TFLOP/s. The bound is latency: a step of the softmax is 64 exponentials (512 of its 1900 cycles, twice that for the two tiles of an SM) between
+// Measured over repeated calls: 8192 rows, 32 heads on 8, window 2048 and 16 first tokens, 302 us, 801 TFLOP/s, at the clock that the power limit
+// leaves (253 us in a short burst); 1792 rows, 64 heads, window 512 and 4 first tokens, 70.5 us, 368 TFLOP/s (63 in a graph); 512 rows after 7680
+// positions in 4 bits, 40 heads, 136 us, 612 TFLOP/s. The bound is latency: a step of the softmax is 64 exponentials (512 of its 1900 cycles, twice that for the two tiles of an SM) between
 // waits, tensor-memory reads and writes of 100 to 200 cycles each; tensor and exponential units are 45 to 50 % busy. What did not shorten it: part of
 // the exponentials by a polynomial, two threads a row, fetching the next scores before the weights are known to have arrived.
 //

@@ -49,10 +49,10 @@ struct AppendArgs {
 // All kernels: a grid over heads, rows, and K and V (with the rotation also q, whose rows go through f32 to where the caller wants them). A thread
 // takes the same block of eight values of every group of a head's row when it reads, which is a quarter of the row's codes side by side
 // (cache4.h), and of half of the groups when it writes; four or eight threads make a row. No thread divides by a runtime size. (1792 rows of 64
-// heads of 128, f32, written and read back: one word a thread, found by 64-bit division: 51 + 49 us; this: 27 + 13 us, of 20 + 11 that the bytes
-// take. A quarter row a thread in the append too: 28, as it leaves room for half of the warps; two rows a thread, or CTAs of 256: up to 10 us
-// more.) With the rotation, 64 heads of q beside them: 48.6 us, 5.2 TB/s (a quarter row a thread: 51.1), where the two ops one after the other take
-// 50 + 27; a token's row is the call's 4 us.
+// heads of 128, f32, written and read back: one word a thread, found by 64-bit division: 51 + 49 us; this: 27 + 14 us, of 20 + 11 that the bytes
+// take; f16 rows 23 in a graph, where f32 rows are 23.5. A quarter row a thread in the append too: 28, as it leaves room for half of the warps; two rows a thread, or CTAs of 256: up to 10 us
+// more.) With the rotation, 64 heads of q beside them: 49 us, 5.2 TB/s (a quarter row a thread: 51), with the norm 57, where the two ops one after the
+// other take 51 + 27; 64 heads on 8, with the norm, 31; a token's row 3.3 us in a graph, and a call's 4.
 constexpr int kThreads = 128;
 template <int G> struct Words;   // a thread's words of a row, and their scales
 template <> struct Words<4> { typedef uint4 T; typedef uint2 D; };

@@ -7,9 +7,9 @@
 //
 // All of it is f32; a cache row is rounded once, to the cache's dtype.
 //
-// Every value is read and written once, so memory is the bound: 1792 rows of 64 heads and 64 K/V heads of 128 into f16 caches, with the norm, take 49 us,
-// 5.9 TB/s (one row a thread at a time 63; two or eight no faster than four; streaming loads and stores neither). Instructions count beside it: with a
-// reduction over the warp, a square root and a division for every row it was 57. A token's row is the call's 5 us.
+// Every value is read and written once, so memory is the bound: 1792 rows of 64 heads and 64 K/V heads of 128 into f16 caches, with the norm, take 51 us
+// a call, 5.7 TB/s (47 in a graph; one row a thread at a time 63; two or eight no faster than four; streaming loads and stores neither). Instructions count
+// beside it: with a reduction over the warp, a square root and a division for every row it was 57. A token's row is 2 us in a graph, and a call's 5 us.
 #include "internal.h"
 
 #include <algorithm>
