@@ -4,7 +4,7 @@
 //
 // A CTA owns one tile of 128 rows of a K/V head (f16; two CTAs share an SM) or two (4 bits) and walks the positions that some of them see in
 // steps of 64:
-//  * K and V steps pass through a ring of shared-memory stages, in the order in which they are used: K0 K1 V0 K2 V1 K3 ...
+//  * K and V steps pass through a ring of shared-memory stages (attention_long_ring.h), in the order in which they are used: K0 K1 V0 K2 V1 K3 ...
 //    An f16 cache's are fetched by TMA (128-byte swizzle, the tensor's extent ends at the last visible position: rows
 //    behind it read as zeros). A 4-bit cache's are unpacked by eight warps; its values are f16 numbers, so the unpacked
 //    operand carries no rounding.
@@ -40,6 +40,7 @@
 #include <algorithm>
 
 #include "attention_long.h"
+#include "attention_long_ring.h"
 
 using namespace attn_long;
 
@@ -205,7 +206,8 @@ template <int KIND, int HD> struct Layout {
     // 16 bytes of a row each then meet no bank twice).
     static constexpr uint32_t OUT_ROW = HD * 2 + 16, Q_ROOM = QT * OUT_ROW;
     static constexpr uint32_t STAGE = TK * HD * 2;
-    static constexpr int STAGES = (TILES == 2 ? 8 : 4) * 128 / HD;
+    typedef KvRing<(TILES == 2 ? 4 : 2) * 128 / HD, (TILES == 2 ? 4 : 2) * 128 / HD> Ring;
+    static constexpr int STAGES = Ring::STAGES;
     static constexpr uint32_t TMEM_COLS = TILES * 256;
     // warps: four a tile for the softmax, two a tile for its MMAs, then one that loads (and an idle one: registers are dealt to four warps
     // at a time), or eight that unpack
@@ -225,6 +227,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     attn_long_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_k_first, const __grid_constant__ CUtensorMap tm_v_first, const __grid_constant__ AttnLongArgs a, int ahead, int* err) {
     typedef Layout<KIND, HD> Y;
+    typedef typename Y::Ring Ring;
     constexpr int NB = Y::NB, STAGES = Y::STAGES, TILES = Y::TILES, QB = Y::ROWS;
     constexpr uint32_t O_COL = TILES * 2 * TK;   // [tile]: S [TK], P [buffer][TK / 2]; then [tile]: O [HD]
     extern __shared__ unsigned char smem_raw[];
@@ -254,13 +257,9 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     const bool two = TILES == 2 && row0 + QT <= row_last;  // the second tile has rows
     auto cols = [&](int t, int j) { return t == 0 || two ? step_cols(a, st, j, pa[t], pb[t]) : Cols{0, 0}; };
 
-    // K and V steps pass through the ring as items K0 K1 V0 K2 V1 ...
-    const int items = 2 * (j1 - j0);
-    auto item_is_v = [&](int x) { return x > 0 && (x % 2 == 0 || x == items - 1); };
-    auto item_step = [&](int x) { return j0 + (x == items - 1 ? x / 2 : item_is_v(x) ? x / 2 - 1 : (x + 1) / 2); };
-    auto load = [&](int x) {   // f16, one thread
-        const int s = x % STAGES, j = item_step(x), t0 = st.at(j);
-        const bool v = item_is_v(x);
+    const int n_steps = j1 - j0;   // items of K, and of V, for the ring
+    auto load = [&](bool v, int i) {   // f16, one thread
+        const int s = Ring::at(v, i).stage, j = j0 + i, t0 = st.at(j);
         const CUtensorMap* map = j < st.n_first ? (v ? &tm_v_first : &tm_k_first) : (v ? &tm_v : &tm_k);
         mbar_expect_tx(&full[s], Y::STAGE);
 #pragma unroll
@@ -284,7 +283,10 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if constexpr (KIND == CACHE_F16)
-            for (int x = 0; x < min(items, STAGES); x++) load(x);
+            for (int k = 0, v = 0; k < min(n_steps, Ring::K) || v < min(n_steps, Ring::V);) {   // as many as there are stages
+                const bool is_v = v < min(n_steps, Ring::V) && (k == min(n_steps, Ring::K) || Ring::next_is_v(k, v, n_steps));
+                load(is_v, is_v ? v++ : k++);
+            }
     }
     __syncwarp();
     if (warp == Y::MMA_WARP) {
@@ -351,13 +353,15 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         // ------------------------------- K and V steps into the ring -------------------------------------------------
         if constexpr (KIND == CACHE_F16) {
             if (warp == Y::LOAD_WARP && lane == 0) {
-                int x = min(items, STAGES);   // (the first are on their way)
-                for (; x < items; x++) {
-                    const int s = x % STAGES;
-                    if (!mbar_wait(&empty[s], (x / STAGES - 1) & 1, dead, err)) break;
-                    load(x);
+                int k = min(n_steps, Ring::K), v = min(n_steps, Ring::V);   // (the first are on their way)
+                while (k < n_steps || v < n_steps) {
+                    const bool is_v = Ring::next_is_v(k, v, n_steps);
+                    const typename Ring::Slot slot = Ring::at(is_v, is_v ? v : k);
+                    if (!mbar_wait(&empty[slot.stage], slot.parity ^ 1, dead, err)) break;
+                    load(is_v, is_v ? v++ : k++);
                 }
-                for (int y = max(0, x - STAGES); y < x; y++) mbar_drain(&full[y % STAGES], (y / STAGES) & 1);  // no copy outlives the CTA
+                for (int i = max(0, k - Ring::K); i < k; i++) mbar_drain(&full[Ring::at(false, i).stage], Ring::at(false, i).parity);   // no copy outlives the CTA
+                for (int i = max(0, v - Ring::V); i < v; i++) mbar_drain(&full[Ring::at(true, i).stage], Ring::at(true, i).parity);
             } else if (warp > Y::LOAD_WARP && a.n_split == 1 && blockIdx.x + ahead < gridDim.x) {
                 // The queries of the CTA that will have this one's place, into L2: the CTAs of a round start together, and memory is idle in
                 // between (1792-row window prompt 68 us without, 66 with).
@@ -369,16 +373,16 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                 }
             }
         } else {
-            // Two groups of four warps take every other item. A thread unpacks a quarter of a row: the same block of eight
+            // Four warps for K and four for V. A thread unpacks a quarter of a row: the same block of eight
             // values of every group (cache4.h), 32 rows a pass; the next AHEAD items of its warps are on their way.
             constexpr int G = HD / kQ4Group, ROWS = 32, PASSES = TK / ROWS, AHEAD = 2;
-            const int x0 = (threadIdx.x - Y::LOAD_WARP * 32) & 127, quarter = x0 & 3, rr = x0 >> 2, group = (warp - Y::LOAD_WARP) >> 2;
+            const int x0 = (threadIdx.x - Y::LOAD_WARP * 32) & 127, quarter = x0 & 3, rr = x0 >> 2;
+            const bool v = warp < Y::LOAD_WARP + 4;
             uint32_t w[AHEAD][PASSES][G];
             __half d[AHEAD][PASSES][G];
             const int64_t base = (int64_t)kvh * a.max_seq + rr;
-            auto fetch = [&](int x, uint32_t (&w)[PASSES][G], __half (&d)[PASSES][G]) {
-                const bool v = item_is_v(x);
-                const int j = item_step(x), t0 = st.at(j), end = (j < st.n_first ? min(a.sinks, a.start + a.n) : a.start + a.n) - t0 - rr;
+            auto fetch = [&](int i, uint32_t (&w)[PASSES][G], __half (&d)[PASSES][G]) {
+                const int j = j0 + i, t0 = st.at(j), end = (j < st.n_first ? min(a.sinks, a.start + a.n) : a.start + a.n) - t0 - rr;
                 const uint8_t* codes = reinterpret_cast<const uint8_t*>(v ? a.v : a.k) + (base + t0) * (HD / 2) + quarter * (HD / 8);
                 const __half* scales = (v ? a.v_scale : a.k_scale) + (base + t0) * G;
 #pragma unroll
@@ -405,11 +409,11 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                 off[g] = (chunk >> 3) * (TK * 128) + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4);
             }
             bool ok = true;
-            auto unpack = [&](int x, uint32_t (&w)[PASSES][G], __half (&d)[PASSES][G]) {
-                const int s = x % STAGES;
-                ok = ok && (x < STAGES || warp_wait(&empty[s], (x / STAGES - 1) & 1, dead, err));
+            auto unpack = [&](int i, uint32_t (&w)[PASSES][G], __half (&d)[PASSES][G]) {
+                const typename Ring::Slot slot = Ring::at(v, i);
+                ok = ok && (!slot.used || warp_wait(&empty[slot.stage], slot.parity ^ 1, dead, err));
                 if (!ok) return;
-                unsigned char* dst = ring + s * Y::STAGE;
+                unsigned char* dst = ring + slot.stage * Y::STAGE;
 #pragma unroll
                 for (int u = 0; u < PASSES; u++) {
 #pragma unroll
@@ -422,18 +426,18 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                         *reinterpret_cast<uint4*>(dst + off[g] + u * ROWS * 128) = *reinterpret_cast<uint4*>(h);
                     }
                 }
-                if (x + 2 * AHEAD < items) fetch(x + 2 * AHEAD, w, d);
+                if (i + AHEAD < n_steps) fetch(i + AHEAD, w, d);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[s]);
+                if (lane == 0) mbar_arrive(&full[slot.stage]);
             };
 #pragma unroll
             for (int u = 0; u < AHEAD; u++)
-                if (group + 2 * u < items) fetch(group + 2 * u, w[u], d[u]);
-            for (int x = group; x < items && ok; x += 2 * AHEAD) {
+                if (u < n_steps) fetch(u, w[u], d[u]);
+            for (int i = 0; i < n_steps && ok; i += AHEAD) {
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
-                    if (x + 2 * u < items) unpack(x + 2 * u, w[u], d[u]);
+                    if (i + u < n_steps) unpack(i + u, w[u], d[u]);
             }
         }
     } else if (warp >= Y::MMA_WARP) {
@@ -455,9 +459,10 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(QT >> 4) << 24);   // | N / 8 << 17
             const uint64_t q_desc = desc_kmajor(smem_u32(q_s) + t * Y::Q_ROOM), k_desc = desc_kmajor(smem_u32(ring));
             for (int j = j0; j < j1 && ok; j++) {
-                const uint32_t x = j == j0 ? 0 : 2 * (j - j0) - 1, stage = x % STAGES;   // the step's place among the items
+                const typename Ring::Slot slot = Ring::at(false, j - j0);
+                const uint32_t stage = slot.stage;
                 const Cols c = cols_at(j);
-                ok = warp_wait(&full[stage], (x / STAGES) & 1, dead, err);
+                ok = warp_wait(&full[stage], slot.parity, dead, err);
                 if (c.any() && done > 0) ok = ok && warp_wait(&s_read[t], (done - 1) & 1, dead, err);
                 if (!ok) break;
                 if (c.any()) {
@@ -476,9 +481,10 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
             const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(QT >> 4) << 24);
             const uint64_t v_desc = desc_mnmajor(smem_u32(ring), TK * 128);
             for (int j = j0; j < j1; j++) {   // the n-th product takes its weights from buffer n & 1
-                const uint32_t x = j == j1 - 1 ? 2 * (j - j0) + 1 : 2 * (j - j0) + 2, stage = x % STAGES, buf = done & 1;
+                const typename Ring::Slot slot = Ring::at(true, j - j0);
+                const uint32_t stage = slot.stage, buf = done & 1;
                 const Cols c = cols_at(j);
-                ok = warp_wait(&full[stage], (x / STAGES) & 1, dead, err);
+                ok = warp_wait(&full[stage], slot.parity, dead, err);
                 if (c.any()) ok = ok && warp_wait(&p_ready[2 * t + buf], (done >> 1) & 1, dead, err);
                 if (!ok) break;
                 if (c.any()) {
