@@ -184,10 +184,9 @@ int rlb_norm_rope_append(rlb_tensor* q_out, rlb_tensor* kcache, rlb_tensor* vcac
  * what unseen cache rows hold does not matter.
  *   q    n x (heads*head_dim) f32, rotated
  *   out  n x (heads*head_dim) in the cache dtype, not q
- * f32 caches: f32 throughout. f16 caches: scores, maxima and sums in f32; the softmax weights
- * are rounded to f16 once, and so are the queries (scaled by a power of two a row) where tiles of
- * many rows are expected to be faster; with few rows they keep 22 bits. rlb_attention_prefill,
- * without a window, holds both as two f16 halves.                                             */
+ * f32 caches: f32 throughout. f16 caches: scores, maxima and sums in f32, queries held to 22
+ * bits; the softmax weights are rounded to f16 once, after their sum is taken (rlb_attention_prefill,
+ * without a window, holds them as two f16 halves).                                            */
 int rlb_attention_window(rlb_tensor* out, const rlb_tensor* q, const rlb_tensor* kcache, const rlb_tensor* vcache, int32_t heads,
                          int32_t kv_heads, int32_t max_seq_len, int32_t start_pos, int32_t window, int32_t sinks);
 

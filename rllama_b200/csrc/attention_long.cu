@@ -200,10 +200,10 @@ int launch_attn_long(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& given) {
     } else {
         // The kernel for few rows reads the cache once for every eight of them, the one for many rows has tiles of 128 (256 in 4 bits) that cost
         // the same however many of their rows there are. Each says what it expects to take, from what was measured; e.g. 32
-        // heads, 8000 positions, us with few / tiles: f16 8 rows 31 / 31, 16 rows 49 / 33, 64 rows 163 / 38; 4 bits 8 rows 21 / 43, 24 rows 62 / 44, 64
-        // rows 104 / 46; 300 positions: f16 32 rows 10 / 13, 64 rows 17 / 14; 4 bits 64 rows 13 / 17, 128 rows 23 / 19. Not covered: prompts with windows
+        // heads, 8000 positions, us with few / tiles: f16 8 rows 30 / 33, 16 rows 47 / 34, 64 rows 161 / 39; 4 bits 8 rows 20 / 43, 24 rows 60 / 44, 64
+        // rows 103 / 45; 300 positions: f16 32 rows 8 / 12, 64 rows 14 / 12; 4 bits 64 rows 10 / 15, 128 rows 18 / 16. Not covered: prompts with windows
         // of up to 16 positions (4 bits, narrow heads: up to 64). A round of CTAs of the kernel for few rows costs about 4 us (4 bits 5.5) however little it
-        // reads, which its estimate leaves out: 1792 rows of 64 heads, window 4, take 378 us where tiles take 45 (4 bits 265 and 68). With wider windows the
+        // reads, which its estimate leaves out: 1792 rows of 64 heads, window 4, take 378 us where tiles take 47 (4 bits 265 and 71). With wider windows the
         // choice was right in all of the shapes measured but one: 512 rows of 8 heads of 64, window 256, 15.9 and 12.1.
         const AttnSplit s = attn_long_few_splits(ctx, kind, a);
         const int t = attn_long_tc_splits(ctx, kind, a);

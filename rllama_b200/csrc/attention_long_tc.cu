@@ -8,8 +8,8 @@
 //    An f16 cache's are fetched by TMA (128-byte swizzle, the tensor's extent ends at the last visible position: rows
 //    behind it read as zeros). A 4-bit cache's are unpacked by eight warps; its values are f16 numbers, so the unpacked
 //    operand carries no rounding.
-//  * two warps a tile issue its MMAs: one S = Q K^T (both operands in shared memory), one O += P V with P in tensor memory as
-//    the A operand. Tensor memory holds, per tile, O, one buffer of 64 scores and two of 64 weights: the scores are free
+//  * two warps a tile issue its MMAs: one S = Q K^T (both operands in shared memory; the queries as two f16 halves, x = high + low, one
+//    after the other), one O += P V with P in tensor memory as the A operand. Tensor memory holds, per tile, O, one buffer of 64 scores and two of 64 weights: the scores are free
 //    again as soon as the softmax has them in registers, so the next ones are computed during the exponentials, and a
 //    weight buffer is only needed again two steps later. Neither side waits for a chain of the other's. (Weights written
 //    over their scores made a step's chain softmax, output product, next scores: with one buffer of 128 scores 5200
@@ -19,15 +19,18 @@
 //    scores exceed it by 2^8 (then the row's O is scaled in place); weights therefore stay below 2^15, and the factor
 //    2^7 keeps weights down to 2^-21 of the largest normal f16 numbers. It cancels in O / l.
 //
-// Measured over repeated calls: 8192 rows, 32 heads on 8, window 2048 and 16 first tokens, 302 us, 801 TFLOP/s, at the clock that the power limit
-// leaves (253 us in a short burst); 1792 rows, 64 heads, window 512 and 4 first tokens, 70.5 us, 368 TFLOP/s (63 in a graph); 512 rows after 7680
-// positions in 4 bits, 40 heads, 136 us, 612 TFLOP/s. The bound is latency: a step of the softmax is 64 exponentials (512 of its 1900 cycles, twice that for the two tiles of an SM) between
-// waits, tensor-memory reads and writes of 100 to 200 cycles each; tensor and exponential units are 45 to 50 % busy. What did not shorten it: part of
-// the exponentials by a polynomial, two threads a row, fetching the next scores before the weights are known to have arrived.
+// Measured over repeated calls: 8192 rows, 32 heads on 8, window 2048 and 16 first tokens, 372 us, 652 TFLOP/s, at the clock that the power limit
+// leaves (320 us in a graph); 1792 rows, 64 heads, window 512 and 4 first tokens, 80 us, 325 TFLOP/s (70.6 in a graph); 512 rows after 7680
+// positions in 4 bits, 40 heads, 150 us, 553 TFLOP/s (140 in a graph; products of the low halves not counted). Two things bound it by turns: the products, of which the
+// scores' read both operands from shared memory (6 KB for 32 cycles of arithmetic; leaving their second half out takes the 8192-row prompt from 320 to 256 us),
+// and latency, since a step of the softmax is 64 exponentials (512 of its cycles, twice that for the two tiles of an SM) between waits, tensor-memory reads and
+// writes of 100 to 200 cycles each. What did not shorten it: part of the exponentials by a polynomial, two threads a row, fetching the next scores before the
+// weights are known to have arrived; two f16 tiles a CTA over one ring of six stages (window prompt 79 us where it is 70 in a graph).
 //
-// Rounded to f16 besides the result: the queries, scaled by a power of two per row so that their largest element lies in
-// [2^8, 2^9) whatever the row's magnitude (an error of at most 2^-11 sum |q k| / sqrt(head_dim) in a score), and the
-// weights (2^-11 each). Scores, maxima, sums and O are f32.
+// Rounded to f16 besides the result: the weights (2^-11 each). Scores, maxima, sums and O are f32. The queries are scaled by a power of two per row so
+// that their largest element lies in [2^8, 2^9) whatever the row's magnitude, and their two halves hold 22 bits of it. With the high halves alone a score was
+// off by up to 2^-11 sum |q k| / sqrt(head_dim), and results by twice what their own rounding is (4.4e-4 from 64 bits, now 2.9e-4); the low ones double the score
+// products and take a stage of the ring (8192-row prompt 253 us in a graph, now 320; 1792-row window prompt 62.6 and 70.6; 512-row 4-bit chunk 132.5 and 139.7).
 //
 // A zero weight times an infinite or NaN value is a NaN in an MMA, so a row whose result is a NaN although its sum is not is computed
 // again, one warp to a row, from the positions that it sees alone. Only rows next to such cache contents pay for it.
@@ -196,24 +199,40 @@ __device__ __noinline__ void slow_row(const AttnLongArgs& a, int kvh, int row, i
     for (int e = 0; e < HD / 32; e++) o[e] = one.o[e];
 }
 
+// With head_dim 128, as many stages as fit beside the queries.
+template <int KIND, int HD> struct RingOf;
+template <> struct RingOf<CACHE_F16, 128> { typedef KvRing<2, 1> T; };
+template <> struct RingOf<CACHE_F16, 64> { typedef KvRing<4, 4> T; };
+template <> struct RingOf<CACHE_Q4, 128> { typedef KvRing<3, 3> T; };
+template <> struct RingOf<CACHE_Q4, 64> { typedef KvRing<8, 8> T; };
+
 template <int KIND, int HD> struct Layout {
     // An f16 CTA has one tile, and two CTAs share an SM: one's first loads, masks and last stores fall into the other's main
     // loop (8192 rows of 32 heads, window 2048: two tiles in one CTA 326 us, two CTAs 278). Unpacking 4-bit rows costs too much to be done for one tile: two share it.
     static constexpr int TILES = KIND == CACHE_Q4 ? 2 : 1;
     static constexpr int ROWS = TILES * QT;                  // rows of a CTA
     static constexpr int NB = HD / 64;                       // 64-column blocks of a row
-    // A tile's queries, 128 rows of f16 one after the other, and in the end its results, in rows that are 16 bytes longer (32 lanes that store
-    // 16 bytes of a row each then meet no bank twice).
-    static constexpr uint32_t OUT_ROW = HD * 2 + 16, Q_ROOM = QT * OUT_ROW;
+    // A tile's queries, 128 rows of f16 one after the other, their high halves and then the low ones, and in the end its results, in rows that are 16
+    // bytes longer (32 lanes that store 16 bytes of a row each then meet no bank twice).
+    static constexpr uint32_t Q_HALF = QT * HD * 2, Q_ROOM = 2 * Q_HALF, OUT_ROW = HD * 2 + 16;
+    static_assert(QT * OUT_ROW <= Q_ROOM, "the results fit in the queries' room");
     static constexpr uint32_t STAGE = TK * HD * 2;
-    typedef KvRing<(TILES == 2 ? 4 : 2) * 128 / HD, (TILES == 2 ? 4 : 2) * 128 / HD> Ring;
+    typedef typename RingOf<KIND, HD>::T Ring;
     static constexpr int STAGES = Ring::STAGES;
     static constexpr uint32_t TMEM_COLS = TILES * 256;
     // warps: four a tile for the softmax, two a tile for its MMAs, then one that loads (and an idle one: registers are dealt to four warps
     // at a time), or eight that unpack
     static constexpr int SOFTMAX_WARPS = 4 * TILES, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = MMA_WARP + 2 * TILES;
     static constexpr int THREADS = (LOAD_WARP + (KIND == CACHE_Q4 ? 8 : 2)) * 32;
-    static constexpr size_t SMEM = TILES * Q_ROOM + STAGES * STAGE + 1024;
+    struct Control {   // behind the queries and the ring
+        uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], drained[4];
+        uint64_t p_ready[4], pv_done[4];   // [tile][buffer]: a phase is seen before the next one begins
+        float c2[ROWS];                    // a row's scores are s * c2 in units of log2 e
+        uint32_t tmem_slot;
+        int dead;
+    };
+    static constexpr size_t SMEM = TILES * Q_ROOM + STAGES * STAGE + sizeof(Control);
+    static_assert((2 / TILES) * (SMEM + 1024) <= 228 * 1024, "the CTAs of an SM fit in its shared memory");
     // A thread is launched with LAUNCH_REGS registers (65536 over the threads of an SM, in eights); the MMA and loading warps give theirs to the
     // softmax warps, whose sum with what is left is what was launched: 128 * 152 + 128 * 104 = 256 * 128 (f16), 256 * 120 + 384 * 80 = 640 * 96.
     static constexpr int LAUNCH_REGS = KIND == CACHE_Q4 ? 96 : 128, SOFTMAX_REGS = KIND == CACHE_Q4 ? 120 : 152, OTHER_REGS = KIND == CACHE_Q4 ? 80 : 104;
@@ -230,15 +249,18 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     typedef typename Y::Ring Ring;
     constexpr int NB = Y::NB, STAGES = Y::STAGES, TILES = Y::TILES, QB = Y::ROWS;
     constexpr uint32_t O_COL = TILES * 2 * TK;   // [tile]: S [TK], P [buffer][TK / 2]; then [tile]: O [HD]
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* q_s = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // [tile][HD/64][128][64]
-    unsigned char* ring = q_s + TILES * Y::Q_ROOM;                                                               // [stage][HD/64][128][64]
-    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2], s_read[2], drained[4];
-    __shared__ __align__(8) uint64_t p_ready[4], pv_done[4];   // [tile][buffer]: a phase is seen before the next one begins
-    __shared__ float c2_s[QB];   // a row's scores are s * c2 in units of log2 e
-    __shared__ uint32_t tmem_slot;
-    __shared__ int dead_flag;
-    volatile int* dead = &dead_flag;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* q_s = smem;                         // [tile][half][HD/64][128][64]
+    unsigned char* ring = q_s + TILES * Y::Q_ROOM;   // [stage][HD/64][64][64]
+    typename Y::Control& ctl = *reinterpret_cast<typename Y::Control*>(ring + STAGES * Y::STAGE);
+    uint64_t (&full)[STAGES] = ctl.full, (&empty)[STAGES] = ctl.empty, (&s_full)[2] = ctl.s_full, (&s_read)[2] = ctl.s_read, (&drained)[4] = ctl.drained;
+    uint64_t (&p_ready)[4] = ctl.p_ready, (&pv_done)[4] = ctl.pv_done;
+    float (&c2_s)[QB] = ctl.c2;
+    volatile int* dead = &ctl.dead;
+    if (smem_u32(smem) & 1023) {   // (the operands' swizzle counts from there; without static shared memory it is where the block's memory begins)
+        if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(err) = 5;
+        return;
+    }
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (known to be uniform)
     const int kvh = blockIdx.x % a.kv_heads;
@@ -266,7 +288,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
         for (int b = 0; b < NB; b++) tma_load_3d(ring + s * Y::STAGE + b * (TK * 128), map, b * 64, t0, kvh, &full[s]);
     };
     if (warp == Y::LOAD_WARP && lane == 0) {
-        dead_flag = 0;
+        ctl.dead = 0;
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&full[s], KIND == CACHE_Q4 ? 4 : 1);
             mbar_init(&empty[s], TILES);
@@ -291,7 +313,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     __syncwarp();
     if (warp == Y::MMA_WARP) {
         __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(Y::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_slot)), "r"(Y::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // The queries, as f16 in the A operand's layout: row r of a tile, 16-byte chunk c of a 64-column block at r * 128 + ((c ^ (r & 7)) * 16).
@@ -329,13 +351,23 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
                 e = e > 127 ? 0 : max(e, -100);
                 const float up = row0 + y0 + u <= row_last ? __uint_as_float((uint32_t)(8 - e + 127) << 23) : 0.f;
                 if (lane == u) c2 = rsqrtf((float)HD) * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 8 + 127) << 23);
-                __half2 h[N / 2];
+                __half2 h[N / 2], low[N / 2];   // x = h + low to 22 bits
 #pragma unroll
-                for (int v = 0; v < N / 2; v++) h[v] = __floats2half2_rn(x[k][u][2 * v] * up, x[k][u][2 * v + 1] * up);
+                for (int v = 0; v < N / 2; v++) {
+                    const float x0 = x[k][u][2 * v] * up, x1 = x[k][u][2 * v + 1] * up;
+                    h[v] = __floats2half2_rn(x0, x1);
+                    const float2 f = __half22float2(h[v]);
+                    low[v] = __floats2half2_rn(x0 - f.x, x1 - f.y);
+                }
                 const int c = lane * N / 8;
                 unsigned char* dst = q_s + y0 / QT * Y::Q_ROOM + (c >> 3) * (QT * 128) + (y0 % QT + u) * 128 + (((c & 7) ^ u) << 4) + (lane * N % 8) * 2;
-                if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
-                else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
+                if constexpr (N == 4) {
+                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
+                    *reinterpret_cast<uint2*>(dst + Y::Q_HALF) = *reinterpret_cast<uint2*>(low);
+                } else {
+                    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
+                    *reinterpret_cast<uint32_t*>(dst + Y::Q_HALF) = *reinterpret_cast<uint32_t*>(low);
+                }
             }
             if (lane < B) c2_s[y0 + lane] = c2;
         }
@@ -344,7 +376,7 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = ctl.tmem_slot;
 
     // (one instruction for all warps of a warpgroup, whatever their roles)
     if (warp >= Y::MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Y::OTHER_REGS));
@@ -472,6 +504,9 @@ __global__ void __launch_bounds__(Layout<KIND, HD>::THREADS, 2 / Layout<KIND, HD
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++)
                         if (leader) umma_ss(d, q_desc + ((k >> 2) * (QT * 128) + (k & 3) * 32) / 16, kb + ((k >> 2) * (TK * 128) + (k & 3) * 32) / 16, id, k > 0);
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++)   // and the low halves of the queries
+                        if (leader) umma_ss(d, q_desc + (Y::Q_HALF + (k >> 2) * (QT * 128) + (k & 3) * 32) / 16, kb + ((k >> 2) * (TK * 128) + (k & 3) * 32) / 16, id, 1);
                     if (leader) umma_commit(&s_full[t]);
                     done++;
                 }
@@ -759,8 +794,8 @@ int attn_long_tc_splits(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a) {
     return (int)best;
 }
 
-// 7 us (10 with the unpacking of 4-bit rows), the longer of the CTAs' steps, 1.15 us each (4 bits 1.3, with one tile 1.0), and the reading of the cache, and
-// for records 2.5 us and what it takes to write and read them.
+// 7 us (10 with the unpacking of 4-bit rows), the longer of the CTAs' steps, 1.15 us each (4 bits 1.3, with one tile 1.0; where the tensor cores are the
+// bound up to a fifth more, which is not where the choice is close), and the reading of the cache, and for records 2.5 us and what it takes to write and read them.
 double attn_long_tc_us(rlb_ctx* ctx, CacheKind kind, const AttnLongArgs& a, int splits) {
     const int tiles = kind == CACHE_Q4 ? 2 : 1;
     const int64_t rows = tiles * QT, ctas = (int64_t)a.kv_heads * (((int64_t)a.n * a.group + rows - 1) / rows), slots = (int64_t)ctx->sm_count * (2 / tiles);

@@ -272,11 +272,9 @@ def test_values_next_to_the_largest_f16(on, n):
         assert ((out.double() - want).abs() <= 2 * 2.0 ** -11 * want.abs()).all() and (out.double().abs() <= 65504).all()
 
 
-@pytest.mark.parametrize("on", [x for x in KERNELS if x[1] == "few" or x[0] == "f32"], ids="-".join, indirect=True)
-@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
 def test_queries_keep_their_low_halves(on, n):
-    """Two kinds of keys whose scores differ by what f16 queries would lose: the kernel for few rows, which holds 22 bits of them, tells them apart (and so
-    does f32). The tile kernel rounds queries to f16 and is not asked."""
+    """Two kinds of keys whose scores differ by what f16 queries would lose: every kernel holds 22 bits of them and tells them apart."""
     kind, cl = on
     heads, kv, hd, start = 4, 2, 128, 300
     total = start + n
