@@ -53,7 +53,7 @@ __device__ __forceinline__ __half q4_scale(float m) {
 // same integer unless it lies next to a half; only then is the quotient itself needed. (A correctly rounded division for every value is most of
 // the arithmetic of an append, which is then bound by it.) Adding 1.5 * 2^23 + 8 rounds to the nearest even and leaves the nibble in the lowest bits
 // of the sum; what stands above them is the same for all and is taken off the word once. (A rounding and a conversion to an integer for each value
-// kept that unit busy for 64 % of an append, at the same 40 us for 1792 rows and their reading back: memory's latency is the bound.)
+// kept that unit busy for 64 % of an append, at the same 40 us for 1792 rows and their reading back: latency beside 76 % of the issue slots now.)
 __device__ __forceinline__ uint32_t q4_pack(const float (&x)[8], float d) {
     if (!(d > 0.f)) return 0x88888888u;
     constexpr float kRound = 12582920.f;
